@@ -121,7 +121,8 @@ def _prepare_sample(c, g):
     dev, rows, n = "cuda", c["rows"], c["n"]
     # most of the vocabulary is unlikely, a few tokens stand out; some are forbidden
     logits = torch.randn(rows, n, generator=g, device=dev) * 2.5
-    top = torch.randint(0, n, (rows, 24), generator=g, device=dev)
+    # (24 places in each row, no place twice: which of two values a scatter leaves there is not determined)
+    top = (torch.randint(0, n, (rows, 1), generator=g, device=dev) + torch.arange(24, device=dev) * (n // 24)) % n
     logits.scatter_(1, top, 6 + 8 * torch.rand(rows, 24, generator=g, device=dev))
     logits[torch.rand(rows, n, generator=g, device=dev) < c["masked"]] = float("-inf")
     u = torch.rand(rows, 6, generator=g, device=dev)
