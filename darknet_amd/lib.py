@@ -68,6 +68,14 @@ SIGNATURES = {
     "forward_shortcut_gpu": (None, [V, V, V] + [i] * 7 + [f, f, i]),
     "forward_yolo_gpu": (None, [V, V] + [i] * 5),
     "forward_avgpool_gpu": (None, [V, V] + [i] * 4),
+    # ---- darknet_hip.h: row operators
+    "forward_rmsnorm_gpu": (i, [V] * 7 + [i, i, i, i, f]),
+    "q4_packed_bytes": (z, [i, i, i]), "q4_pack_codes_gpu": (i, [V, V, V, V, i, i, i]),
+    "q4_pack_weights_gpu": (i, [V, V, i, i, i]), "q4_unpack_weights_gpu": (i, [V, V, i, i, i]),
+    "connected_q4_workspace_bytes": (z, [i, i, i, i, i]),
+    "forward_connected_q4_gpu": (i, [V, i, V, i, V, V, V, i, i, i, i, i, i, V]),
+    "sample_workspace_bytes": (z, [i, i]),
+    "sample_rows_gpu": (i, [V, i, i, i, C.c_long, V, V, V, V, V, V, V, V]),
     # ---- darknet_amd.h: layer / network API
     "parse_network_cfg": (V, [C.c_char_p]), "load_network": (V, [C.c_char_p, C.c_char_p, i]),
     "load_weights": (None, [V, C.c_char_p]), "load_weights_upto": (None, [V, C.c_char_p, i, i]),

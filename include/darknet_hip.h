@@ -437,6 +437,83 @@ void forward_crop_gpu(const float *input, float *output, int batch, int c, int h
                       int out_w, int noadjust);
 
 /* ------------------------------------------------------------------------------------------
+ * Row operators: the steps a served model with 4-bit weights ends with - the norm in front of a
+ * product, the product, and the choice of a token from its scores.  No counterpart in the reference
+ * (its own forms of these steps: batchnorm and shortcut, the connected layer, softmax followed by
+ * sample_array, src/utils.c).
+ *
+ * Rows are dense unless a stride says otherwise.  `type` arguments take the codes below; parameters
+ * (scales, biases, settings of the sampling) are fp32 or int as written.  All buffers lie on the current
+ * device.  These calls allocate nothing and keep nothing from one call for the next: a call under
+ * stream capture is recorded like any other, and calls that overlap (two streams, two captured graphs) only need
+ * workspaces and outputs of their own.  The workspace needs no initial contents and is aligned to 16 bytes.
+ * They return 0, or -1 after a message on stderr when the arguments cannot be honoured: then nothing has
+ * been launched.  No rows (rows or batch 0) is a call that does nothing.
+ * ---------------------------------------------------------------------------------------- */
+enum { DN_F32 = 0, DN_F16, DN_BF16, DN_I8 };
+
+/* Root-mean-square norm of each row of [rows][n], with a residual added in front of it:
+ *   s = input + add                         (add may be NULL; the sum is rounded to `type`)
+ *   y = s / sqrt(mean(s^2) + eps) * scales  (scales: n floats, or NULL for ones)
+ *   sum_output  NULL, or where s goes (needs add)
+ *   output      NULL, or where y goes
+ *   q8_output   NULL, or where y goes in 8 bits, with q8_scales [rows][groups]: for each group of q8_group
+ *               values (32, 64 or 128; the last may be shorter; 0 = one group, the row) the scale
+ *               c = max|y| / 127 and the codes rint(y / c), ties to even, y being evaluated in 64 bits.
+ *               A group of zeros has c = 0; a group with a value that is not finite has c = NaN and
+ *               codes 0, so that what is computed from it is NaN too
+ * At least one of output and q8_output is given.  sum_output and output may each take the place of input
+ * or add (the same buffer, not one that overlaps it in part).  The sum of squares is held in 64 bits. */
+int forward_rmsnorm_gpu(const void *input, const void *add, const float *scales, void *sum_output, void *output,
+                        signed char *q8_output, float *q8_scales, int type, int rows, int n, int q8_group, float eps);
+
+/* Connected layer with 4-bit weights: output[b][o] = activation(biases[o] + sum_k input[b][k] * w[o][k]),
+ *   w[o][k] = (code[o][k] - zero[o][k / group]) * scale[o][k / group]       group = 32, 64 or 128
+ * (the last group of a row may be shorter).  The weights are laid out once, when they are loaded:
+ *   q4_packed_bytes       size of the packed copy; 0 for a geometry that is not served
+ *   q4_pack_codes_gpu     from weights that are 4-bit already: codes [outputs][(inputs + 1) / 2], the lower
+ *                         half of a byte is the even input; scales [outputs][groups]; zeros the same in
+ *                         bytes (0 .. 15), or NULL for 8 everywhere
+ *   q4_pack_weights_gpu   from [outputs][inputs] floats: each group's range, widened to hold zero, in 15 steps
+ *   q4_unpack_weights_gpu the values the packed copy stands for, [outputs][inputs] floats
+ * packed is aligned to 16 bytes.  input [batch][inputs] is fp32, fp16, bf16, or 8 bits with input_scales
+ * [batch][groups of input_group] (input_group: 0 = one scale a row, or `group`), as forward_rmsnorm_gpu
+ * writes them; input_scales and input_group are read for DN_I8 only.  biases may be NULL.  output
+ * [batch][outputs] is fp32, fp16 or bf16.  workspace: connected_q4_workspace_bytes() bytes (NULL if that
+ * is 0).  Every output is the same in every run.  A row of the input that holds a value that is not finite
+ * has NaN in all its outputs. */
+size_t q4_packed_bytes(int inputs, int outputs, int group);
+int q4_pack_codes_gpu(const unsigned char *codes, const float *scales, const unsigned char *zeros, void *packed,
+                      int inputs, int outputs, int group);
+int q4_pack_weights_gpu(const float *weights, void *packed, int inputs, int outputs, int group);
+int q4_unpack_weights_gpu(const void *packed, float *weights, int inputs, int outputs, int group);
+size_t connected_q4_workspace_bytes(int input_type, int batch, int inputs, int outputs, int group);
+int forward_connected_q4_gpu(const void *input, int input_type, const float *input_scales, int input_group,
+                             const void *packed, const float *biases, void *output, int output_type, int batch,
+                             int inputs, int outputs, int group, int activation, void *workspace);
+
+/* One token for each row of logits [rows][stride], of which the first n (up to 2^24) count, from the
+ * random number uniform[row] in [0, 1] (hip_random's are; one outside counts as the nearer end).  The tokens of
+ * a row are ordered by (logit descending, index ascending), w = exp((logit - largest) / temperature):
+ *   temperature   not above 0 (or NaN): the first token of the order; NULL: 1
+ *   top_k         the first top_k of the order; NULL, or not above 0: all
+ *   top_p         the shortest run of first tokens whose mass is at least top_p times the mass top_k left (one
+ *                 at least); NULL, or not below 1: all
+ *   min_p         of these the tokens with w >= min_p; NULL, or not above 0: all; above 1 counts as 1
+ *   tokens        the first token in index order at which the running mass of what is kept reaches
+ *                 uniform * (mass kept), as sample_array draws (src/utils.c)
+ *   probs         NULL, or the token's share of the mass kept
+ * Each array holds one value for each row, on the device.  NaN and -inf logits are never drawn; a row of
+ * nothing else gives token -1 and probability 0.  If the largest logit is +inf the tokens that have it are
+ * equally likely.  Masses are held as whole numbers of at least 38 bits below the largest token's, so sums do not
+ * depend on their order: the same row gives the same token in every run and at every place in a batch.
+ * workspace: sample_workspace_bytes() bytes (NULL if that is 0). */
+size_t sample_workspace_bytes(int rows, int n);
+int sample_rows_gpu(const void *logits, int type, int rows, int n, long stride, const float *temperature,
+                    const int *top_k, const float *top_p, const float *min_p, const float *uniform, int *tokens,
+                    float *probs, void *workspace);
+
+/* ------------------------------------------------------------------------------------------
  * Input side.  Images are [c][h][w] floats as the reference's `image` (include/darknet.h:508).
  * ---------------------------------------------------------------------------------------- */
 
