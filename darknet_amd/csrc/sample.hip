@@ -35,7 +35,7 @@ struct sample_args {
     float *probs;
     unsigned char *workspace;
     long stride;
-    int rows, n, segments, length; /* length: tokens of a segment */
+    int rows, n, segments, length, block; /* length: tokens of a segment, block: of what its mass is summed over */
 };
 
 /* A row's settings, those that are off in one form. */
@@ -453,47 +453,88 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
 }
 
 /* ---- longer rows: cut into segments, four passes ---------------------------------------------------------
- * 1 largest of each segment   2 bins of each segment (rows with top-k or top-p)
- * 3 borders from the bins of all segments; each segment's kept mass and its candidates
- * 4 one workgroup a row: the prefix' end among the candidates, the segment that the draw falls into, the token */
+ * 1 largest of each segment (and the row's bins cleared)
+ * 2 bins of the row, rows with top-k or top-p only: each segment's in LDS, then added to the row's
+ * 3 borders from the bins; the kept mass of each block of tokens and each segment's candidates
+ * 4 one workgroup a row: the prefix' end among the candidates, the block that the draw falls into, the token */
+#define SM_SPLIT_THREADS 256
+#define SM_STRIP (SM_SPLIT_THREADS * 8) /* tokens that a workgroup takes at a time */
+#define SM_BLOCKS 512                   /* of a row, at most: they are summed in LDS */
+#define SM_LISTED 512                   /* candidates that a segment keeps a list of */
+
 struct sample_space {
-    size_t largest, kept, found, bins_mass, bins_count, border, list, bytes;
+    size_t kept, bins_mass, border, list, bins_count, largest, found, bytes;
 };
 
-__host__ __device__ static inline sample_space space_of(int rows, int segments, int length)
+__host__ __device__ static inline sample_space space_of(int rows, int segments)
 {
     sample_space w;
     const size_t all = (size_t)rows * segments;
     w.kept = 0;
-    w.bins_mass = w.kept + all * 8;
-    w.border = w.bins_mass + all * SM_BINS * 8;
-    w.bins_count = w.border + (size_t)rows * sizeof(sample_border);
-    w.largest = w.bins_count + all * SM_BINS * 4;
+    w.bins_mass = w.kept + (size_t)rows * SM_BLOCKS * 8;
+    w.border = w.bins_mass + (size_t)rows * SM_BINS * 8;
+    w.list = w.border + (size_t)rows * sizeof(sample_border);
+    w.bins_count = w.list + all * SM_LISTED * 8;
+    w.largest = w.bins_count + (size_t)rows * SM_BINS * 4;
     w.found = w.largest + all * 4;
-    w.list = w.found + all * 4;
-    w.bytes = w.list + all * (size_t)length * 4;
+    w.bytes = w.found + all * 4;
     return w;
 }
 
-#define SM_SPLIT_THREADS 256
+/* Eight neighbouring tokens from i on; -inf behind `end`. */
+template <int T>
+__device__ __forceinline__ void load8(const typename dn_elt<T>::store *x, int i, int end, bool vectors, float l[8])
+{
+    typedef typename dn_elt<T>::store S;
+    typedef S S4 __attribute__((ext_vector_type(4)));
+    if (vectors && i + 8 <= end) {
+        const S4 u = *(const S4 *)(x + i), v = *(const S4 *)(x + i + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            l[e] = (float)u[e];
+            l[e + 4] = (float)v[e];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) l[e] = i + e < end ? (float)x[i + e] : -INFINITY;
+    }
+}
+
+template <int T>
+__device__ __forceinline__ bool rows_aligned(const sample_args &a)
+{
+    const int size = sizeof(typename dn_elt<T>::store);
+    return ((uintptr_t)a.logits & 15) == 0 && ((a.stride * size) & 15) == 0;
+}
 
 template <int T>
 __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_largest_kernel(sample_args a)
 {
     typedef typename dn_elt<T>::store S;
     __shared__ float part[SM_SPLIT_THREADS / 64];
-    const sample_space ws = space_of(a.rows, a.segments, a.length);
+    const sample_space ws = space_of(a.rows, a.segments);
+    const bool vectors = rows_aligned<T>(a);
     for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
         const S *x = (const S *)a.logits + row * a.stride;
         const int lo = blockIdx.x * a.length, hi = min(a.n, lo + a.length);
         float m = -INFINITY;
-        for (int i = lo + threadIdx.x; i < hi; i += SM_SPLIT_THREADS) m = (float)x[i] > m ? (float)x[i] : m;
+        for (int i = lo + threadIdx.x * 8; i < hi; i += SM_STRIP) {
+            float l[8];
+            load8<T>(x, i, hi, vectors, l);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = l[e] > m ? l[e] : m;
+        }
         m = dn_wave_max(m);
         __syncthreads();
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
         __syncthreads();
         if (threadIdx.x == 0)
             ((float *)(a.workspace + ws.largest))[row * a.segments + blockIdx.x] = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+        if (blockIdx.x == 0)
+            for (int i = threadIdx.x; i < SM_BINS; i += SM_SPLIT_THREADS) {
+                ((u64 *)(a.workspace + ws.bins_mass))[row * SM_BINS + i] = 0;
+                ((unsigned *)(a.workspace + ws.bins_count))[row * SM_BINS + i] = 0;
+            }
     }
 }
 
@@ -510,7 +551,8 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_bins_kernel(sample_ar
     typedef typename dn_elt<T>::store S;
     __shared__ u64 mass[SM_BINS];
     __shared__ unsigned count[SM_BINS];
-    const sample_space ws = space_of(a.rows, a.segments, a.length);
+    const sample_space ws = space_of(a.rows, a.segments);
+    const bool vectors = rows_aligned<T>(a);
     const int tid = threadIdx.x;
     for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
         const sample_row r = settings_of(a, row);
@@ -524,18 +566,21 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_bins_kernel(sample_ar
             count[i] = 0;
         }
         __syncthreads();
-        for (int i = lo + tid; i < hi; i += SM_SPLIT_THREADS) {
-            const float l = (float)x[i];
-            if (!(l > -INFINITY)) continue;
-            const int b = bin_of(l, largest, r);
-            if (r.k) atomicAdd(&count[b], 1u);
-            if (r.p < 1) atomicAdd(&mass[b], mass_of(weight_of(l, largest, r)));
+        for (int i = lo + tid * 8; i < hi; i += SM_STRIP) {
+            float l[8];
+            load8<T>(x, i, hi, vectors, l);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (!(l[e] > -INFINITY)) continue;
+                const int b = bin_of(l[e], largest, r);
+                if (r.k) atomicAdd(&count[b], 1u);
+                if (r.p < 1) atomicAdd(&mass[b], mass_of(weight_of(l[e], largest, r)));
+            }
         }
         __syncthreads();
-        const size_t at = ((size_t)row * a.segments + blockIdx.x) * SM_BINS;
         for (int i = tid; i < SM_BINS; i += SM_SPLIT_THREADS) {
-            ((u64 *)(a.workspace + ws.bins_mass))[at + i] = mass[i];
-            ((unsigned *)(a.workspace + ws.bins_count))[at + i] = count[i];
+            if (mass[i]) atomicAdd((u64 *)(a.workspace + ws.bins_mass) + row * SM_BINS + i, mass[i]);
+            if (count[i]) atomicAdd((unsigned *)(a.workspace + ws.bins_count) + row * SM_BINS + i, count[i]);
         }
     }
 }
@@ -546,24 +591,17 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_kept_kernel(sample_ar
     typedef typename dn_elt<T>::store S;
     __shared__ sample_lds s;
     __shared__ unsigned s_count;
-    const sample_space ws = space_of(a.rows, a.segments, a.length);
+    const sample_space ws = space_of(a.rows, a.segments);
+    const bool vectors = rows_aligned<T>(a);
     const int tid = threadIdx.x;
     for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
         const sample_row r = settings_of(a, row);
         const float largest = row_largest(a, ws, row);
-        const bool cut = r.k || r.p < 1;
         __syncthreads();
-        if (cut)
+        if (r.k || r.p < 1)
             for (int i = tid; i < SM_BINS; i += SM_SPLIT_THREADS) {
-                u64 m = 0;
-                unsigned c = 0;
-                for (int g = 0; g < a.segments; ++g) {
-                    const size_t at = ((size_t)row * a.segments + g) * SM_BINS + i;
-                    m += ((const u64 *)(a.workspace + ws.bins_mass))[at];
-                    c += ((const unsigned *)(a.workspace + ws.bins_count))[at];
-                }
-                s.mass[i] = m;
-                s.count[i] = c;
+                s.mass[i] = ((const u64 *)(a.workspace + ws.bins_mass))[row * SM_BINS + i];
+                s.count[i] = ((const unsigned *)(a.workspace + ws.bins_count))[row * SM_BINS + i];
             }
         if (tid == 0) s_count = 0;
         __syncthreads();
@@ -578,39 +616,47 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_kept_kernel(sample_ar
         const sample_border b = s.border;
         const S *x = (const S *)a.logits + row * a.stride;
         const int lo = blockIdx.x * a.length, hi = min(a.n, lo + a.length);
-        int *list = (int *)(a.workspace + ws.list) + ((size_t)row * a.segments + blockIdx.x) * a.length;
-        u64 own = 0;
-        for (int i = lo + tid; i < hi; i += SM_SPLIT_THREADS) {
-            const float l = (float)x[i];
-            if (!(l > -INFINITY)) continue;
-            const int bin = bin_of(l, largest, r);
-            if (bin < b.first) {
-                const double w = weight_of(l, largest, r);
-                if (w >= r.floor) own += mass_of(w);
-            } else if (is_candidate(b, bin)) {
-                list[atomicAdd(&s_count, 1u)] = i;
+        u64 *list = (u64 *)(a.workspace + ws.list) + ((size_t)row * a.segments + blockIdx.x) * SM_LISTED;
+        for (int from = lo; from < hi; from += a.block) {
+            u64 own = 0;
+            const int to = min(hi, from + a.block);
+            for (int i = from + tid * 8; i < to; i += SM_STRIP) {
+                float l[8];
+                load8<T>(x, i, to, vectors, l);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (!(l[e] > -INFINITY)) continue;
+                    const int bin = bin_of(l[e], largest, r);
+                    if (bin < b.first) {
+                        const double w = weight_of(l[e], largest, r);
+                        if (w >= r.floor) own += mass_of(w);
+                    } else if (is_candidate(b, bin)) {
+                        const unsigned at = atomicAdd(&s_count, 1u);
+                        if (at < SM_LISTED) list[at] = place_of(l[e], i + e);
+                    }
+                }
             }
+            const u64 kept = block_sum(own, s);
+            if (tid == 0) ((u64 *)(a.workspace + ws.kept))[row * SM_BLOCKS + from / a.block] = kept;
         }
-        const u64 kept = block_sum(own, s);
-        if (tid == 0) {
-            ((u64 *)(a.workspace + ws.kept))[row * a.segments + blockIdx.x] = kept;
-            ((int *)(a.workspace + ws.found))[row * a.segments + blockIdx.x] = (int)s_count;
-        }
+        __syncthreads();
+        if (tid == 0) ((int *)(a.workspace + ws.found))[row * a.segments + blockIdx.x] = (int)s_count;
     }
 }
 
 template <int T>
-__global__ __launch_bounds__(1024) void sample_draw_kernel(sample_args a)
+__global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_draw_kernel(sample_args a)
 {
     typedef typename dn_elt<T>::store S;
     __shared__ sample_lds s;
     __shared__ u64 candidates[SM_CANDIDATES];
-    __shared__ u64 s_kept[SM_SEGMENTS];
-    __shared__ int s_from[SM_SEGMENTS + 1];
-    __shared__ u64 s_before, s_total;
-    __shared__ int s_segment;
-    const sample_space ws = space_of(a.rows, a.segments, a.length);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ u64 s_kept[SM_BLOCKS];
+    __shared__ int s_from[SM_SEGMENTS + 1], s_listed;
+    __shared__ u64 s_before;
+    __shared__ int s_block;
+    const sample_space ws = space_of(a.rows, a.segments);
+    const bool vectors = rows_aligned<T>(a);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, blocks = (a.n + a.block - 1) / a.block;
     for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const sample_row r = settings_of(a, row);
         const float largest = row_largest(a, ws, row);
@@ -620,98 +666,112 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(sample_args a)
         }
         const S *x = (const S *)a.logits + row * a.stride;
         const sample_border b = ((const sample_border *)(a.workspace + ws.border))[row];
-        const int *lists = (const int *)(a.workspace + ws.list) + (size_t)row * a.segments * a.length;
         __syncthreads();
+        for (int i = tid; i < SM_BLOCKS; i += SM_SPLIT_THREADS)
+            s_kept[i] = i < blocks ? ((const u64 *)(a.workspace + ws.kept))[row * SM_BLOCKS + i] : 0;
         if (wave == 0) {
             const int c = lane < a.segments ? ((const int *)(a.workspace + ws.found))[row * a.segments + lane] : 0;
             const int upto = (int)wave_scan((u64)c, lane);
-            if (lane < a.segments) {
-                s_kept[lane] = ((const u64 *)(a.workspace + ws.kept))[row * a.segments + lane];
-                s_from[lane + 1] = upto;
-            }
+            if (lane < a.segments) s_from[lane + 1] = upto;
             if (lane == 0) s_from[0] = 0;
+            const bool whole = __all(c <= SM_LISTED);
+            if (lane == 63) s_listed = whole && upto <= SM_CANDIDATES;
         }
         __syncthreads();
         const int count = s_from[a.segments];
         u64 last = 0;
         if (count) {
-            auto listed = [&](auto f) {
-                for (int g = wave; g < a.segments; g += 16) {
-                    const int c = s_from[g + 1] - s_from[g];
-                    for (int j = lane; j < c; j += 64) {
-                        const int i = lists[(size_t)g * a.length + j];
-                        f(place_of((float)x[i], i), s_from[g] + j);
-                    }
-                }
-            };
-            auto keep = [&](u64 c) {
-                const double w = weight_of(logit_of(c), largest, r);
-                if (c >= last && w >= r.floor) atomicAdd(&s_kept[(int)(0xffffffffu - (unsigned)c) / a.length], mass_of(w));
-            };
-            const bool fits = count <= SM_CANDIDATES;
+            const bool fits = s_listed;
             if (fits) {
-                listed([&](u64 c, int at) { candidates[at] = c; });
+                for (int g = wave; g < a.segments; g += SM_SPLIT_THREADS / 64) {
+                    const u64 *list = (const u64 *)(a.workspace + ws.list) + ((size_t)row * a.segments + g) * SM_LISTED;
+                    for (int j = lane; j < s_from[g + 1] - s_from[g]; j += 64) candidates[s_from[g] + j] = list[j];
+                }
                 __syncthreads();
             }
             auto each = [&](auto f) {
-                if (fits)
-                    for (int i = tid; i < count; i += 1024) f(candidates[i]);
-                else
-                    listed([&](u64 c, int) { f(c); });
+                if (fits) {
+                    for (int i = tid; i < count; i += SM_SPLIT_THREADS) f(candidates[i]);
+                    return;
+                }
+                for (int i = tid * 8; i < a.n; i += SM_STRIP) { /* too many for the lists: from the row again */
+                    float l[8];
+                    load8<T>(x, i, a.n, vectors, l);
+                    for (int e = 0; e < 8; ++e)
+                        if (l[e] > -INFINITY && is_candidate(b, bin_of(l[e], largest, r))) f(place_of(l[e], i + e));
+                }
             };
             last = last_place(each, b, r, largest, s);
-            each(keep);
+            each([&](u64 c) {
+                if (c < last) return;
+                const double w = weight_of(logit_of(c), largest, r);
+                if (w >= r.floor) atomicAdd(&s_kept[(int)(0xffffffffu - (unsigned)c) / a.block], mass_of(w));
+            });
         }
         __syncthreads();
-        if (wave == 0) {
-            const u64 own = lane < a.segments ? s_kept[lane] : 0, incl = wave_scan(own, lane);
-            const u64 total = __shfl(incl, 63, 64);
-            const double target = draw_target(a, row, total);
-            const u64 any = __ballot(own && (double)incl >= target);
-            if (lane == __ffsll((unsigned long long)any) - 1) {
-                s_segment = lane;
-                s_before = incl - own;
-                s_total = total;
-            }
-        }
-        __syncthreads();
-        /* the segment, each lane a piece of it */
-        const u64 total = s_total;
-        const double target = draw_target(a, row, total);
-        const int piece = (a.length + 1023) / 1024, lo = min(a.n, s_segment * a.length + tid * piece);
-        const int hi = min(min(a.n, (s_segment + 1) * a.length), lo + piece);
-        auto kept_mass = [&](int i) {
-            const float l = (float)x[i];
-            const u64 c = place_of(l, i);
-            if (!c || c < last) return (u64)0;
-            const double w = weight_of(l, largest, r);
-            return w >= r.floor ? mass_of(w) : (u64)0;
-        };
         u64 own = 0, run;
-        for (int i = lo; i < hi; ++i) own += kept_mass(i);
-        if (reaches(own, s_before, target, run, s)) {
-            for (int i = lo; i < hi; ++i) {
-                const u64 m = kept_mass(i);
-                run += m;
-                if (m && (double)run >= target) {
-                    answer(a, row, i, m, total);
-                    break;
+        constexpr int E = SM_BLOCKS / SM_SPLIT_THREADS;
+#pragma unroll
+        for (int e = 0; e < E; ++e) own += s_kept[tid * E + e];
+        const u64 total = block_sum(own, s);
+        const double target = draw_target(a, row, total);
+        if (reaches(own, 0, target, run, s)) {
+            int at = tid * E;
+            while ((double)(run + s_kept[at]) < target) run += s_kept[at++];
+            s_block = at;
+            s_before = run;
+        }
+        __syncthreads();
+        /* the block, a strip at a time, eight tokens a lane */
+        run = s_before;
+        const int lo = s_block * a.block, hi = min(a.n, lo + a.block);
+        for (int from = lo; from < hi; from += SM_STRIP) {
+            const int i = from + tid * 8;
+            float l[8];
+            u64 m[8], before;
+            load8<T>(x, i, hi, vectors, l);
+            own = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const u64 c = place_of(l[e], i + e);
+                m[e] = 0;
+                if (c && c >= last) {
+                    const double w = weight_of(l[e], largest, r);
+                    if (w >= r.floor) m[e] = mass_of(w);
                 }
+                own += m[e];
+            }
+            if (reaches(own, run, target, before, s)) {
+                bool done = false;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    before += m[e];
+                    if (!done && m[e] && (double)before >= target) {
+                        answer(a, row, i + e, m[e], total);
+                        done = true;
+                    }
+                }
+            }
+            if (from + SM_STRIP < hi) {
+                run += block_sum(own, s);
+                if ((double)run >= target) break;
             }
         }
     }
 }
 
 /* Rows of up to 16384 tokens take one workgroup each.  Longer ones are cut so that about 1024 workgroups have a
- * share, of 1024 tokens at least. */
+ * share of one block of tokens at least. */
 static bool sample_in_one(int n) { return n <= 16384; }
 
 static void sample_cut(sample_args &a)
 {
+    a.block = (int)(((long)a.n + (long)SM_STRIP * SM_BLOCKS - 1) / ((long)SM_STRIP * SM_BLOCKS)) * SM_STRIP;
+    const int blocks = (a.n + a.block - 1) / a.block;
     int segments = 1;
-    while (segments < SM_SEGMENTS && (long)a.rows * segments < 1024 && a.n / (segments * 2) >= 1024) segments *= 2;
+    while (segments < SM_SEGMENTS && (long)a.rows * segments < 1024 && segments * 2 <= blocks) segments *= 2;
     a.segments = segments;
-    a.length = ((a.n + segments - 1) / segments + 7) / 8 * 8;
+    a.length = (blocks + segments - 1) / segments * a.block;
 }
 
 extern "C" size_t sample_workspace_bytes(int rows, int n)
@@ -721,7 +781,7 @@ extern "C" size_t sample_workspace_bytes(int rows, int n)
     a.rows = rows;
     a.n = n;
     sample_cut(a);
-    return space_of(rows, a.segments, a.length).bytes;
+    return space_of(rows, a.segments).bytes;
 }
 
 template <int T>
@@ -738,7 +798,7 @@ static void sample_launch(const sample_args &a)
     hipLaunchKernelGGL((sample_largest_kernel<T>), grid, block, 0, dn_stream(), a);
     if (a.top_k || a.top_p || a.temperature) hipLaunchKernelGGL((sample_bins_kernel<T>), grid, block, 0, dn_stream(), a);
     hipLaunchKernelGGL((sample_kept_kernel<T>), grid, block, 0, dn_stream(), a);
-    hipLaunchKernelGGL((sample_draw_kernel<T>), dim3(a.rows < 65535 ? a.rows : 65535), dim3(1024), 0, dn_stream(), a);
+    hipLaunchKernelGGL((sample_draw_kernel<T>), dim3(a.rows < 65535 ? a.rows : 65535), block, 0, dn_stream(), a);
 }
 
 extern "C" int sample_rows_gpu(const void *logits, int type, int rows, int n, long stride, const float *temperature,
@@ -758,7 +818,7 @@ extern "C" int sample_rows_gpu(const void *logits, int type, int rows, int n, lo
     if (!workspace && !sample_in_one(n)) return dn_refuse(me, "the workspace is missing");
     hip_require_device(me);
     sample_args a = {logits, temperature, top_p, min_p, uniform, top_k, tokens, probs, (unsigned char *)workspace,
-                     stride, rows, n, 1, n};
+                     stride, rows, n, 1, n, n};
     if (!sample_in_one(n)) sample_cut(a);
     if (type == DN_F32) sample_launch<DN_F32>(a);
     else if (type == DN_F16) sample_launch<DN_F16>(a);
