@@ -250,13 +250,6 @@ __device__ __forceinline__ unsigned q4_largest4(unsigned m, const float x[4])
     return m;
 }
 
-__device__ __forceinline__ unsigned q4_wave_largest(unsigned m)
-{
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
-    return m;
-}
-
 /* The operand form of four inputs: hi, and what it leaves of the value in lo. */
 __device__ __forceinline__ void q4_split4(const float x[4], int shift, half4_t &hi, half4_t &lo)
 {
@@ -409,7 +402,7 @@ __global__ __launch_bounds__(Q4_THREADS) void q4_direct_kernel(q4_args a)
                 q4_load4<TI>((const char *)a.input + b * row_bytes, k, a.s.inputs, vectors, x);
                 m = q4_largest4(m, x);
             }
-            m = q4_wave_largest(m);
+            m = dn_wave_max(m);
             if (lane == 0) s_largest[b][wave] = m;
         }
         __syncthreads();
@@ -500,7 +493,7 @@ __global__ __launch_bounds__(256) void q4_prepare_kernel(q4_args a)
             q4_load4<TI>(row, k, a.s.inputs, vectors, x);
             m = q4_largest4(m, x);
         }
-        m = q4_wave_largest(m);
+        m = dn_wave_max(m);
         if ((tid & 63) == 0) s_largest[tid >> 6] = m;
         __syncthreads();
         shift = q4_row_shift(max(max(s_largest[0], s_largest[1]), max(s_largest[2], s_largest[3])));

@@ -31,32 +31,78 @@ static inline int dn_type_bytes(int type) { return type == DN_F32 ? 4 : type == 
 static inline bool dn_is_float_type(int type) { return type == DN_F32 || type == DN_F16 || type == DN_BF16; }
 static inline bool dn_aligned(const void *p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
-__device__ __forceinline__ double dn_wave_sum(double v)
+/* Reductions and running sums over the 64 lanes by data-parallel-primitive moves between registers (rows of 16
+ * lanes, then row 0 to 1 and 2 to 3, then the lower half to the upper): a quarter of the time of the shuffles, which
+ * go through the LDS crossbar.  All 64 lanes must be active.  Lanes without a source take `none`. */
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned dn_move(unsigned none, unsigned v)
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return (unsigned)__builtin_amdgcn_update_dpp((int)none, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long dn_move(unsigned long long none, unsigned long long v)
+{
+    const unsigned lo = dn_move<CTRL, ROWS>((unsigned)none, (unsigned)v);
+    const unsigned hi = dn_move<CTRL, ROWS>((unsigned)(none >> 32), (unsigned)(v >> 32));
+    return (unsigned long long)hi << 32 | lo;
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dn_move(double none, double v)
+{
+    return __longlong_as_double((long long)dn_move<CTRL, ROWS>((unsigned long long)__double_as_longlong(none),
+                                                              (unsigned long long)__double_as_longlong(v)));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dn_move(float none, float v)
+{
+    return __uint_as_float(dn_move<CTRL, ROWS>(__float_as_uint(none), __float_as_uint(v)));
+}
+
+/* The running result of op in lane order, from lane 0 to each lane. */
+template <class T, class Op>
+__device__ __forceinline__ T dn_wave_scan(T v, T none, Op op)
+{
+    v = op(v, dn_move<0x111, 0xf>(none, v));
+    v = op(v, dn_move<0x112, 0xf>(none, v));
+    v = op(v, dn_move<0x114, 0xf>(none, v));
+    v = op(v, dn_move<0x118, 0xf>(none, v));
+    v = op(v, dn_move<0x142, 0xa>(none, v));
+    v = op(v, dn_move<0x143, 0xc>(none, v));
     return v;
 }
 
+__device__ __forceinline__ unsigned dn_lane(unsigned v, int lane) { return (unsigned)__builtin_amdgcn_readlane((int)v, lane); }
+__device__ __forceinline__ unsigned long long dn_lane(unsigned long long v, int lane)
+{
+    return (unsigned long long)dn_lane((unsigned)(v >> 32), lane) << 32 | dn_lane((unsigned)v, lane);
+}
+__device__ __forceinline__ double dn_lane(double v, int lane)
+{
+    return __longlong_as_double((long long)dn_lane((unsigned long long)__double_as_longlong(v), lane));
+}
+__device__ __forceinline__ float dn_lane(float v, int lane) { return __uint_as_float(dn_lane(__float_as_uint(v), lane)); }
+
+template <class T>
+__device__ __forceinline__ T dn_wave_sum(T v)
+{
+    return dn_lane(dn_wave_scan(v, (T)0, [](T a, T b) { return a + b; }), 63);
+}
 __device__ __forceinline__ double dn_wave_max(double v)
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
-    return v;
+    return dn_lane(dn_wave_scan(v, v, [](double a, double b) { return fmax(a, b); }), 63);
 }
-
 __device__ __forceinline__ float dn_wave_max(float v)
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+    return dn_lane(dn_wave_scan(v, v, [](float a, float b) { return fmaxf(a, b); }), 63);
 }
-
-__device__ __forceinline__ unsigned long long dn_wave_sum(unsigned long long v)
+__device__ __forceinline__ unsigned dn_wave_max(unsigned v)
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+    return dn_lane(dn_wave_scan(v, v, [](unsigned a, unsigned b) { return a > b ? a : b; }), 63);
+}
+__device__ __forceinline__ unsigned long long dn_wave_max(unsigned long long v)
+{
+    typedef unsigned long long u64;
+    return dn_lane(dn_wave_scan(v, v, [](u64 a, u64 b) { return a > b ? a : b; }), 63);
 }
 
 #endif

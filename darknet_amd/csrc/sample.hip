@@ -42,24 +42,30 @@ struct sample_args {
 struct sample_row {
     double log2_per_logit; /* log2(e) / T */
     double floor;          /* min-p */
+    double uniform;        /* in 0 .. 1 */
     float bins_per_logit;
     float p;               /* 2: off */
     int k;                 /* 0: off */
 };
 
+/* Every array is read, a missing one at another's place, so that the loads are in flight together. */
 __device__ __forceinline__ sample_row settings_of(const sample_args &a, long row)
 {
     sample_row s;
-    float t = a.temperature ? a.temperature[row] : 1.f;
-    int k = a.top_k ? a.top_k[row] : 0;
+    const float t_of = (a.temperature ? a.temperature : a.uniform)[row], p_of = (a.top_p ? a.top_p : a.uniform)[row];
+    const float m_of = (a.min_p ? a.min_p : a.uniform)[row];
+    const int k_of = (a.top_k ? a.top_k : (const int *)a.uniform)[row];
+    const float u = a.uniform[row];
+    float t = a.temperature ? t_of : 1.f;
+    int k = a.top_k ? k_of : 0;
     if (!(t > 0)) { /* the first of the order */
         t = 1;
         k = 1;
     }
     s.k = k > 0 && k < a.n ? k : 0;
-    const float p = a.top_p ? a.top_p[row] : 2.f, m = a.min_p ? a.min_p[row] : 0.f;
-    s.p = p < 1 ? p : 2.f;
-    s.floor = m > 0 ? (double)fminf(m, 1.f) : 0.;
+    s.p = a.top_p && p_of < 1 ? p_of : 2.f;
+    s.floor = a.min_p && m_of > 0 ? (double)fminf(m_of, 1.f) : 0.;
+    s.uniform = u > 0 ? (double)fminf(u, 1.f) : 0.;
     s.log2_per_logit = 1.4426950408889634 / (double)t;
     s.bins_per_logit = fminf(SM_PER_T / t, 3.402823466e38f);
     return s;
@@ -121,24 +127,30 @@ struct sample_border {
 };
 
 struct sample_lds {
-    u64 mass[SM_BINS];
-    unsigned count[SM_BINS];
-    u64 digit[256], part[16];
+    u64 mass[SM_BINS + 64];
+    unsigned count[SM_BINS + 64];
+    u64 digit[256 + 64], part[16];
     unsigned digit_count[256];
     u64 prefix, base, found;
     unsigned single;
     sample_border border;
 };
 
-__device__ __forceinline__ u64 wave_scan(u64 v, int lane)
+template <class V>
+__device__ __forceinline__ V wave_scan(V v)
 {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const u64 u = __shfl_up(v, o, 64);
-        if (lane >= o) v += u;
-    }
-    return v;
+    return dn_wave_scan(v, (V)0, [](V a, V b) { return a + b; });
 }
+
+/* Where bin b stands in LDS: a gap after every E bins spreads the runs of E that the lanes read over the banks. */
+template <int E>
+__device__ __forceinline__ int slot_of(int b)
+{
+    return b + b / E;
+}
+#define SM_SLOTS (SM_BINS + 64)
+__device__ __forceinline__ int bin_slot(int b) { return slot_of<SM_BINS / 64>(b); }
+__device__ __forceinline__ int digit_slot(int d) { return slot_of<4>(d); }
 
 /* One wave: the first of N bins (in order, or from the last one down) at which base + running sum reaches the
  * target, and the sum before it; N if none does.  The target is at least 1. */
@@ -150,10 +162,10 @@ __device__ __forceinline__ int find_bin(const V *bins, u64 base, double target, 
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int b = lane * E + e;
-        v[e] = bins[DOWN ? N - 1 - b : b];
+        v[e] = bins[slot_of<E>(DOWN ? N - 1 - b : b)];
         own += v[e];
     }
-    u64 run = base + wave_scan(own, lane) - own;
+    u64 run = base + wave_scan(own) - own;
     int at = N;
     u64 sum = 0;
 #pragma unroll
@@ -169,9 +181,9 @@ __device__ __forceinline__ int find_bin(const V *bins, u64 base, double target, 
         before = 0;
         return N;
     }
-    const int src = __ffsll((unsigned long long)any) - 1;
-    before = __shfl(sum, src, 64);
-    at = __shfl(at, src, 64);
+    const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)any) - 1);
+    before = dn_lane(sum, src);
+    at = (int)dn_lane((unsigned)at, src);
     return DOWN ? N - 1 - at : at;
 }
 
@@ -190,10 +202,10 @@ __device__ __forceinline__ sample_border border_of(const sample_lds &s, const sa
 #pragma unroll
         for (int e = 0; e < SM_BINS / 64; ++e) {
             const int at = lane * (SM_BINS / 64) + e;
-            if (b.k_bin < 0 || at < b.k_bin) own_mass += s.mass[at];
+            if (b.k_bin < 0 || at < b.k_bin) own_mass += s.mass[bin_slot(at)];
         }
         mass_least = dn_wave_sum(own_mass);
-        mass_most = b.k_bin < 0 ? mass_least : mass_least + s.mass[b.k_bin];
+        mass_most = b.k_bin < 0 ? mass_least : mass_least + s.mass[bin_slot(b.k_bin)];
         b.mass_k = mass_least;
     }
     if (r.p < 1) {
@@ -247,11 +259,8 @@ __device__ __forceinline__ u64 find_place(Each each, Value value, u64 base, doub
         most = c > most ? c : most;
         least = c < least ? c : least;
     });
-    for (int o = 32; o > 0; o >>= 1) {
-        const u64 m = __shfl_xor(most, o, 64), l = __shfl_xor(least, o, 64);
-        most = m > most ? m : most;
-        least = l < least ? l : least;
-    }
+    most = dn_wave_max(most);
+    least = ~dn_wave_max(~least);
     __syncthreads();
     if (tid == 0) {
         s.prefix = 0;
@@ -272,14 +281,14 @@ __device__ __forceinline__ u64 find_place(Each each, Value value, u64 base, doub
         const int next = bit > 8 ? bit - 8 : 0;
         __syncthreads();
         if (tid < 256) {
-            s.digit[tid] = 0;
+            s.digit[digit_slot(tid)] = 0;
             s.digit_count[tid] = 0;
         }
         __syncthreads();
         each([&](u64 c) {
             if (shift_right(c, bit) != prefix) return;
             const int d = (int)(c >> next) & ((1 << (bit - next)) - 1);
-            atomicAdd(&s.digit[d], value(c));
+            atomicAdd(&s.digit[digit_slot(d)], value(c));
             atomicAdd(&s.digit_count[d], 1u);
         });
         __syncthreads();
@@ -337,7 +346,7 @@ __device__ __forceinline__ u64 last_place(Each each, const sample_border &b, con
 __device__ __forceinline__ bool reaches(u64 own, u64 base, double target, u64 &before, sample_lds &s)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const u64 incl = wave_scan(own, lane);
+    const u64 incl = wave_scan(own);
     __syncthreads();
     if (lane == 63) s.part[wave] = incl;
     __syncthreads();
@@ -347,11 +356,7 @@ __device__ __forceinline__ bool reaches(u64 own, u64 base, double target, u64 &b
     return own && (double)run < target && (double)(run + own) >= target;
 }
 
-__device__ __forceinline__ double draw_target(const sample_args &a, long row, u64 total)
-{
-    const double u = a.uniform[row];
-    return fmax((u > 0 ? fmin(u, 1.) : 0.) * (double)total, 1.);
-}
+__device__ __forceinline__ double draw_target(const sample_row &r, u64 total) { return fmax(r.uniform * (double)total, 1.); }
 
 __device__ __forceinline__ void answer(const sample_args &a, long row, int token, u64 mass, u64 total)
 {
@@ -359,7 +364,33 @@ __device__ __forceinline__ void answer(const sample_args &a, long row, int token
     if (a.probs) a.probs[row] = total ? (float)((double)mass / (double)total) : 0.f;
 }
 
-/* ---- a row of up to 16384 tokens: one workgroup, the row in registers ---------------------------------- */
+/* Eight neighbouring tokens from i on; -inf behind `end`. */
+template <int T>
+__device__ __forceinline__ void load8(const typename dn_elt<T>::store *x, int i, int end, bool vectors, float l[8])
+{
+    typedef typename dn_elt<T>::store S;
+    typedef S S4 __attribute__((ext_vector_type(4)));
+    if (vectors && i + 8 <= end) {
+        const S4 u = *(const S4 *)(x + i), v = *(const S4 *)(x + i + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            l[e] = (float)u[e];
+            l[e + 4] = (float)v[e];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) l[e] = i + e < end ? (float)x[i + e] : -INFINITY;
+    }
+}
+
+template <int T>
+__device__ __forceinline__ bool rows_aligned(const sample_args &a)
+{
+    const int size = sizeof(typename dn_elt<T>::store);
+    return ((uintptr_t)a.logits & 15) == 0 && ((a.stride * size) & 15) == 0;
+}
+
+/* ---- a row of up to 8192 tokens: one workgroup, the row in registers ---------------------------------- */
 template <int T, int E, int THREADS>
 __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
 {
@@ -368,12 +399,13 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
     __shared__ u64 candidates[SM_CANDIDATES];
     __shared__ unsigned s_count;
     const int tid = threadIdx.x;
+    const bool vectors = rows_aligned<T>(a);
     for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const S *x = (const S *)a.logits + row * a.stride;
         const sample_row r = settings_of(a, row);
         float l[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) l[e] = tid * E + e < a.n ? (float)x[tid * E + e] : -INFINITY;
+        for (int e = 0; e < E; e += 8) load8<T>(x, tid * E + e, a.n, vectors, l + e);
         float largest = -INFINITY;
 #pragma unroll
         for (int e = 0; e < E; ++e) largest = l[e] > largest ? l[e] : largest;
@@ -384,7 +416,7 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
         }
         u64 last = 0;
         if (r.k || r.p < 1) {
-            for (int i = tid; i < SM_BINS; i += THREADS) {
+            for (int i = tid; i < SM_SLOTS; i += THREADS) {
                 s.count[i] = 0;
                 s.mass[i] = 0;
             }
@@ -393,7 +425,7 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
 #pragma unroll
             for (int e = 0; e < E; ++e)
                 if (l[e] > -INFINITY) {
-                    const int b = bin_of(l[e], largest, r);
+                    const int b = bin_slot(bin_of(l[e], largest, r));
                     if (r.k) atomicAdd(&s.count[b], 1u);
                     if (r.p < 1) atomicAdd(&s.mass[b], mass_of(weight_of(l[e], largest, r)));
                 }
@@ -434,7 +466,7 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
 #pragma unroll
         for (int e = 0; e < E; ++e) own += kept_mass(e);
         const u64 total = block_sum(own, s);
-        const double target = draw_target(a, row, total);
+        const double target = draw_target(r, total);
         u64 run;
         if (reaches(own, 0, target, run, s)) {
             bool done = false;
@@ -479,32 +511,6 @@ __host__ __device__ static inline sample_space space_of(int rows, int segments)
     w.found = w.largest + all * 4;
     w.bytes = w.found + all * 4;
     return w;
-}
-
-/* Eight neighbouring tokens from i on; -inf behind `end`. */
-template <int T>
-__device__ __forceinline__ void load8(const typename dn_elt<T>::store *x, int i, int end, bool vectors, float l[8])
-{
-    typedef typename dn_elt<T>::store S;
-    typedef S S4 __attribute__((ext_vector_type(4)));
-    if (vectors && i + 8 <= end) {
-        const S4 u = *(const S4 *)(x + i), v = *(const S4 *)(x + i + 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            l[e] = (float)u[e];
-            l[e + 4] = (float)v[e];
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) l[e] = i + e < end ? (float)x[i + e] : -INFINITY;
-    }
-}
-
-template <int T>
-__device__ __forceinline__ bool rows_aligned(const sample_args &a)
-{
-    const int size = sizeof(typename dn_elt<T>::store);
-    return ((uintptr_t)a.logits & 15) == 0 && ((a.stride * size) & 15) == 0;
 }
 
 template <int T>
@@ -600,8 +606,8 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_kept_kernel(sample_ar
         __syncthreads();
         if (r.k || r.p < 1)
             for (int i = tid; i < SM_BINS; i += SM_SPLIT_THREADS) {
-                s.mass[i] = ((const u64 *)(a.workspace + ws.bins_mass))[row * SM_BINS + i];
-                s.count[i] = ((const unsigned *)(a.workspace + ws.bins_count))[row * SM_BINS + i];
+                s.mass[bin_slot(i)] = ((const u64 *)(a.workspace + ws.bins_mass))[row * SM_BINS + i];
+                s.count[bin_slot(i)] = ((const unsigned *)(a.workspace + ws.bins_count))[row * SM_BINS + i];
             }
         if (tid == 0) s_count = 0;
         __syncthreads();
@@ -671,7 +677,7 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_draw_kernel(sample_ar
             s_kept[i] = i < blocks ? ((const u64 *)(a.workspace + ws.kept))[row * SM_BLOCKS + i] : 0;
         if (wave == 0) {
             const int c = lane < a.segments ? ((const int *)(a.workspace + ws.found))[row * a.segments + lane] : 0;
-            const int upto = (int)wave_scan((u64)c, lane);
+            const int upto = (int)wave_scan((unsigned)c);
             if (lane < a.segments) s_from[lane + 1] = upto;
             if (lane == 0) s_from[0] = 0;
             const bool whole = __all(c <= SM_LISTED);
@@ -714,7 +720,7 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_draw_kernel(sample_ar
 #pragma unroll
         for (int e = 0; e < E; ++e) own += s_kept[tid * E + e];
         const u64 total = block_sum(own, s);
-        const double target = draw_target(a, row, total);
+        const double target = draw_target(r, total);
         if (reaches(own, 0, target, run, s)) {
             int at = tid * E;
             while ((double)(run + s_kept[at]) < target) run += s_kept[at++];
@@ -760,9 +766,9 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_draw_kernel(sample_ar
     }
 }
 
-/* Rows of up to 16384 tokens take one workgroup each.  Longer ones are cut so that about 1024 workgroups have a
+/* Rows of up to 8192 tokens take one workgroup each.  Longer ones are cut so that about 1024 workgroups have a
  * share of one block of tokens at least. */
-static bool sample_in_one(int n) { return n <= 16384; }
+static bool sample_in_one(int n) { return n <= 8192; }
 
 static void sample_cut(sample_args &a)
 {
@@ -790,8 +796,7 @@ static void sample_launch(const sample_args &a)
     if (sample_in_one(a.n)) {
         const dim3 grid(a.rows < 65536 ? a.rows : 65536);
         if (a.n <= 2048) hipLaunchKernelGGL((sample_row_kernel<T, 8, 256>), grid, dim3(256), 0, dn_stream(), a);
-        else if (a.n <= 4096) hipLaunchKernelGGL((sample_row_kernel<T, 4, 1024>), grid, dim3(1024), 0, dn_stream(), a);
-        else hipLaunchKernelGGL((sample_row_kernel<T, 16, 1024>), grid, dim3(1024), 0, dn_stream(), a);
+        else hipLaunchKernelGGL((sample_row_kernel<T, 16, 512>), grid, dim3(512), 0, dn_stream(), a);
         return;
     }
     const dim3 grid(a.segments, a.rows < 65535 ? a.rows : 65535), block(SM_SPLIT_THREADS);
