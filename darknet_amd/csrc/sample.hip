@@ -11,7 +11,8 @@
  * lanes and atomics add them, so the same row gives the same token in every run, and a border between two
  * tokens lies where the formula puts it to within 2^-38 of the largest mass.
  *
- * No row is sorted.  The logits are counted and weighed in 512 bins, an eighth of T wide, below the largest; the
+ * No row is sorted.  The logits are counted and weighed in 512 bins, a sixteenth of T wide, below the largest (what is
+ * further below weighs nothing); the
  * bin in which the order's prefix ends is known from the running sums, everything in the bins before it is
  * kept, and only that bin's tokens (the candidates) are looked at more closely: digit by digit of their places.
  */
@@ -22,9 +23,11 @@
 typedef unsigned long long u64;
 
 #define SM_BINS 512
-#define SM_PER_T 8
+#define SM_PER_T 16
 #define SM_SHIFT 38
-#define SM_CANDIDATES 4096 /* that fit into LDS */
+#define SM_CANDIDATES 2048 /* that are kept in LDS */
+#define SM_LISTED 8192     /* of a long row that are kept in memory */
+#define SM_FOUND 512       /* of a segment that are handed on */
 #define SM_SEGMENTS 32
 
 struct sample_args {
@@ -131,8 +134,7 @@ struct sample_lds {
     unsigned count[SM_BINS + 64];
     u64 digit[256 + 64], part[16];
     unsigned digit_count[256];
-    u64 prefix, base, found;
-    unsigned single;
+    u64 digit_place[256], prefix, base, found;
     sample_border border;
 };
 
@@ -152,37 +154,42 @@ __device__ __forceinline__ int slot_of(int b)
 __device__ __forceinline__ int bin_slot(int b) { return slot_of<SM_BINS / 64>(b); }
 __device__ __forceinline__ int digit_slot(int d) { return slot_of<4>(d); }
 
+/* A share of a mass as the whole number that a running sum has to reach: at least 1, at most the mass. */
+__device__ __forceinline__ u64 share_of(double share, u64 mass)
+{
+    const u64 t = (u64)ceil(fmax(share * (double)mass, 1.));
+    return t < mass || !mass ? t : mass;
+}
+
 /* One wave: the first of N bins (in order, or from the last one down) at which base + running sum reaches the
  * target, and the sum before it; N if none does.  The target is at least 1. */
 template <int N, bool DOWN, class V>
-__device__ __forceinline__ int find_bin(const V *bins, u64 base, double target, u64 &before, int lane)
+__device__ __forceinline__ int find_bin(const V *bins, u64 base, u64 target, u64 &before, int lane)
 {
     constexpr int E = N / 64;
-    u64 own = 0, v[E];
+    u64 own = 0;
+    V v[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int b = lane * E + e;
         v[e] = bins[slot_of<E>(DOWN ? N - 1 - b : b)];
         own += v[e];
     }
-    u64 run = base + wave_scan(own) - own;
-    int at = N;
-    u64 sum = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        if (at == N && v[e] && (double)(run + v[e]) >= target) {
-            at = lane * E + e;
-            sum = run;
-        }
-        run += v[e];
-    }
-    const u64 any = __ballot(at < N);
-    if (!any) {
-        before = 0;
-        return N;
-    }
+    u64 run = base + wave_scan(own);
+    const u64 any = __ballot(run >= target);
+    before = 0;
+    if (!any) return N;
     const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)any) - 1);
-    before = dn_lane(sum, src);
+    run -= own;
+    int at = lane * E;
+    bool done = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) { /* of use in lane src only */
+        done = done || run + v[e] >= target;
+        run += done ? 0 : v[e];
+        at += done ? 0 : 1;
+    }
+    before = dn_lane(run, src);
     at = (int)dn_lane((unsigned)at, src);
     return DOWN ? N - 1 - at : at;
 }
@@ -195,7 +202,7 @@ __device__ __forceinline__ sample_border border_of(const sample_lds &s, const sa
     if (r.p < 1 || r.k) {
         u64 own_mass = 0;
         if (r.k) {
-            b.k_bin = find_bin<SM_BINS, false>(s.count, 0, (double)r.k, count, lane);
+            b.k_bin = find_bin<SM_BINS, false>(s.count, 0, (u64)r.k, count, lane);
             if (b.k_bin == SM_BINS) b.k_bin = -1; /* fewer than k tokens can be drawn at all */
             else b.k_need = r.k - (int)count;
         }
@@ -209,9 +216,11 @@ __device__ __forceinline__ sample_border border_of(const sample_lds &s, const sa
         b.mass_k = mass_least;
     }
     if (r.p < 1) {
-        u64 ignore;
-        b.lo = find_bin<SM_BINS, false>(s.mass, 0, fmax((double)r.p * (double)mass_least, 1.), b.mass_lo, lane);
-        b.hi = find_bin<SM_BINS, false>(s.mass, 0, fmax((double)r.p * (double)mass_most, 1.), ignore, lane);
+#pragma unroll 1
+        for (int end = 1; end >= 0; --end) {
+            b.lo = find_bin<SM_BINS, false>(s.mass, 0, share_of(r.p, end ? mass_most : mass_least), b.mass_lo, lane);
+            if (end) b.hi = b.lo;
+        }
         b.first = b.lo;
     } else if (b.k_bin >= 0) {
         b.first = b.k_bin;
@@ -248,102 +257,125 @@ __device__ __forceinline__ float block_largest(float v, sample_lds &s)
 
 __device__ __forceinline__ u64 shift_right(u64 v, int bits) { return bits > 63 ? 0 : v >> bits; }
 
-/* The place at which base + the running sum of value(place) over the places handed out by each(), from the largest
- * down, reaches the target.  By eight bits a round, from the first bit in which two of the places differ. */
-template <class Each, class Value>
-__device__ __forceinline__ u64 find_place(Each each, Value value, u64 base, double target, sample_lds &s)
+/* mass_of the weight, and in the top bit whether min-p keeps it. */
+#define SM_KEPT (1ull << 63)
+__device__ __forceinline__ u64 weigh(float l, float largest, const sample_row &r)
 {
-    const int tid = threadIdx.x, lane = tid & 63;
-    u64 most = 0, least = ~0ull;
-    each([&](u64 c) {
-        most = c > most ? c : most;
-        least = c < least ? c : least;
-    });
-    most = dn_wave_max(most);
-    least = ~dn_wave_max(~least);
-    __syncthreads();
-    if (tid == 0) {
-        s.prefix = 0;
-        s.found = ~0ull;
-    }
-    __syncthreads();
-    if (lane == 0) {
-        atomicMax(&s.prefix, most);
-        atomicMin(&s.found, least);
-    }
-    __syncthreads();
-    most = s.prefix;
-    least = s.found;
-    if (most <= least) return most;
-    int bit = 64 - __clzll((long long)(most ^ least));
-    u64 prefix = shift_right(most, bit);
-    while (bit > 0) {
-        const int next = bit > 8 ? bit - 8 : 0;
-        __syncthreads();
-        if (tid < 256) {
-            s.digit[digit_slot(tid)] = 0;
-            s.digit_count[tid] = 0;
-        }
-        __syncthreads();
-        each([&](u64 c) {
-            if (shift_right(c, bit) != prefix) return;
-            const int d = (int)(c >> next) & ((1 << (bit - next)) - 1);
-            atomicAdd(&s.digit[digit_slot(d)], value(c));
-            atomicAdd(&s.digit_count[d], 1u);
-        });
-        __syncthreads();
-        if (tid < 64) {
-            u64 before;
-            const int d = find_bin<256, true>(s.digit, base, target, before, lane);
-            if (lane == 0) {
-                s.prefix = prefix << (bit - next) | (u64)(d & 255);
-                s.base = before;
-                s.single = s.digit_count[d & 255] == 1;
-            }
-        }
-        __syncthreads();
-        prefix = s.prefix;
-        base = s.base;
-        bit = next;
-        if (bit > 0 && s.single) {
-            each([&](u64 c) {
-                if (shift_right(c, bit) == prefix) s.found = c;
-            });
-            __syncthreads();
-            return s.found;
-        }
-    }
-    return prefix;
+    const double w = weight_of(l, largest, r);
+    return mass_of(w) | (w >= r.floor ? SM_KEPT : 0);
 }
 
-/* The last place of the kept prefix, from the candidates: top-k first, then top-p of what it left. */
+/* The candidates of a row: places and what weigh() says of them in LDS; where they are too many, a list of places
+ * in memory; where they are too many for that (values that most tokens share), the row itself, a strip of 8 tokens a
+ * lane at a time.  Loops over them are kept rolled, here and below: these kernels run their code about once, so
+ * that its size is time. */
+struct sample_candidates {
+    u64 place[SM_CANDIDATES], weight[SM_CANDIDATES];
+};
+
+template <int THREADS, class Strip, class F>
+__device__ __forceinline__ void each_candidate(const sample_candidates &c, const u64 *list, int count, int n, Strip strip,
+                                               const sample_border &b, const sample_row &r, float largest, F f)
+{
+    const bool in_lds = count <= SM_CANDIDATES, in_row = !in_lds && !list;
+    const int end = in_row ? n : count, step = in_row ? 8 : 1;
+#pragma unroll 1
+    for (int i = threadIdx.x * step; i < end; i += THREADS * step) {
+        const float *l = in_row ? strip(i) : 0;
+#pragma unroll 1
+        for (int e = 0; e < step; ++e) {
+            u64 place;
+            if (in_row) {
+                if (!(l[e] > -INFINITY) || !is_candidate(b, bin_of(l[e], largest, r))) continue;
+                place = place_of(l[e], i + e);
+            } else {
+                place = in_lds ? c.place[i] : list[i];
+            }
+            f(place, in_lds ? c.weight[i] : weigh(logit_of(place), largest, r));
+        }
+    }
+}
+
+/* The last place of the kept prefix, from the candidates: top-k among those of its bin, then top-p among those that it
+ * left.  Each is found by eight bits a round, from the first bit in which two of the places differ. */
 template <class Each>
 __device__ __forceinline__ u64 last_place(Each each, const sample_border &b, const sample_row &r, float largest, sample_lds &s)
 {
-    auto mass = [&](u64 c) { return mass_of(weight_of(logit_of(c), largest, r)); };
-    u64 k_place = 0, p_place = 0, mass_k = b.mass_k;
-    if (b.k_bin >= 0) {
-        auto in_k_bin = [&](auto f) {
-            each([&](u64 c) {
-                if (bin_of(logit_of(c), largest, r) == b.k_bin) f(c);
-            });
-        };
-        k_place = find_place(in_k_bin, [](u64) { return (u64)1; }, 0, (double)b.k_need, s);
-        if (r.p < 1) {
-            u64 m = 0;
-            in_k_bin([&](u64 c) { m += c >= k_place ? mass(c) : 0; });
-            mass_k += block_sum(m, s);
+    const int tid = threadIdx.x, lane = tid & 63;
+    u64 last = 0, mass_k = b.mass_k;
+#pragma unroll 1
+    for (int stage = 0; stage < 2; ++stage) {
+        const bool by_mass = stage == 1;
+        if (by_mass ? !(r.p < 1) : b.k_bin < 0) continue;
+        u64 most = 0, least = ~0ull, in_k = 0;
+        auto takes_part = [&](u64 c) { return by_mass ? c >= last : bin_of(logit_of(c), largest, r) == b.k_bin; };
+        each([&](u64 c, u64 w) {
+            if (!takes_part(c)) return;
+            most = c > most ? c : most;
+            least = c < least ? c : least;
+            if (bin_of(logit_of(c), largest, r) == b.k_bin) in_k += w & ~SM_KEPT;
+        });
+        most = dn_wave_max(most);
+        least = ~dn_wave_max(~least);
+        if (by_mass) mass_k += block_sum(in_k, s);
+        __syncthreads();
+        if (tid == 0) {
+            s.prefix = 0;
+            s.found = ~0ull;
         }
+        __syncthreads();
+        if (lane == 0) {
+            atomicMax(&s.prefix, most);
+            atomicMin(&s.found, least);
+        }
+        __syncthreads();
+        most = s.prefix;
+        least = s.found;
+        const u64 target = by_mass ? share_of(r.p, mass_k) : (u64)b.k_need;
+        u64 base = by_mass ? b.mass_lo : 0;
+        int bit = most > least ? 64 - __clzll((long long)(most ^ least)) : 0;
+        u64 prefix = shift_right(most, bit);
+        while (bit > 0) {
+            const int next = bit > 8 ? bit - 8 : 0;
+            __syncthreads();
+            if (tid < 256) {
+                s.digit[digit_slot(tid)] = 0;
+                s.digit_count[tid] = 0;
+            }
+            __syncthreads();
+            each([&](u64 c, u64 w) {
+                if (!takes_part(c) || shift_right(c, bit) != prefix) return;
+                const int d = (int)(c >> next) & ((1 << (bit - next)) - 1);
+                atomicAdd(&s.digit[digit_slot(d)], by_mass ? w & ~SM_KEPT : 1ull);
+                if (atomicAdd(&s.digit_count[d], 1u) == 0) s.digit_place[d] = c;
+            });
+            __syncthreads();
+            if (tid < 64) {
+                u64 before;
+                const int d = find_bin<256, true>(s.digit, base, target, before, lane) & 255;
+                if (lane == 0) {
+                    s.prefix = prefix << (bit - next) | (u64)d;
+                    s.base = before;
+                    s.found = s.digit_count[d] == 1 ? s.digit_place[d] : 0;
+                }
+            }
+            __syncthreads();
+            prefix = s.prefix;
+            base = s.base;
+            bit = next;
+            if (s.found) { /* the only one with this digit */
+                prefix = s.found;
+                break;
+            }
+        }
+        last = prefix > last ? prefix : last;
     }
-    if (r.p < 1)
-        p_place = find_place([&](auto f) { each([&](u64 c) { if (c >= k_place) f(c); }); }, mass, b.mass_lo,
-                             fmax((double)r.p * (double)mass_k, 1.), s);
-    return k_place > p_place ? k_place : p_place;
+    return last;
 }
 
 /* Each lane has `own`, the mass of its piece of consecutive tokens; pieces follow each other in lane order.  Finds the
  * piece in which base + running mass reaches the target: true for its lane, with the sum before it. */
-__device__ __forceinline__ bool reaches(u64 own, u64 base, double target, u64 &before, sample_lds &s)
+__device__ __forceinline__ bool reaches(u64 own, u64 base, u64 target, u64 &before, sample_lds &s)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const u64 incl = wave_scan(own);
@@ -353,10 +385,8 @@ __device__ __forceinline__ bool reaches(u64 own, u64 base, double target, u64 &b
     u64 run = base + incl - own;
     for (int w = 0; w < wave; ++w) run += s.part[w];
     before = run;
-    return own && (double)run < target && (double)(run + own) >= target;
+    return run < target && run + own >= target;
 }
-
-__device__ __forceinline__ double draw_target(const sample_row &r, u64 total) { return fmax(r.uniform * (double)total, 1.); }
 
 __device__ __forceinline__ void answer(const sample_args &a, long row, int token, u64 mass, u64 total)
 {
@@ -396,19 +426,32 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
 {
     typedef typename dn_elt<T>::store S;
     __shared__ sample_lds s;
-    __shared__ u64 candidates[SM_CANDIDATES];
+    __shared__ sample_candidates c;
+    __shared__ float row_lds[THREADS * (E + 1)]; /* E neighbours a lane; the gap spreads them over the banks */
     __shared__ unsigned s_count;
     const int tid = threadIdx.x;
     const bool vectors = rows_aligned<T>(a);
+    float *own_l = row_lds + tid * (E + 1);
     for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const S *x = (const S *)a.logits + row * a.stride;
         const sample_row r = settings_of(a, row);
-        float l[E];
-#pragma unroll
-        for (int e = 0; e < E; e += 8) load8<T>(x, tid * E + e, a.n, vectors, l + e);
         float largest = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < E; ++e) largest = l[e] > largest ? l[e] : largest;
+        for (int e = 0; e < E; e += 8) {
+            float l[8];
+            load8<T>(x, tid * E + e, a.n, vectors, l);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                own_l[e + i] = l[i];
+                largest = l[i] > largest ? l[i] : largest;
+            }
+        }
+        if (r.k || r.p < 1)
+            for (int i = tid; i < SM_SLOTS; i += THREADS) {
+                s.count[i] = 0;
+                s.mass[i] = 0;
+            }
+        if (tid == 0) s_count = 0;
         largest = block_largest(largest, s);
         if (!(largest > -INFINITY)) {
             if (tid == 0) answer(a, row, -1, 0, 0);
@@ -416,19 +459,14 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
         }
         u64 last = 0;
         if (r.k || r.p < 1) {
-            for (int i = tid; i < SM_SLOTS; i += THREADS) {
-                s.count[i] = 0;
-                s.mass[i] = 0;
+#pragma unroll 1
+            for (int e = 0; e < E; ++e) {
+                const float l = own_l[e];
+                if (!(l > -INFINITY)) continue;
+                const int b = bin_slot(bin_of(l, largest, r));
+                if (r.k) atomicAdd(&s.count[b], 1u);
+                if (r.p < 1) atomicAdd(&s.mass[b], mass_of(weight_of(l, largest, r)));
             }
-            if (tid == 0) s_count = 0;
-            __syncthreads();
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (l[e] > -INFINITY) {
-                    const int b = bin_slot(bin_of(l[e], largest, r));
-                    if (r.k) atomicAdd(&s.count[b], 1u);
-                    if (r.p < 1) atomicAdd(&s.mass[b], mass_of(weight_of(l[e], largest, r)));
-                }
             __syncthreads();
             if (tid < 64) {
                 const sample_border b = border_of(s, r, tid);
@@ -437,46 +475,40 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
             __syncthreads();
             const sample_border b = s.border;
             if (b.k_bin >= 0 || r.p < 1) {
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (l[e] > -INFINITY && is_candidate(b, bin_of(l[e], largest, r))) {
-                        const unsigned at = atomicAdd(&s_count, 1u);
-                        if (at < SM_CANDIDATES) candidates[at] = place_of(l[e], tid * E + e);
-                    }
+#pragma unroll 1
+                for (int e = 0; e < E; ++e) {
+                    const float l = own_l[e];
+                    if (!(l > -INFINITY) || !is_candidate(b, bin_of(l, largest, r))) continue;
+                    const unsigned at = atomicAdd(&s_count, 1u);
+                    if (at >= SM_CANDIDATES) continue;
+                    c.place[at] = place_of(l, tid * E + e);
+                    c.weight[at] = weigh(l, largest, r);
+                }
                 __syncthreads();
                 const int count = (int)s_count;
-                last = last_place([&](auto f) {
-                    if (count <= SM_CANDIDATES) {
-                        for (int i = tid; i < count; i += THREADS) f(candidates[i]);
-                        return;
-                    }
-#pragma unroll
-                    for (int e = 0; e < E; ++e)
-                        if (l[e] > -INFINITY && is_candidate(b, bin_of(l[e], largest, r))) f(place_of(l[e], tid * E + e));
-                }, b, r, largest, s);
+                auto strip = [&](int i) { return row_lds + i + i / E; }; /* E is a multiple of 8 */
+                last = last_place([&](auto f) { each_candidate<THREADS>(c, 0, count, a.n, strip, b, r, largest, f); },
+                                  b, r, largest, s);
             }
         }
         auto kept_mass = [&](int e) {
-            const u64 c = place_of(l[e], tid * E + e);
-            if (!c || c < last) return (u64)0;
-            const double w = weight_of(l[e], largest, r);
-            return w >= r.floor ? mass_of(w) : (u64)0;
+            const u64 place = place_of(own_l[e], tid * E + e);
+            if (!place || place < last) return (u64)0;
+            const u64 w = weigh(own_l[e], largest, r);
+            return w & SM_KEPT ? w & ~SM_KEPT : 0;
         };
-        u64 own = 0;
-#pragma unroll
+        u64 own = 0, run;
+#pragma unroll 1
         for (int e = 0; e < E; ++e) own += kept_mass(e);
-        const u64 total = block_sum(own, s);
-        const double target = draw_target(r, total);
-        u64 run;
+        const u64 total = block_sum(own, s), target = share_of(r.uniform, total);
         if (reaches(own, 0, target, run, s)) {
-            bool done = false;
-#pragma unroll
+#pragma unroll 1
             for (int e = 0; e < E; ++e) {
-                const u64 m = done ? 0 : kept_mass(e);
+                const u64 m = kept_mass(e);
                 run += m;
-                if (m && (double)run >= target) {
+                if (run >= target) {
                     answer(a, row, tid * E + e, m, total);
-                    done = true;
+                    break;
                 }
             }
         }
@@ -492,7 +524,6 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
 #define SM_SPLIT_THREADS 256
 #define SM_STRIP (SM_SPLIT_THREADS * 8) /* tokens that a workgroup takes at a time */
 #define SM_BLOCKS 512                   /* of a row, at most: they are summed in LDS */
-#define SM_LISTED 512                   /* candidates that a segment keeps a list of */
 
 struct sample_space {
     size_t kept, bins_mass, border, list, bins_count, largest, found, bytes;
@@ -506,10 +537,10 @@ __host__ __device__ static inline sample_space space_of(int rows, int segments)
     w.bins_mass = w.kept + (size_t)rows * SM_BLOCKS * 8;
     w.border = w.bins_mass + (size_t)rows * SM_BINS * 8;
     w.list = w.border + (size_t)rows * sizeof(sample_border);
-    w.bins_count = w.list + all * SM_LISTED * 8;
+    w.bins_count = w.list + (size_t)rows * SM_LISTED * 8;
     w.largest = w.bins_count + (size_t)rows * SM_BINS * 4;
     w.found = w.largest + all * 4;
-    w.bytes = w.found + all * 4;
+    w.bytes = w.found + (size_t)rows * 8;
     return w;
 }
 
@@ -540,6 +571,7 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_largest_kernel(sample
             for (int i = threadIdx.x; i < SM_BINS; i += SM_SPLIT_THREADS) {
                 ((u64 *)(a.workspace + ws.bins_mass))[row * SM_BINS + i] = 0;
                 ((unsigned *)(a.workspace + ws.bins_count))[row * SM_BINS + i] = 0;
+                if (i < 2) ((unsigned *)(a.workspace + ws.found))[row * 2 + i] = 0;
             }
     }
 }
@@ -596,7 +628,8 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_kept_kernel(sample_ar
 {
     typedef typename dn_elt<T>::store S;
     __shared__ sample_lds s;
-    __shared__ unsigned s_count;
+    __shared__ u64 s_list[SM_FOUND];
+    __shared__ unsigned s_count, s_from;
     const sample_space ws = space_of(a.rows, a.segments);
     const bool vectors = rows_aligned<T>(a);
     const int tid = threadIdx.x;
@@ -622,7 +655,6 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_kept_kernel(sample_ar
         const sample_border b = s.border;
         const S *x = (const S *)a.logits + row * a.stride;
         const int lo = blockIdx.x * a.length, hi = min(a.n, lo + a.length);
-        u64 *list = (u64 *)(a.workspace + ws.list) + ((size_t)row * a.segments + blockIdx.x) * SM_LISTED;
         for (int from = lo; from < hi; from += a.block) {
             u64 own = 0;
             const int to = min(hi, from + a.block);
@@ -638,15 +670,26 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_kept_kernel(sample_ar
                         if (w >= r.floor) own += mass_of(w);
                     } else if (is_candidate(b, bin)) {
                         const unsigned at = atomicAdd(&s_count, 1u);
-                        if (at < SM_LISTED) list[at] = place_of(l[e], i + e);
+                        if (at < SM_FOUND) s_list[at] = place_of(l[e], i + e);
                     }
                 }
             }
             const u64 kept = block_sum(own, s);
             if (tid == 0) ((u64 *)(a.workspace + ws.kept))[row * SM_BLOCKS + from / a.block] = kept;
         }
+        /* the segment's candidates behind those of the segments that came first; their order does not matter.  More than
+         * can be handed on: the second number */
         __syncthreads();
-        if (tid == 0) ((int *)(a.workspace + ws.found))[row * a.segments + blockIdx.x] = (int)s_count;
+        const unsigned count = s_count;
+        unsigned *found = (unsigned *)(a.workspace + ws.found) + row * 2;
+        if (tid == 0 && count) {
+            if (count > SM_FOUND) atomicAdd(found + 1, 1u);
+            s_from = atomicAdd(found, count);
+        }
+        __syncthreads();
+        u64 *list = (u64 *)(a.workspace + ws.list) + (size_t)row * SM_LISTED;
+        for (unsigned i = tid; i < count && i < SM_FOUND; i += SM_SPLIT_THREADS)
+            if (s_from + i < SM_LISTED) list[s_from + i] = s_list[i];
     }
 }
 
@@ -655,112 +698,101 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_draw_kernel(sample_ar
 {
     typedef typename dn_elt<T>::store S;
     __shared__ sample_lds s;
-    __shared__ u64 candidates[SM_CANDIDATES];
+    __shared__ sample_candidates c;
     __shared__ u64 s_kept[SM_BLOCKS];
-    __shared__ int s_from[SM_SEGMENTS + 1], s_listed;
+    __shared__ float strip[SM_SPLIT_THREADS * 9];
     __shared__ u64 s_before;
     __shared__ int s_block;
     const sample_space ws = space_of(a.rows, a.segments);
     const bool vectors = rows_aligned<T>(a);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, blocks = (a.n + a.block - 1) / a.block;
+    const int tid = threadIdx.x, blocks = (a.n + a.block - 1) / a.block;
     for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        /* all that the first steps read is asked for at once */
         const sample_row r = settings_of(a, row);
+        const sample_border b = ((const sample_border *)(a.workspace + ws.border))[row];
+        const u64 *kept = (const u64 *)(a.workspace + ws.kept) + row * SM_BLOCKS;
+        const u64 kept0 = tid < blocks ? kept[tid] : 0, kept1 = tid + SM_SPLIT_THREADS < blocks ? kept[tid + SM_SPLIT_THREADS] : 0;
+        const int count = ((const int *)(a.workspace + ws.found))[row * 2], lost = ((const int *)(a.workspace + ws.found))[row * 2 + 1];
+        const u64 *in_memory = (const u64 *)(a.workspace + ws.list) + (size_t)row * SM_LISTED;
         const float largest = row_largest(a, ws, row);
+        const S *x = (const S *)a.logits + row * a.stride;
         if (!(largest > -INFINITY)) {
             if (tid == 0) answer(a, row, -1, 0, 0);
             continue;
         }
-        const S *x = (const S *)a.logits + row * a.stride;
-        const sample_border b = ((const sample_border *)(a.workspace + ws.border))[row];
         __syncthreads();
-        for (int i = tid; i < SM_BLOCKS; i += SM_SPLIT_THREADS)
-            s_kept[i] = i < blocks ? ((const u64 *)(a.workspace + ws.kept))[row * SM_BLOCKS + i] : 0;
-        if (wave == 0) {
-            const int c = lane < a.segments ? ((const int *)(a.workspace + ws.found))[row * a.segments + lane] : 0;
-            const int upto = (int)wave_scan((unsigned)c);
-            if (lane < a.segments) s_from[lane + 1] = upto;
-            if (lane == 0) s_from[0] = 0;
-            const bool whole = __all(c <= SM_LISTED);
-            if (lane == 63) s_listed = whole && upto <= SM_CANDIDATES;
-        }
-        __syncthreads();
-        const int count = s_from[a.segments];
+        s_kept[tid] = kept0;
+        s_kept[tid + SM_SPLIT_THREADS] = kept1;
         u64 last = 0;
         if (count) {
-            const bool fits = s_listed;
-            if (fits) {
-                for (int g = wave; g < a.segments; g += SM_SPLIT_THREADS / 64) {
-                    const u64 *list = (const u64 *)(a.workspace + ws.list) + ((size_t)row * a.segments + g) * SM_LISTED;
-                    for (int j = lane; j < s_from[g + 1] - s_from[g]; j += 64) candidates[s_from[g] + j] = list[j];
+            const bool whole = !lost && count <= SM_LISTED;
+            const u64 *list = whole ? in_memory : 0;
+            const int held = whole ? count : 0x7fffffff;
+            if (held <= SM_CANDIDATES)
+#pragma unroll 1
+                for (int i = tid; i < held; i += SM_SPLIT_THREADS) {
+                    c.place[i] = list[i];
+                    c.weight[i] = weigh(logit_of(list[i]), largest, r);
                 }
-                __syncthreads();
-            }
-            auto each = [&](auto f) {
-                if (fits) {
-                    for (int i = tid; i < count; i += SM_SPLIT_THREADS) f(candidates[i]);
-                    return;
-                }
-                for (int i = tid * 8; i < a.n; i += SM_STRIP) { /* too many for the lists: from the row again */
-                    float l[8];
-                    load8<T>(x, i, a.n, vectors, l);
-                    for (int e = 0; e < 8; ++e)
-                        if (l[e] > -INFINITY && is_candidate(b, bin_of(l[e], largest, r))) f(place_of(l[e], i + e));
-                }
+            __syncthreads();
+            auto strip_at = [&](int i) {
+                float l[8], *to = strip + tid * 9;
+                load8<T>(x, i, a.n, vectors, l);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) to[e] = l[e];
+                return to;
             };
+            auto each = [&](auto f) { each_candidate<SM_SPLIT_THREADS>(c, list, held, a.n, strip_at, b, r, largest, f); };
             last = last_place(each, b, r, largest, s);
-            each([&](u64 c) {
-                if (c < last) return;
-                const double w = weight_of(logit_of(c), largest, r);
-                if (w >= r.floor) atomicAdd(&s_kept[(int)(0xffffffffu - (unsigned)c) / a.block], mass_of(w));
+            each([&](u64 place, u64 w) {
+                if (place >= last && w & SM_KEPT) atomicAdd(&s_kept[(int)(0xffffffffu - (unsigned)place) / a.block], w & ~SM_KEPT);
             });
         }
         __syncthreads();
-        u64 own = 0, run;
-        constexpr int E = SM_BLOCKS / SM_SPLIT_THREADS;
-#pragma unroll
-        for (int e = 0; e < E; ++e) own += s_kept[tid * E + e];
-        const u64 total = block_sum(own, s);
-        const double target = draw_target(r, total);
+        static_assert(SM_BLOCKS == 2 * SM_SPLIT_THREADS, "two blocks a lane");
+        const u64 first = s_kept[2 * tid];
+        u64 own = first + s_kept[2 * tid + 1], run;
+        const u64 total = block_sum(own, s), target = share_of(r.uniform, total);
         if (reaches(own, 0, target, run, s)) {
-            int at = tid * E;
-            while ((double)(run + s_kept[at]) < target) run += s_kept[at++];
-            s_block = at;
-            s_before = run;
+            const bool second = run + first < target;
+            s_block = 2 * tid + second;
+            s_before = second ? run + first : run;
         }
         __syncthreads();
         /* the block, a strip at a time, eight tokens a lane */
         run = s_before;
         const int lo = s_block * a.block, hi = min(a.n, lo + a.block);
+#pragma unroll 1
         for (int from = lo; from < hi; from += SM_STRIP) {
             const int i = from + tid * 8;
             float l[8];
-            u64 m[8], before;
             load8<T>(x, i, hi, vectors, l);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) strip[tid * 9 + e] = l[e];
+            auto kept_mass = [&](int e) {
+                const u64 place = place_of(strip[tid * 9 + e], i + e);
+                if (!place || place < last) return (u64)0;
+                const u64 w = weigh(strip[tid * 9 + e], largest, r);
+                return w & SM_KEPT ? w & ~SM_KEPT : 0;
+            };
             own = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const u64 c = place_of(l[e], i + e);
-                m[e] = 0;
-                if (c && c >= last) {
-                    const double w = weight_of(l[e], largest, r);
-                    if (w >= r.floor) m[e] = mass_of(w);
-                }
-                own += m[e];
-            }
+#pragma unroll 1
+            for (int e = 0; e < 8; ++e) own += kept_mass(e);
+            u64 before;
             if (reaches(own, run, target, before, s)) {
-                bool done = false;
-#pragma unroll
+#pragma unroll 1
                 for (int e = 0; e < 8; ++e) {
-                    before += m[e];
-                    if (!done && m[e] && (double)before >= target) {
-                        answer(a, row, i + e, m[e], total);
-                        done = true;
+                    const u64 m = kept_mass(e);
+                    before += m;
+                    if (before >= target) {
+                        answer(a, row, i + e, m, total);
+                        break;
                     }
                 }
             }
             if (from + SM_STRIP < hi) {
                 run += block_sum(own, s);
-                if ((double)run >= target) break;
+                if (run >= target) break;
             }
         }
     }
