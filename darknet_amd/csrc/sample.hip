@@ -38,7 +38,9 @@ struct sample_args {
     float *probs;
     unsigned char *workspace;
     long stride;
-    int rows, n, segments, length, block; /* length: tokens of a segment, block: of what its mass is summed over */
+    int rows, n;
+    int index_bits; /* that hold n - 1 */
+    int segments, length, block; /* length: tokens of a segment, block: of what its mass is summed over */
 };
 
 /* A row's settings, those that are off in one form. */
@@ -74,20 +76,27 @@ __device__ __forceinline__ sample_row settings_of(const sample_args &a, long row
     return s;
 }
 
-/* A token's place in the order as one number: larger is earlier.  0 for a token that cannot be drawn (NaN, -inf). */
-__device__ __forceinline__ u64 place_of(float l, int i)
-{
-    if (!(l > -INFINITY)) return 0;
-    const unsigned b = __float_as_uint(l + 0.f); /* -0 ranks as 0 */
-    const unsigned key = b & 0x80000000u ? ~b : b | 0x80000000u;
-    return ((u64)key << 32) | (0xffffffffu - (unsigned)i);
-}
-
-__device__ __forceinline__ float logit_of(u64 place)
-{
-    const unsigned key = (unsigned)(place >> 32);
-    return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
-}
+/* A token's place in the order as one number, larger is earlier: the logit's bits in their order, without those that
+ * are the same in every value of the type (the fewer bits, the fewer rounds find one), and the index from the end.
+ * 0 for a token that cannot be drawn (NaN, -inf). */
+template <int T>
+struct sample_places {
+    static constexpr int SAME = T == DN_F32 ? 0 : T == DN_BF16 ? 16 : 13;
+    int bits; /* of an index */
+    __device__ u64 of(float l, int i) const
+    {
+        if (!(l > -INFINITY)) return 0;
+        const unsigned b = __float_as_uint(l + 0.f); /* -0 ranks as 0 */
+        const unsigned key = b & 0x80000000u ? ~b : b | 0x80000000u;
+        return ((u64)(key >> SAME) << bits) + ((1u << bits) - 1 - (unsigned)i);
+    }
+    __device__ float logit(u64 place) const
+    {
+        const unsigned key = ((unsigned)(place >> bits) << SAME) | ((1u << SAME) - 1);
+        return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu & ~((1u << SAME) - 1) : ~key);
+    }
+    __device__ int index(u64 place) const { return (int)((1u << bits) - 1 - ((unsigned)place & ((1u << bits) - 1))); }
+};
 
 /* 2^x for x <= 0 as the first ten terms of its series around the nearest whole exponent: to 7e-12. */
 __device__ __forceinline__ double weight_of(float l, float largest, const sample_row &s)
@@ -129,11 +138,12 @@ struct sample_border {
     u64 mass_lo, mass_k; /* mass in the bins before lo, before k_bin */
 };
 
+#define SM_DIGIT_SLOTS (256 + 64)
 struct sample_lds {
     u64 mass[SM_BINS + 64];
     unsigned count[SM_BINS + 64];
-    u64 digit[256 + 64], part[16];
-    unsigned digit_count[256];
+    u64 digit[2][SM_DIGIT_SLOTS], part[16];
+    unsigned digit_count[2][256];
     u64 digit_place[256], prefix, base, found;
     sample_border border;
 };
@@ -161,71 +171,105 @@ __device__ __forceinline__ u64 share_of(double share, u64 mass)
     return t < mass || !mass ? t : mass;
 }
 
-/* One wave: the first of N bins (in order, or from the last one down) at which base + running sum reaches the
- * target, and the sum before it; N if none does.  The target is at least 1. */
+/* N bins (in order, or from the last one down) over the lanes of a wave, and where running sums over them reach a
+ * target. */
 template <int N, bool DOWN, class V>
-__device__ __forceinline__ int find_bin(const V *bins, u64 base, u64 target, u64 &before, int lane)
-{
-    constexpr int E = N / 64;
-    u64 own = 0;
+struct sample_sums {
+    static constexpr int E = N / 64;
     V v[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int b = lane * E + e;
-        v[e] = bins[slot_of<E>(DOWN ? N - 1 - b : b)];
-        own += v[e];
-    }
-    u64 run = base + wave_scan(own);
-    const u64 any = __ballot(run >= target);
-    before = 0;
-    if (!any) return N;
-    const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)any) - 1);
-    run -= own;
-    int at = lane * E;
-    bool done = false;
-#pragma unroll
-    for (int e = 0; e < E; ++e) { /* of use in lane src only */
-        done = done || run + v[e] >= target;
-        run += done ? 0 : v[e];
-        at += done ? 0 : 1;
-    }
-    before = dn_lane(run, src);
-    at = (int)dn_lane((unsigned)at, src);
-    return DOWN ? N - 1 - at : at;
-}
+    u64 own, upto; /* a lane's sum, and the running sum through it */
+    int lane;
 
-/* One wave: the borders from the bins in LDS. */
-__device__ __forceinline__ sample_border border_of(const sample_lds &s, const sample_row &r, int lane)
-{
-    sample_border b = {SM_BINS, SM_BINS, SM_BINS - 1, -1, 0, 0, 0};
-    u64 mass_least = 0, mass_most = 0, count = 0;
-    if (r.p < 1 || r.k) {
-        u64 own_mass = 0;
-        if (r.k) {
-            b.k_bin = find_bin<SM_BINS, false>(s.count, 0, (u64)r.k, count, lane);
-            if (b.k_bin == SM_BINS) b.k_bin = -1; /* fewer than k tokens can be drawn at all */
-            else b.k_need = r.k - (int)count;
-        }
+    __device__ void read(const V *bins, int lane_)
+    {
+        lane = lane_;
+        own = 0;
 #pragma unroll
-        for (int e = 0; e < SM_BINS / 64; ++e) {
-            const int at = lane * (SM_BINS / 64) + e;
-            if (b.k_bin < 0 || at < b.k_bin) own_mass += s.mass[bin_slot(at)];
+        for (int e = 0; e < E; ++e) {
+            const int b = lane * E + e;
+            v[e] = bins[slot_of<E>(DOWN ? N - 1 - b : b)];
+            own += v[e];
         }
-        mass_least = dn_wave_sum(own_mass);
-        mass_most = b.k_bin < 0 ? mass_least : mass_least + s.mass[bin_slot(b.k_bin)];
-        b.mass_k = mass_least;
+        upto = wave_scan(own);
     }
-    if (r.p < 1) {
-#pragma unroll 1
-        for (int end = 1; end >= 0; --end) {
-            b.lo = find_bin<SM_BINS, false>(s.mass, 0, share_of(r.p, end ? mass_most : mass_least), b.mass_lo, lane);
-            if (end) b.hi = b.lo;
+    __device__ u64 total() const { return dn_lane(upto, 63); }
+    /* the first bin at which base + running sum reaches the target (at least 1), and the sum before it; N: none */
+    __device__ int find(u64 base, u64 target, u64 &before) const
+    {
+        const u64 any = __ballot(base + upto >= target);
+        before = 0;
+        if (!any) return N;
+        const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)any) - 1);
+        u64 run = base + upto - own;
+        int at = lane * E;
+        bool done = false;
+#pragma unroll
+        for (int e = 0; e < E; ++e) { /* of use in lane src only */
+            done = done || run + v[e] >= target;
+            run += done ? 0 : v[e];
+            at += done ? 0 : 1;
         }
-        b.first = b.lo;
-    } else if (b.k_bin >= 0) {
-        b.first = b.k_bin;
+        before = dn_lane(run, src);
+        at = (int)dn_lane((unsigned)at, src);
+        return DOWN ? N - 1 - at : at;
     }
-    return b;
+    /* the sum before bin b, and with it */
+    __device__ u64 sum_to(int b, u64 &with) const
+    {
+        u64 run = upto - own, next = run;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            run += e < b % E ? v[e] : 0;
+            next += e <= b % E ? v[e] : 0;
+        }
+        with = dn_lane(next, b / E);
+        return dn_lane(run, b / E);
+    }
+};
+
+/* The workgroup: the borders from the bins in LDS, into LDS.  The first wave counts, the second weighs. */
+__device__ __forceinline__ void find_border(sample_lds &s, const sample_row &r)
+{
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    sample_sums<SM_BINS, false, u64> sums;
+    __syncthreads();
+    if (wave == 0) {
+        int bin = -1, need = 0;
+        if (r.k) {
+            sample_sums<SM_BINS, false, unsigned> counts;
+            counts.read(s.count, lane);
+            u64 before;
+            bin = counts.find(0, (u64)r.k, before);
+            need = r.k - (int)before;
+            if (bin == SM_BINS) bin = -1; /* fewer than k tokens can be drawn at all */
+        }
+        if (lane == 0) {
+            s.border.k_bin = bin;
+            s.border.k_need = need;
+        }
+    } else if (wave == 1) {
+        sums.read(s.mass, lane);
+    }
+    __syncthreads();
+    if (wave == 1) {
+        const int k_bin = __builtin_amdgcn_readfirstlane(s.border.k_bin);
+        u64 least, most, mass_lo = 0, ignore;
+        if (k_bin < 0) least = most = sums.total();
+        else least = sums.sum_to(k_bin, most);
+        int lo = SM_BINS, hi = SM_BINS - 1;
+        if (r.p < 1) {
+            lo = hi = sums.find(0, share_of(r.p, least), mass_lo);
+            if (most > least) hi = sums.find(0, share_of(r.p, most), ignore);
+        }
+        if (lane == 0) {
+            s.border.first = r.p < 1 ? lo : k_bin >= 0 ? k_bin : SM_BINS;
+            s.border.lo = lo;
+            s.border.hi = hi;
+            s.border.mass_lo = mass_lo;
+            s.border.mass_k = least;
+        }
+    }
+    __syncthreads();
 }
 
 __device__ __forceinline__ bool is_candidate(const sample_border &b, int bin)
@@ -233,29 +277,30 @@ __device__ __forceinline__ bool is_candidate(const sample_border &b, int bin)
     return (bin >= b.lo && bin <= b.hi) || bin == b.k_bin;
 }
 
-template <class T>
-__device__ __forceinline__ T block_sum(T v, sample_lds &s)
+template <int THREADS>
+__device__ __forceinline__ u64 block_sum(u64 v, sample_lds &s)
 {
     v = dn_wave_sum(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) s.part[threadIdx.x >> 6] = v;
     __syncthreads();
-    T t = 0;
-    for (int w = 0; w < (int)blockDim.x / 64; ++w) t += s.part[w];
+    u64 t = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) t += s.part[w];
     return t;
 }
 
+template <int THREADS>
 __device__ __forceinline__ float block_largest(float v, sample_lds &s)
 {
     v = dn_wave_max(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) s.part[threadIdx.x >> 6] = __float_as_uint(v);
     __syncthreads();
-    for (int w = 0; w < (int)blockDim.x / 64; ++w) v = fmaxf(v, __uint_as_float((unsigned)s.part[w]));
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) v = fmaxf(v, __uint_as_float((unsigned)s.part[w]));
     return v;
 }
-
-__device__ __forceinline__ u64 shift_right(u64 v, int bits) { return bits > 63 ? 0 : v >> bits; }
 
 /* mass_of the weight, and in the top bit whether min-p keeps it. */
 #define SM_KEPT (1ull << 63)
@@ -273,9 +318,10 @@ struct sample_candidates {
     u64 place[SM_CANDIDATES], weight[SM_CANDIDATES];
 };
 
-template <int THREADS, class Strip, class F>
+template <int T, int THREADS, class Strip, class F>
 __device__ __forceinline__ void each_candidate(const sample_candidates &c, const u64 *list, int count, int n, Strip strip,
-                                               const sample_border &b, const sample_row &r, float largest, F f)
+                                               const sample_places<T> &places, const sample_border &b,
+                                               const sample_row &r, float largest, F f)
 {
     const bool in_lds = count <= SM_CANDIDATES, in_row = !in_lds && !list;
     const int end = in_row ? n : count, step = in_row ? 8 : 1;
@@ -287,82 +333,75 @@ __device__ __forceinline__ void each_candidate(const sample_candidates &c, const
             u64 place;
             if (in_row) {
                 if (!(l[e] > -INFINITY) || !is_candidate(b, bin_of(l[e], largest, r))) continue;
-                place = place_of(l[e], i + e);
+                place = places.of(l[e], i + e);
             } else {
                 place = in_lds ? c.place[i] : list[i];
             }
-            f(place, in_lds ? c.weight[i] : weigh(logit_of(place), largest, r));
+            f(place, in_lds ? c.weight[i] : weigh(places.logit(place), largest, r));
         }
     }
 }
 
 /* The last place of the kept prefix, from the candidates: top-k among those of its bin, then top-p among those that it
- * left.  Each is found by eight bits a round, from the first bit in which two of the places differ. */
-template <class Each>
-__device__ __forceinline__ u64 last_place(Each each, const sample_border &b, const sample_row &r, float largest, sample_lds &s)
+ * left.  Each is found by eight bits a round, from the first bit in which two logits of these bins can differ. */
+template <int T, int THREADS, class Each>
+__device__ __forceinline__ u64 last_place(Each each, const sample_places<T> &places, const sample_border &b,
+                                          const sample_row &r, float largest, sample_lds &s)
 {
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     u64 last = 0, mass_k = b.mass_k;
 #pragma unroll 1
     for (int stage = 0; stage < 2; ++stage) {
         const bool by_mass = stage == 1;
         if (by_mass ? !(r.p < 1) : b.k_bin < 0) continue;
-        u64 most = 0, least = ~0ull, in_k = 0;
-        auto takes_part = [&](u64 c) { return by_mass ? c >= last : bin_of(logit_of(c), largest, r) == b.k_bin; };
-        each([&](u64 c, u64 w) {
-            if (!takes_part(c)) return;
-            most = c > most ? c : most;
-            least = c < least ? c : least;
-            if (bin_of(logit_of(c), largest, r) == b.k_bin) in_k += w & ~SM_KEPT;
-        });
-        most = dn_wave_max(most);
-        least = ~dn_wave_max(~least);
-        if (by_mass) mass_k += block_sum(in_k, s);
-        __syncthreads();
-        if (tid == 0) {
-            s.prefix = 0;
-            s.found = ~0ull;
+        const int from = by_mass ? b.lo : b.k_bin, to = by_mass ? b.hi : b.k_bin;
+        auto bin = [&](u64 c) { return bin_of(places.logit(c), largest, r); };
+        __syncthreads(); /* the last use of s is over */
+        for (int i = tid; i < SM_DIGIT_SLOTS; i += THREADS) s.digit[0][i] = 0;
+        for (int i = tid; i < 256; i += THREADS) s.digit_count[0][i] = 0;
+        if (by_mass && b.k_bin >= 0) {
+            u64 in_k = 0;
+            each([&](u64 c, u64 w) { in_k += c >= last && bin(c) == b.k_bin ? w & ~SM_KEPT : 0; });
+            mass_k += block_sum<THREADS>(in_k, s);
         }
         __syncthreads();
-        if (lane == 0) {
-            atomicMax(&s.prefix, most);
-            atomicMin(&s.found, least);
-        }
-        __syncthreads();
-        most = s.prefix;
-        least = s.found;
         const u64 target = by_mass ? share_of(r.p, mass_k) : (u64)b.k_need;
         u64 base = by_mass ? b.mass_lo : 0;
-        int bit = most > least ? 64 - __clzll((long long)(most ^ least)) : 0;
-        u64 prefix = shift_right(most, bit);
+        /* logits of bins from .. to, a hundredth of a bin more on either side than the rounding of bin_of needs */
+        const float upper = fminf(largest, largest - (from - 0.01f) / r.bins_per_logit);
+        const float lower = to < SM_BINS - 1 ? largest - (to + 1.01f) / r.bins_per_logit : -INFINITY;
+        const u64 most = places.of(upper, 0), least = places.of(lower, (1 << places.bits) - 1);
+        int bit = most > least ? 64 - __clzll((long long)(most ^ least)) : 0, turn = 0;
+        u64 prefix = most >> bit; /* places have 56 bits at most */
         while (bit > 0) {
             const int next = bit > 8 ? bit - 8 : 0;
-            __syncthreads();
-            if (tid < 256) {
-                s.digit[digit_slot(tid)] = 0;
-                s.digit_count[tid] = 0;
-            }
-            __syncthreads();
             each([&](u64 c, u64 w) {
-                if (!takes_part(c) || shift_right(c, bit) != prefix) return;
+                const int in = bin(c);
+                if (in < from || in > to || c < last || c >> bit != prefix) return;
                 const int d = (int)(c >> next) & ((1 << (bit - next)) - 1);
-                atomicAdd(&s.digit[digit_slot(d)], by_mass ? w & ~SM_KEPT : 1ull);
-                if (atomicAdd(&s.digit_count[d], 1u) == 0) s.digit_place[d] = c;
+                atomicAdd(&s.digit[turn][digit_slot(d)], by_mass ? w & ~SM_KEPT : 1ull);
+                if (atomicAdd(&s.digit_count[turn][d], 1u) == 0) s.digit_place[d] = c;
             });
             __syncthreads();
-            if (tid < 64) {
+            if (wave == 0) {
                 u64 before;
-                const int d = find_bin<256, true>(s.digit, base, target, before, lane) & 255;
+                sample_sums<256, true, u64> sums;
+                sums.read(s.digit[turn], lane);
+                const int d = sums.find(base, target, before) & 255;
                 if (lane == 0) {
                     s.prefix = prefix << (bit - next) | (u64)d;
                     s.base = before;
-                    s.found = s.digit_count[d] == 1 ? s.digit_place[d] : 0;
+                    s.found = s.digit_count[turn][d] == 1 ? s.digit_place[d] : 0;
                 }
+            } else { /* what the next round counts in */
+                for (int i = tid - 64; i < SM_DIGIT_SLOTS; i += THREADS - 64) s.digit[turn ^ 1][i] = 0;
+                for (int i = tid - 64; i < 256; i += THREADS - 64) s.digit_count[turn ^ 1][i] = 0;
             }
             __syncthreads();
             prefix = s.prefix;
             base = s.base;
             bit = next;
+            turn ^= 1;
             if (s.found) { /* the only one with this digit */
                 prefix = s.found;
                 break;
@@ -375,6 +414,7 @@ __device__ __forceinline__ u64 last_place(Each each, const sample_border &b, con
 
 /* Each lane has `own`, the mass of its piece of consecutive tokens; pieces follow each other in lane order.  Finds the
  * piece in which base + running mass reaches the target: true for its lane, with the sum before it. */
+template <int THREADS>
 __device__ __forceinline__ bool reaches(u64 own, u64 base, u64 target, u64 &before, sample_lds &s)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -383,7 +423,8 @@ __device__ __forceinline__ bool reaches(u64 own, u64 base, u64 target, u64 &befo
     if (lane == 63) s.part[wave] = incl;
     __syncthreads();
     u64 run = base + incl - own;
-    for (int w = 0; w < wave; ++w) run += s.part[w];
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) run += w < wave ? s.part[w] : 0;
     before = run;
     return run < target && run + own >= target;
 }
@@ -394,23 +435,27 @@ __device__ __forceinline__ void answer(const sample_args &a, long row, int token
     if (a.probs) a.probs[row] = total ? (float)((double)mass / (double)total) : 0.f;
 }
 
-/* Eight neighbouring tokens from i on; -inf behind `end`. */
+/* Four (eight) neighbouring tokens from i on; -inf behind `end`. */
 template <int T>
-__device__ __forceinline__ void load8(const typename dn_elt<T>::store *x, int i, int end, bool vectors, float l[8])
+__device__ __forceinline__ void load4(const typename dn_elt<T>::store *x, int i, int end, bool vectors, float *l)
 {
     typedef typename dn_elt<T>::store S;
     typedef S S4 __attribute__((ext_vector_type(4)));
-    if (vectors && i + 8 <= end) {
-        const S4 u = *(const S4 *)(x + i), v = *(const S4 *)(x + i + 4);
+    if (vectors && i + 4 <= end) {
+        const S4 u = *(const S4 *)(x + i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            l[e] = (float)u[e];
-            l[e + 4] = (float)v[e];
-        }
+        for (int e = 0; e < 4; ++e) l[e] = (float)u[e];
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) l[e] = i + e < end ? (float)x[i + e] : -INFINITY;
+        for (int e = 0; e < 4; ++e) l[e] = i + e < end ? (float)x[i + e] : -INFINITY;
     }
+}
+
+template <int T>
+__device__ __forceinline__ void load8(const typename dn_elt<T>::store *x, int i, int end, bool vectors, float l[8])
+{
+    load4<T>(x, i, end, vectors, l);
+    load4<T>(x, i + 4, end, vectors, l + 4);
 }
 
 template <int T>
@@ -431,17 +476,18 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
     __shared__ unsigned s_count;
     const int tid = threadIdx.x;
     const bool vectors = rows_aligned<T>(a);
+    const sample_places<T> places = {a.index_bits};
     float *own_l = row_lds + tid * (E + 1);
     for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const S *x = (const S *)a.logits + row * a.stride;
         const sample_row r = settings_of(a, row);
         float largest = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < E; e += 8) {
-            float l[8];
-            load8<T>(x, tid * E + e, a.n, vectors, l);
+        for (int e = 0; e < E; e += 4) {
+            float l[4];
+            load4<T>(x, tid * E + e, a.n, vectors, l);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 4; ++i) {
                 own_l[e + i] = l[i];
                 largest = l[i] > largest ? l[i] : largest;
             }
@@ -452,14 +498,14 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
                 s.mass[i] = 0;
             }
         if (tid == 0) s_count = 0;
-        largest = block_largest(largest, s);
+        largest = block_largest<THREADS>(largest, s);
         if (!(largest > -INFINITY)) {
             if (tid == 0) answer(a, row, -1, 0, 0);
             continue;
         }
         u64 last = 0;
         if (r.k || r.p < 1) {
-#pragma unroll 1
+#pragma unroll 4
             for (int e = 0; e < E; ++e) {
                 const float l = own_l[e];
                 if (!(l > -INFINITY)) continue;
@@ -467,12 +513,7 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
                 if (r.k) atomicAdd(&s.count[b], 1u);
                 if (r.p < 1) atomicAdd(&s.mass[b], mass_of(weight_of(l, largest, r)));
             }
-            __syncthreads();
-            if (tid < 64) {
-                const sample_border b = border_of(s, r, tid);
-                if (tid == 0) s.border = b;
-            }
-            __syncthreads();
+            find_border(s, r);
             const sample_border b = s.border;
             if (b.k_bin >= 0 || r.p < 1) {
 #pragma unroll 1
@@ -481,18 +522,18 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
                     if (!(l > -INFINITY) || !is_candidate(b, bin_of(l, largest, r))) continue;
                     const unsigned at = atomicAdd(&s_count, 1u);
                     if (at >= SM_CANDIDATES) continue;
-                    c.place[at] = place_of(l, tid * E + e);
+                    c.place[at] = places.of(l, tid * E + e);
                     c.weight[at] = weigh(l, largest, r);
                 }
                 __syncthreads();
                 const int count = (int)s_count;
-                auto strip = [&](int i) { return row_lds + i + i / E; }; /* E is a multiple of 8 */
-                last = last_place([&](auto f) { each_candidate<THREADS>(c, 0, count, a.n, strip, b, r, largest, f); },
-                                  b, r, largest, s);
+                auto strip = [&](int i) { return row_lds + i + i / E; }; /* (E = 4: a row has no more tokens than the list holds) */
+                last = last_place<T, THREADS>([&](auto f) { each_candidate<T, THREADS>(c, 0, count, a.n, strip, places, b, r, largest, f); },
+                                     places, b, r, largest, s);
             }
         }
         auto kept_mass = [&](int e) {
-            const u64 place = place_of(own_l[e], tid * E + e);
+            const u64 place = places.of(own_l[e], tid * E + e);
             if (!place || place < last) return (u64)0;
             const u64 w = weigh(own_l[e], largest, r);
             return w & SM_KEPT ? w & ~SM_KEPT : 0;
@@ -500,8 +541,8 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
         u64 own = 0, run;
 #pragma unroll 1
         for (int e = 0; e < E; ++e) own += kept_mass(e);
-        const u64 total = block_sum(own, s), target = share_of(r.uniform, total);
-        if (reaches(own, 0, target, run, s)) {
+        const u64 total = block_sum<THREADS>(own, s), target = share_of(r.uniform, total);
+        if (reaches<THREADS>(own, 0, target, run, s)) {
 #pragma unroll 1
             for (int e = 0; e < E; ++e) {
                 const u64 m = kept_mass(e);
@@ -523,6 +564,7 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
  * 4 one workgroup a row: the prefix' end among the candidates, the block that the draw falls into, the token */
 #define SM_SPLIT_THREADS 256
 #define SM_STRIP (SM_SPLIT_THREADS * 8) /* tokens that a workgroup takes at a time */
+#define SM_DRAW_THREADS 512
 #define SM_BLOCKS 512                   /* of a row, at most: they are summed in LDS */
 
 struct sample_space {
@@ -632,6 +674,7 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_kept_kernel(sample_ar
     __shared__ unsigned s_count, s_from;
     const sample_space ws = space_of(a.rows, a.segments);
     const bool vectors = rows_aligned<T>(a);
+    const sample_places<T> places = {a.index_bits};
     const int tid = threadIdx.x;
     for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
         const sample_row r = settings_of(a, row);
@@ -643,15 +686,8 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_kept_kernel(sample_ar
                 s.count[bin_slot(i)] = ((const unsigned *)(a.workspace + ws.bins_count))[row * SM_BINS + i];
             }
         if (tid == 0) s_count = 0;
-        __syncthreads();
-        if (tid < 64) {
-            const sample_border b = border_of(s, r, tid);
-            if (tid == 0) {
-                s.border = b;
-                if (blockIdx.x == 0) ((sample_border *)(a.workspace + ws.border))[row] = b;
-            }
-        }
-        __syncthreads();
+        find_border(s, r);
+        if (tid == 0 && blockIdx.x == 0) ((sample_border *)(a.workspace + ws.border))[row] = s.border;
         const sample_border b = s.border;
         const S *x = (const S *)a.logits + row * a.stride;
         const int lo = blockIdx.x * a.length, hi = min(a.n, lo + a.length);
@@ -670,11 +706,11 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_kept_kernel(sample_ar
                         if (w >= r.floor) own += mass_of(w);
                     } else if (is_candidate(b, bin)) {
                         const unsigned at = atomicAdd(&s_count, 1u);
-                        if (at < SM_FOUND) s_list[at] = place_of(l[e], i + e);
+                        if (at < SM_FOUND) s_list[at] = places.of(l[e], i + e);
                     }
                 }
             }
-            const u64 kept = block_sum(own, s);
+            const u64 kept = block_sum<SM_SPLIT_THREADS>(own, s);
             if (tid == 0) ((u64 *)(a.workspace + ws.kept))[row * SM_BLOCKS + from / a.block] = kept;
         }
         /* the segment's candidates behind those of the segments that came first; their order does not matter.  More than
@@ -694,24 +730,26 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_kept_kernel(sample_ar
 }
 
 template <int T>
-__global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_draw_kernel(sample_args a)
+__global__ __launch_bounds__(SM_DRAW_THREADS) void sample_draw_kernel(sample_args a)
 {
     typedef typename dn_elt<T>::store S;
     __shared__ sample_lds s;
     __shared__ sample_candidates c;
     __shared__ u64 s_kept[SM_BLOCKS];
-    __shared__ float strip[SM_SPLIT_THREADS * 9];
+    constexpr int P = 9; /* a lane's tokens and a gap */
+    __shared__ float strip[SM_DRAW_THREADS * P];
     __shared__ u64 s_before;
     __shared__ int s_block;
     const sample_space ws = space_of(a.rows, a.segments);
     const bool vectors = rows_aligned<T>(a);
+    const sample_places<T> places = {a.index_bits};
     const int tid = threadIdx.x, blocks = (a.n + a.block - 1) / a.block;
     for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         /* all that the first steps read is asked for at once */
         const sample_row r = settings_of(a, row);
         const sample_border b = ((const sample_border *)(a.workspace + ws.border))[row];
         const u64 *kept = (const u64 *)(a.workspace + ws.kept) + row * SM_BLOCKS;
-        const u64 kept0 = tid < blocks ? kept[tid] : 0, kept1 = tid + SM_SPLIT_THREADS < blocks ? kept[tid + SM_SPLIT_THREADS] : 0;
+        const u64 own_kept = tid < blocks ? kept[tid] : 0;
         const int count = ((const int *)(a.workspace + ws.found))[row * 2], lost = ((const int *)(a.workspace + ws.found))[row * 2 + 1];
         const u64 *in_memory = (const u64 *)(a.workspace + ws.list) + (size_t)row * SM_LISTED;
         const float largest = row_largest(a, ws, row);
@@ -721,8 +759,7 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_draw_kernel(sample_ar
             continue;
         }
         __syncthreads();
-        s_kept[tid] = kept0;
-        s_kept[tid + SM_SPLIT_THREADS] = kept1;
+        s_kept[tid] = own_kept;
         u64 last = 0;
         if (count) {
             const bool whole = !lost && count <= SM_LISTED;
@@ -730,58 +767,56 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_draw_kernel(sample_ar
             const int held = whole ? count : 0x7fffffff;
             if (held <= SM_CANDIDATES)
 #pragma unroll 1
-                for (int i = tid; i < held; i += SM_SPLIT_THREADS) {
+                for (int i = tid; i < held; i += SM_DRAW_THREADS) {
                     c.place[i] = list[i];
-                    c.weight[i] = weigh(logit_of(list[i]), largest, r);
+                    c.weight[i] = weigh(places.logit(list[i]), largest, r);
                 }
             __syncthreads();
             auto strip_at = [&](int i) {
-                float l[8], *to = strip + tid * 9;
+                float l[8], *to = strip + tid * P;
                 load8<T>(x, i, a.n, vectors, l);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) to[e] = l[e];
                 return to;
             };
-            auto each = [&](auto f) { each_candidate<SM_SPLIT_THREADS>(c, list, held, a.n, strip_at, b, r, largest, f); };
-            last = last_place(each, b, r, largest, s);
+            auto each = [&](auto f) { each_candidate<T, SM_DRAW_THREADS>(c, list, held, a.n, strip_at, places, b, r, largest, f); };
+            last = last_place<T, SM_DRAW_THREADS>(each, places, b, r, largest, s);
             each([&](u64 place, u64 w) {
-                if (place >= last && w & SM_KEPT) atomicAdd(&s_kept[(int)(0xffffffffu - (unsigned)place) / a.block], w & ~SM_KEPT);
+                if (place >= last && w & SM_KEPT) atomicAdd(&s_kept[places.index(place) / a.block], w & ~SM_KEPT);
             });
         }
         __syncthreads();
-        static_assert(SM_BLOCKS == 2 * SM_SPLIT_THREADS, "two blocks a lane");
-        const u64 first = s_kept[2 * tid];
-        u64 own = first + s_kept[2 * tid + 1], run;
-        const u64 total = block_sum(own, s), target = share_of(r.uniform, total);
-        if (reaches(own, 0, target, run, s)) {
-            const bool second = run + first < target;
-            s_block = 2 * tid + second;
-            s_before = second ? run + first : run;
+        static_assert(SM_BLOCKS == SM_DRAW_THREADS, "a block a lane");
+        u64 own = s_kept[tid], run;
+        const u64 total = block_sum<SM_DRAW_THREADS>(own, s), target = share_of(r.uniform, total);
+        if (reaches<SM_DRAW_THREADS>(own, 0, target, run, s)) {
+            s_block = tid;
+            s_before = run;
         }
         __syncthreads();
-        /* the block, a strip at a time, eight tokens a lane */
+        /* the block, a strip at a time, four tokens a lane */
         run = s_before;
         const int lo = s_block * a.block, hi = min(a.n, lo + a.block);
 #pragma unroll 1
         for (int from = lo; from < hi; from += SM_STRIP) {
-            const int i = from + tid * 8;
-            float l[8];
-            load8<T>(x, i, hi, vectors, l);
+            const int i = from + tid * 4;
+            float l[4];
+            load4<T>(x, i, hi, vectors, l);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) strip[tid * 9 + e] = l[e];
+            for (int e = 0; e < 4; ++e) strip[tid * P + e] = l[e];
             auto kept_mass = [&](int e) {
-                const u64 place = place_of(strip[tid * 9 + e], i + e);
+                const u64 place = places.of(strip[tid * P + e], i + e);
                 if (!place || place < last) return (u64)0;
-                const u64 w = weigh(strip[tid * 9 + e], largest, r);
+                const u64 w = weigh(strip[tid * P + e], largest, r);
                 return w & SM_KEPT ? w & ~SM_KEPT : 0;
             };
             own = 0;
 #pragma unroll 1
-            for (int e = 0; e < 8; ++e) own += kept_mass(e);
+            for (int e = 0; e < 4; ++e) own += kept_mass(e);
             u64 before;
-            if (reaches(own, run, target, before, s)) {
+            if (reaches<SM_DRAW_THREADS>(own, run, target, before, s)) {
 #pragma unroll 1
-                for (int e = 0; e < 8; ++e) {
+                for (int e = 0; e < 4; ++e) {
                     const u64 m = kept_mass(e);
                     before += m;
                     if (before >= target) {
@@ -791,7 +826,7 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_draw_kernel(sample_ar
                 }
             }
             if (from + SM_STRIP < hi) {
-                run += block_sum(own, s);
+                run += block_sum<SM_DRAW_THREADS>(own, s);
                 if (run >= target) break;
             }
         }
@@ -827,15 +862,16 @@ static void sample_launch(const sample_args &a)
 {
     if (sample_in_one(a.n)) {
         const dim3 grid(a.rows < 65536 ? a.rows : 65536);
-        if (a.n <= 2048) hipLaunchKernelGGL((sample_row_kernel<T, 8, 256>), grid, dim3(256), 0, dn_stream(), a);
-        else hipLaunchKernelGGL((sample_row_kernel<T, 16, 512>), grid, dim3(512), 0, dn_stream(), a);
+        if (a.n <= 1024) hipLaunchKernelGGL((sample_row_kernel<T, 4, 256>), grid, dim3(256), 0, dn_stream(), a);
+        else if (a.n <= 4096) hipLaunchKernelGGL((sample_row_kernel<T, 8, 512>), grid, dim3(512), 0, dn_stream(), a);
+        else hipLaunchKernelGGL((sample_row_kernel<T, 8, 1024>), grid, dim3(1024), 0, dn_stream(), a);
         return;
     }
     const dim3 grid(a.segments, a.rows < 65535 ? a.rows : 65535), block(SM_SPLIT_THREADS);
     hipLaunchKernelGGL((sample_largest_kernel<T>), grid, block, 0, dn_stream(), a);
     if (a.top_k || a.top_p || a.temperature) hipLaunchKernelGGL((sample_bins_kernel<T>), grid, block, 0, dn_stream(), a);
     hipLaunchKernelGGL((sample_kept_kernel<T>), grid, block, 0, dn_stream(), a);
-    hipLaunchKernelGGL((sample_draw_kernel<T>), dim3(a.rows < 65535 ? a.rows : 65535), block, 0, dn_stream(), a);
+    hipLaunchKernelGGL((sample_draw_kernel<T>), dim3(a.rows < 65535 ? a.rows : 65535), dim3(SM_DRAW_THREADS), 0, dn_stream(), a);
 }
 
 extern "C" int sample_rows_gpu(const void *logits, int type, int rows, int n, long stride, const float *temperature,
@@ -855,7 +891,8 @@ extern "C" int sample_rows_gpu(const void *logits, int type, int rows, int n, lo
     if (!workspace && !sample_in_one(n)) return dn_refuse(me, "the workspace is missing");
     hip_require_device(me);
     sample_args a = {logits, temperature, top_p, min_p, uniform, top_k, tokens, probs, (unsigned char *)workspace,
-                     stride, rows, n, 1, n, n};
+                     stride, rows, n, 1, 1, n, n};
+    while (1 << a.index_bits < n) ++a.index_bits;
     if (!sample_in_one(n)) sample_cut(a);
     if (type == DN_F32) sample_launch<DN_F32>(a);
     else if (type == DN_F16) sample_launch<DN_F16>(a);
