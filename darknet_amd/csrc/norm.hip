@@ -21,6 +21,7 @@ struct norm_args {
     float *q8_scales;
     int rows, n, group; /* group: values that share a scale, 0 = the row */
     float eps;
+    double inv_n;
 };
 
 /* Sum (or maximum) over the workgroup, the same bits on every lane and in every run. */
@@ -38,35 +39,52 @@ __device__ __forceinline__ double block_all(double v, double *lds)
     return t;
 }
 
-/* |y| for the maximum: a value that is not finite counts as infinity and so marks its group. */
-__device__ __forceinline__ double finite_abs(double y)
-{
-    const double a = fabs(y);
-    return a <= 1.7976931348623157e308 ? a : __longlong_as_double(0x7ff0000000000000LL);
-}
-
+/* The scale of a group whose largest |y| is given; NaN where that is not finite. */
 __device__ __forceinline__ float q8_step(double largest)
 {
-    const float c = (float)(largest / 127);
+    const float c = (float)(largest * (1. / 127));
     return c <= 3.402823466e38f ? c : __int_as_float(0x7fc00000);
 }
 
-/* The code of y for a step of c, inv = 1 / (double)c: the product differs from the quotient by its last bit, which
- * matters to a rounding as little as the last bit of y. */
-__device__ __forceinline__ int q8_code(double y, float c, double inv)
+/* r / c for a step c > 0: the hardware's reciprocal after two steps of Newton's iteration, in 64 bits. */
+__device__ __forceinline__ double q8_factor(double r, float c)
 {
-    if (!(c > 0)) return 0; /* nothing but zeros, or a group with a value that is not finite */
-    return (int)fmin(fmax(rint(y * inv), -127.), 127.);
+    const double d = (double)c;
+    double x = __builtin_amdgcn_rcp(d);
+    x = fma(fma(-d, x, 1.), x, x);
+    x = fma(fma(-d, x, 1.), x, x);
+    return r * x;
 }
 
-/* V neighbouring elements as floats; VECTORS: they all exist, on a boundary of V elements. */
-template <int T, int V, bool VECTORS>
+/* The maximum over 4, 8, 16 or 32 neighbouring lanes, on each of them: the lane's pair, the other
+ * pair of its quad, the other quad of its 8, the other 8 of its 16, and the other 16. */
+__device__ __forceinline__ double group_largest(double v, int lanes)
+{
+    v = fmax(v, dn_move<0xb1, 0xf>(v, v));
+    v = fmax(v, dn_move<0x4e, 0xf>(v, v));
+    if (lanes >= 8) v = fmax(v, dn_move<0x141, 0xf>(v, v));
+    if (lanes >= 16) v = fmax(v, dn_move<0x140, 0xf>(v, v));
+    if (lanes >= 32) v = fmax(v, __shfl_xor(v, 16, 64));
+    return v;
+}
+
+/* rint(p * factor) within -127 .. 127: added to 1.5 * 2^52 the whole number stands in the low word of the sum. */
+__device__ __forceinline__ int q8_code(double p, double factor)
+{
+    const int q = (int)__double_as_longlong(fma(p, factor, 0x1.8p52));
+    return max(-127, min(127, q));
+}
+
+/* V neighbouring elements as floats, 0 behind the row's end.  Runs that lie within the row go in one access whatever
+ * their alignment. */
+template <int T, int V>
 __device__ __forceinline__ void load_run(const typename dn_elt<T>::store *p, int i, int n, float *v)
 {
     typedef typename dn_elt<T>::store E;
     typedef E EV __attribute__((ext_vector_type(V)));
-    if (VECTORS) {
-        const EV x = *(const EV *)(p + i);
+    typedef EV EU __attribute__((aligned(sizeof(E))));
+    if (i + V <= n) {
+        const EV x = *(const EU *)(p + i);
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] = (float)x[e];
     } else {
@@ -75,16 +93,16 @@ __device__ __forceinline__ void load_run(const typename dn_elt<T>::store *p, int
     }
 }
 
-template <int T, int V, bool VECTORS>
-__device__ __forceinline__ void store_run(typename dn_elt<T>::store *p, int i, int n, const float *v)
+template <class E, int V>
+__device__ __forceinline__ void store_run(E *p, int i, int n, const float *v)
 {
-    typedef typename dn_elt<T>::store E;
     typedef E EV __attribute__((ext_vector_type(V)));
-    if (VECTORS) {
+    typedef EV EU __attribute__((aligned(sizeof(E))));
+    if (i + V <= n) {
         EV x;
 #pragma unroll
         for (int e = 0; e < V; ++e) x[e] = (E)v[e];
-        *(EV *)(p + i) = x;
+        *(EU *)(p + i) = x;
     } else {
 #pragma unroll
         for (int e = 0; e < V; ++e)
@@ -92,185 +110,177 @@ __device__ __forceinline__ void store_run(typename dn_elt<T>::store *p, int i, i
     }
 }
 
+/* max(a, |b|); the language's fmax takes two instructions for it, to quiet signalling NaNs. */
+__device__ __forceinline__ double max_abs(double a, double b)
+{
+    double d;
+    asm("v_max_f64 %0, %1, |%2|" : "=v"(d) : "v"(a), "v"(b));
+    return d;
+}
+
 /* One workgroup for each row, which it holds in registers: RUNS runs of V neighbouring values a lane, the runs of
  * the lanes next to each other (lane t, run j: values (j * THREADS + t) * V on).  Every buffer is read and written once.
- * A group of 8-bit values is a power of two of neighbouring lanes' runs, so that its maximum takes lane moves only. */
-template <int T, int THREADS, int RUNS, int V, bool VECTORS, bool Q8>
+ * RUNS = 0: as many runs as the row has, read again for each step (from the stored sum, if there is one).
+ * A group of 8-bit values is a power of two of neighbouring lanes' runs, so that its maximum takes lane moves only.
+ *
+ * The 8-bit form works on p = s * scales, exact in 64 bits: max|y| = max|p| * r, and code = rint(p * (r / c)). */
+template <int T, int THREADS, int RUNS, int V, bool Q8>
 __global__ __launch_bounds__(THREADS) void rmsnorm_kernel(norm_args a)
 {
     typedef typename dn_elt<T>::store E;
     __shared__ double lds[THREADS / 64];
-    const int tid = threadIdx.x, n = a.n;
+    const int tid = threadIdx.x, n = a.n, runs = RUNS ? RUNS : (n + THREADS * V - 1) / (THREADS * V);
     for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        float s[RUNS][V];
+        const E *in = (const E *)a.input + row * n, *add = a.add ? (const E *)a.add + row * n : 0;
+        E *sum = a.sum ? (E *)a.sum + row * n : 0;
+        auto at = [&](int j) { return (j * THREADS + tid) * V; };
+        auto added = [&](float s[V], const float t[V]) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[e] = (float)(E)(s[e] + t[e]);
+        };
+        float s[RUNS ? RUNS : 1][V];
         double acc = 0;
-        {
-            float add[RUNS][V];
+        auto square = [&](const float v[V]) {
 #pragma unroll
-            for (int j = 0; j < RUNS; ++j) {
-                const int i = (j * THREADS + tid) * V;
-                if (i < n) load_run<T, V, VECTORS>((const E *)a.input + row * n, i, n, s[j]);
-                else
+            for (int e = 0; e < V; ++e) acc = fma((double)v[e], (double)v[e], acc);
+        };
+        if (RUNS) {
+            float t[RUNS ? RUNS : 1][V];
 #pragma unroll
-                    for (int e = 0; e < V; ++e) s[j][e] = 0;
-            }
-            if (a.add) {
+            for (int j = 0; j < RUNS; ++j) load_run<T, V>(in, at(j), n, s[j]);
+            if (add) {
+#pragma unroll
+                for (int j = 0; j < RUNS; ++j) load_run<T, V>(add, at(j), n, t[j]);
 #pragma unroll
                 for (int j = 0; j < RUNS; ++j) {
-                    const int i = (j * THREADS + tid) * V;
-                    if (i < n) load_run<T, V, VECTORS>((const E *)a.add + row * n, i, n, add[j]);
+                    added(s[j], t[j]);
+                    if (sum) store_run<E, V>(sum, at(j), n, s[j]);
                 }
+            }
 #pragma unroll
-                for (int j = 0; j < RUNS; ++j) {
-                    const int i = (j * THREADS + tid) * V;
-                    if (i >= n) continue;
+            for (int j = 0; j < RUNS; ++j) square(s[j]);
+        } else {
+            for (int j = 0; j < runs; ++j) {
+                float v[V], t[V];
+                load_run<T, V>(in, at(j), n, v);
+                if (add) {
+                    load_run<T, V>(add, at(j), n, t);
+                    added(v, t);
+                    if (sum) store_run<E, V>(sum, at(j), n, v);
+                }
+                square(v);
+            }
+        }
+        acc = block_all<THREADS, false>(acc, lds);
+        const double r = 1. / sqrt(fma(acc, a.inv_n, (double)a.eps));
+        auto values = [&](int j, float v[V]) {
+            if (RUNS) {
 #pragma unroll
-                    for (int e = 0; e < V; ++e) s[j][e] = (float)(E)(s[j][e] + add[j][e]);
-                    if (a.sum) store_run<T, V, VECTORS>((E *)a.sum + row * n, i, n, s[j]);
+                for (int e = 0; e < V; ++e) v[e] = s[j][e];
+                return;
+            }
+            load_run<T, V>(sum ? sum : in, at(j), n, v);
+            if (add && !sum) {
+                float t[V];
+                load_run<T, V>(add, at(j), n, t);
+                added(v, t);
+            }
+        };
+        auto scales = [&](int j, float g[V]) {
+            if (a.scales) load_run<DN_F32, V>(a.scales, at(j), n, g);
+            else
+#pragma unroll
+                for (int e = 0; e < V; ++e) g[e] = 1;
+        };
+        if (Q8) { /* before the output, which may take the place of what is read here */
+            /* convert s again below rather than hold its 64-bit forms: with fewer registers more rows fit on a CU */
+#pragma unroll
+            for (int j = 0; j < RUNS; ++j)
+#pragma unroll
+                for (int e = 0; e < V; ++e) asm volatile("" : "+v"(s[j][e]));
+            const int lanes = a.group / V, groups = a.group ? (n + a.group - 1) / a.group : 1;
+            const bool finite = acc <= 1.7976931348623157e308; /* and so every s */
+            const double inf = __longlong_as_double(0x7ff0000000000000LL);
+            /* p of a run, and max|p|: infinity where a factor is not finite (x * 0 is NaN then) */
+            auto products = [&](int j, double p[V]) {
+                float v[V], g[V], poison = 0;
+                double largest = 0;
+                values(j, v);
+                scales(j, g);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    p[e] = (double)v[e] * (double)g[e];
+                    poison = fmaf(g[e], 0.f, poison);
+                    largest = max_abs(largest, p[e]);
+                }
+                if (!finite)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) poison = fmaf(v[e], 0.f, poison);
+                return poison == 0 && r == r ? largest : inf;
+            };
+            double row_largest = 0;
+            if (a.group == 0) {
+#pragma unroll
+                for (int j = 0; j < runs; ++j) {
+                    double p[V];
+                    row_largest = fmax(row_largest, products(j, p));
+                }
+                row_largest = block_all<THREADS, true>(row_largest, lds);
+            }
+#pragma unroll
+            for (int j = 0; j < runs; ++j) {
+                const int i = at(j);
+                double p[V];
+                const double largest = a.group ? group_largest(products(j, p), lanes) : (products(j, p), row_largest);
+                /* an infinite maximum stays one: r may be 0 then */
+                const float c = largest < inf ? q8_step(largest * r) : __int_as_float(0x7fc00000);
+                const double factor = c > 0 ? q8_factor(r, c) : 0; /* codes are 0 where c is 0 or NaN */
+                if (a.group ? i < n && (tid & (lanes - 1)) == 0 : i == 0) a.q8_scales[row * groups + (a.group ? i / a.group : 0)] = c;
+                unsigned q[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) q[e] = (unsigned)(c > 0 ? q8_code(p[e], factor) : 0);
+                signed char *to = a.q8 + row * n;
+                if (i + V <= n) {
+                    typedef unsigned __attribute__((ext_vector_type(V / 4))) words;
+                    typedef words __attribute__((aligned(1))) words_anywhere;
+                    words w;
+#pragma unroll
+                    for (int e = 0; e < V; e += 4)
+                        w[e / 4] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(q[e + 3], q[e + 2], 0x0c0c0400),
+                                                         __builtin_amdgcn_perm(q[e + 1], q[e], 0x0c0c0400), 0x05040100);
+                    *(words_anywhere *)(to + i) = w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (i + e < n) to[i + e] = (signed char)q[e];
                 }
             }
         }
-#pragma unroll
-        for (int j = 0; j < RUNS; ++j)
-#pragma unroll
-            for (int e = 0; e < V; ++e) acc = fma((double)s[j][e], (double)s[j][e], acc);
-        acc = block_all<THREADS, false>(acc, lds);
-        const double r = 1. / sqrt(acc / n + (double)a.eps);
-        auto scales = [&](int i, float g[V]) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) g[e] = 1;
-            if (a.scales && i < n) load_run<DN_F32, V, VECTORS>(a.scales, i, n, g);
-        };
         if (a.output) {
             const float rf = (float)r;
 #pragma unroll
-            for (int j = 0; j < RUNS; ++j) {
-                const int i = (j * THREADS + tid) * V;
-                float y[V], g[V];
-                scales(i, g);
+            for (int j = 0; j < runs; ++j) {
+                float v[V], g[V];
+                values(j, v);
+                scales(j, g);
 #pragma unroll
-                for (int e = 0; e < V; ++e) y[e] = s[j][e] * rf * g[e];
-                if (i < n) store_run<T, V, VECTORS>((E *)a.output + row * n, i, n, y);
+                for (int e = 0; e < V; ++e) v[e] = v[e] * rf * g[e];
+                store_run<E, V>((E *)a.output + row * n, at(j), n, v);
             }
-        }
-        if (!Q8) continue;
-        const int lanes = a.group / V, groups = a.group ? (n + a.group - 1) / a.group : 1;
-        double row_largest = 0;
-        if (a.group == 0) {
-#pragma unroll
-            for (int j = 0; j < RUNS; ++j) {
-                float g[V];
-                scales((j * THREADS + tid) * V, g);
-#pragma unroll
-                for (int e = 0; e < V; ++e) row_largest = fmax(row_largest, finite_abs((double)s[j][e] * r * (double)g[e]));
-            }
-            row_largest = block_all<THREADS, true>(row_largest, lds);
-            if (tid == 0) a.q8_scales[row] = q8_step(row_largest);
-        }
-#pragma unroll
-        for (int j = 0; j < RUNS; ++j) {
-            const int i = (j * THREADS + tid) * V;
-            float g[V];
-            double y[V], largest = 0;
-            scales(i, g);
-#pragma unroll
-            for (int e = 0; e < V; ++e) y[e] = (double)s[j][e] * r * (double)g[e];
-            if (a.group) {
-#pragma unroll
-                for (int e = 0; e < V; ++e) largest = fmax(largest, finite_abs(y[e]));
-                for (int o = 1; o < lanes; o <<= 1) largest = fmax(largest, __shfl_xor(largest, o, 64));
-            } else {
-                largest = row_largest;
-            }
-            const float c = q8_step(largest);
-            const double inv = 1. / (double)c;
-            if (a.group && i < n && (tid & (lanes - 1)) == 0) a.q8_scales[row * groups + i / a.group] = c;
-            if (i >= n) continue;
-            signed char *q = a.q8 + row * n;
-            if (VECTORS) {
-                typedef signed char QV __attribute__((ext_vector_type(V)));
-                QV x;
-#pragma unroll
-                for (int e = 0; e < V; ++e) x[e] = (signed char)q8_code(y[e], c, inv);
-                *(QV *)(q + i) = x;
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; ++e)
-                    if (i + e < n) q[i + e] = (signed char)q8_code(y[e], c, inv);
-            }
-        }
-    }
-}
-
-/* Rows that no workgroup holds in registers: read again for each step. */
-template <int T>
-__global__ __launch_bounds__(1024) void rmsnorm_long_kernel(norm_args a)
-{
-    typedef typename dn_elt<T>::store E;
-    constexpr int THREADS = 1024;
-    __shared__ double lds[THREADS / 64];
-    const int tid = threadIdx.x, n = a.n;
-    for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const E *in = (const E *)a.input + row * n;
-        const E *add = a.add ? (const E *)a.add + row * n : 0;
-        E *sum = a.sum ? (E *)a.sum + row * n : 0;
-        double acc = 0;
-        for (int i = tid; i < n; i += THREADS) {
-            float s = (float)in[i];
-            if (add) s = (float)(E)(s + (float)add[i]);
-            if (sum) sum[i] = (E)s;
-            acc += (double)s * s;
-        }
-        acc = block_all<THREADS, false>(acc, lds);
-        const double r = 1. / sqrt(acc / n + (double)a.eps);
-        /* the sum where it was stored (it may have taken the input's place), else added again */
-        auto value = [&](int i) {
-            if (sum) return (float)sum[i];
-            const float s = (float)in[i];
-            return add ? (float)(E)(s + (float)add[i]) : s;
-        };
-        auto norm = [&](int i) { return (double)value(i) * r * (a.scales ? (double)a.scales[i] : 1.); };
-        if (a.q8) {
-            signed char *q = a.q8 + row * n;
-            if (a.group == 0) {
-                double largest = 0;
-                for (int i = tid; i < n; i += THREADS) largest = fmax(largest, finite_abs(norm(i)));
-                const float c = q8_step(block_all<THREADS, true>(largest, lds));
-                const double inv = 1. / (double)c;
-                if (tid == 0) a.q8_scales[row] = c;
-                for (int i = tid; i < n; i += THREADS) q[i] = (signed char)q8_code(norm(i), c, inv);
-            } else {
-                const int groups = (n + a.group - 1) / a.group;
-                __syncthreads(); /* a group's values may have been stored by another wave */
-                for (int g = tid >> 6; g < groups; g += THREADS / 64) {
-                    const int lo = g * a.group, hi = min(n, lo + a.group);
-                    double largest = 0;
-                    for (int i = lo + (tid & 63); i < hi; i += 64) largest = fmax(largest, finite_abs(norm(i)));
-                    const float c = q8_step(dn_wave_max(largest));
-                    const double inv = 1. / (double)c;
-                    if ((tid & 63) == 0) a.q8_scales[row * groups + g] = c;
-                    for (int i = lo + (tid & 63); i < hi; i += 64) q[i] = (signed char)q8_code(norm(i), c, inv);
-                }
-            }
-        }
-        if (a.output) {
-            E *out = (E *)a.output + row * n;
-            if (a.q8) __syncthreads(); /* it may take the input's place, which the groups above read */
-            for (int i = tid; i < n; i += THREADS) out[i] = (E)(float)norm(i);
         }
     }
 }
 
 /* Which form a row takes: one run a lane up to 256 lanes, then two, so that several rows share a CU and their loads
  * and stores overlap; a row of more than 16384 values is read again for each step. */
-template <int T, bool VECTORS, bool Q8>
+template <int T, bool Q8>
 static void norm_launch(const norm_args &a)
 {
     constexpr int V = T == DN_F32 ? 4 : 8;
     const dim3 grid(a.rows < 65536 ? a.rows : 65536);
     const int runs = (int)(((long)a.n + V - 1) / V);
 #define NM_LAUNCH(THREADS, RUNS) \
-    hipLaunchKernelGGL((rmsnorm_kernel<T, THREADS, RUNS, V, VECTORS, Q8>), grid, dim3(THREADS), 0, dn_stream(), a)
+    hipLaunchKernelGGL((rmsnorm_kernel<T, THREADS, RUNS, V, Q8>), grid, dim3(THREADS), 0, dn_stream(), a)
     if (runs <= 64) NM_LAUNCH(64, 1);
     else if (runs <= 128) NM_LAUNCH(128, 1);
     else if (runs <= 256) NM_LAUNCH(256, 1);
@@ -278,24 +288,8 @@ static void norm_launch(const norm_args &a)
     else if (runs <= 1024) NM_LAUNCH(512, 2);
     else if (runs <= 2048) NM_LAUNCH(1024, 2);
     else if (V == 4 && runs <= 4096) NM_LAUNCH(1024, 16 / V);
-    else hipLaunchKernelGGL((rmsnorm_long_kernel<T>), grid, dim3(1024), 0, dn_stream(), a);
+    else NM_LAUNCH(1024, 0);
 #undef NM_LAUNCH
-}
-
-/* Sixteen-byte runs want rows of whole runs from 16-byte boundaries on (8-bit codes: from V-byte boundaries). */
-template <int T>
-static void norm_launch_type(const norm_args &a)
-{
-    const int v = T == DN_F32 ? 4 : 8;
-    const bool vectors = a.n % v == 0 && dn_aligned(a.input, 16) && dn_aligned(a.add, 16) && dn_aligned(a.sum, 16) &&
-                         dn_aligned(a.output, 16) && dn_aligned(a.scales, 16) && dn_aligned(a.q8, v);
-    if (a.q8) {
-        if (vectors) norm_launch<T, true, true>(a);
-        else norm_launch<T, false, true>(a);
-    } else {
-        if (vectors) norm_launch<T, true, false>(a);
-        else norm_launch<T, false, false>(a);
-    }
 }
 
 extern "C" int forward_rmsnorm_gpu(const void *input, const void *add, const float *scales, void *sum_output,
@@ -319,10 +313,10 @@ extern "C" int forward_rmsnorm_gpu(const void *input, const void *add, const flo
         return dn_refuse(me, "a buffer is not aligned to its element type");
     if (rows == 0) return 0;
     hip_require_device(me);
-    const norm_args a = {input, add, scales, sum_output, output, q8_output, q8_scales, rows, n, q8_group, eps};
-    if (type == DN_F32) norm_launch_type<DN_F32>(a);
-    else if (type == DN_F16) norm_launch_type<DN_F16>(a);
-    else norm_launch_type<DN_BF16>(a);
+    const norm_args a = {input, add, scales, sum_output, output, q8_output, q8_scales, rows, n, q8_group, eps, 1. / n};
+    if (type == DN_F32) q8_output ? norm_launch<DN_F32, true>(a) : norm_launch<DN_F32, false>(a);
+    else if (type == DN_F16) q8_output ? norm_launch<DN_F16, true>(a) : norm_launch<DN_F16, false>(a);
+    else q8_output ? norm_launch<DN_BF16, true>(a) : norm_launch<DN_BF16, false>(a);
     dn_check_launch(me);
     return 0;
 }
