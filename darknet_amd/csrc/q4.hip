@@ -9,8 +9,8 @@
  * a lane.  Dword s of lane r + 16*j holds output r, inputs 32*s + 8*j + i (i = 0..7), which is what that lane
  * gives to the matrix instruction of 16 x 16 x 32; input i stands in the four bits from
  * 4 * (i / 2) + 16 * (i % 2) on, so that a mask leaves two neighbours in the two halves of a register.
- * Behind the codes the scales, [outputs / 16][groups][16] floats, and the zeros, [outputs / 16][inputs / 128]
- * [16][groups in 128] bytes.  What fills the last tiles up has code, scale and zero 0.
+ * Behind the codes the scales, [outputs / 16][inputs / 128][16][groups in 128] floats, and the zeros, the same in
+ * bytes.  What fills the last tiles up has code, scale and zero 0.
  */
 #include <math.h>
 
@@ -56,12 +56,8 @@ __device__ __forceinline__ long q4_dword_at(const q4_shape &s, int o, int k)
 __device__ __forceinline__ int q4_bit_of(int k) { return ((k & 6) << 1) + ((k & 1) << 4); }
 __device__ __forceinline__ long q4_group_at(const q4_shape &s, int o, int g)
 {
-    return ((long)(o >> 4) * s.groups + g) * 16 + (o & 15);
-}
-__device__ __forceinline__ long q4_zero_at(const q4_shape &s, int o, int g)
-{
     const int per = 128 / s.group;
-    return s.zeros_at + (((long)(o >> 4) * s.kblocks + g / per) * 16 + (o & 15)) * per + g % per;
+    return (((long)(o >> 4) * s.kblocks + g / per) * 16 + (o & 15)) * per + g % per;
 }
 
 /* One thread for each (output, 32 inputs) of the filled-up matrix: its four dwords are written by it alone. */
@@ -86,7 +82,7 @@ __global__ void q4_pack_codes_kernel(const unsigned char *codes, const float *sc
             const int g = k0 / s.group;
             const bool in = o < s.outputs && g < groups;
             ((float *)(packed + s.scales_at))[q4_group_at(s, o, g)] = in ? scales[(long)o * groups + g] : 0.f;
-            packed[q4_zero_at(s, o, g)] = in ? (zeros ? zeros[(long)o * groups + g] & 15 : 8) : 0;
+            packed[s.zeros_at + q4_group_at(s, o, g)] = in ? (zeros ? zeros[(long)o * groups + g] & 15 : 8) : 0;
         }
     }
 }
@@ -117,7 +113,7 @@ __global__ void q4_pack_weights_kernel(const float *weights, unsigned char *pack
             ((unsigned *)packed)[q4_dword_at(s, o, lo_k + j * 8)] = v;
         }
         ((float *)(packed + s.scales_at))[q4_group_at(s, o, g)] = scale;
-        packed[q4_zero_at(s, o, g)] = (unsigned char)zero;
+        packed[s.zeros_at + q4_group_at(s, o, g)] = (unsigned char)zero;
     }
 }
 
@@ -128,7 +124,7 @@ __global__ void q4_unpack_kernel(const unsigned char *packed, float *weights, q4
         const int o = (int)(t / s.inputs), k = (int)(t % s.inputs);
         const long at = q4_group_at(s, o, k / s.group);
         const int code = (((const unsigned *)packed)[q4_dword_at(s, o, k)] >> q4_bit_of(k)) & 15;
-        weights[t] = (float)(code - (int)packed[q4_zero_at(s, o, k / s.group)]) * ((const float *)(packed + s.scales_at))[at];
+        weights[t] = (float)(code - (int)packed[s.zeros_at + at]) * ((const float *)(packed + s.scales_at))[at];
     }
 }
 
@@ -182,12 +178,15 @@ extern "C" int q4_unpack_weights_gpu(const void *packed, float *weights, int inp
 }
 
 /* ---- the product --------------------------------------------------------------------------------------
- * On the fp16 matrix instruction: code - zero is a whole number of at most 15, exact in fp16.  A row of the
- * input is scaled by a power of two that brings its largest value to 2^14 .. 2^15 and held as one fp16 value (8-bit,
- * fp16 and bf16 input: exact, short of values 2^-29 below the row's largest) or as the sum of two (fp32 input:
- * to 2^-23 of each value).  Products are exact in the fp32 accumulators, which a group starts
- * from zero; its sum is then multiplied with the scale and added to the output's.  A row with a value that is
- * not finite gets NaN for the factor that undoes its scaling. */
+ * On the fp16 matrix instruction: code - zero is a whole number of at most 15, exact in fp16.  The input is
+ * scaled by a power of two that brings its largest value to 2^14 .. 2^15 and held as one fp16 value (8-bit, fp16
+ * and bf16 input: exact, short of values 2^-29 below the largest) or as the sum of two (fp32 input: to
+ * 2^-23 of each value).  Products are exact in the fp32 accumulators, which a group starts from zero; its sum
+ * is then multiplied with the scale and added to the output's.  Where a value is not finite the factor that
+ * undoes the scaling is NaN.
+ *
+ * The input is the instruction's first operand and the weights the second, so that a lane's results are those
+ * of one output, whose scale and zero it has read beside the codes. */
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
@@ -203,38 +202,34 @@ struct q4_args {
     const float *biases;
     void *output;
     unsigned char *workspace;
-    int input_type, output_type;
+    int output_type;
     int batch, x_group; /* x_group: 0, or the inputs that share one of input_scales */
     int activation;
-    int ksplit;         /* waves of a workgroup that share a row tile, each taking a part of the inputs */
-    int chunk;          /* staged form: 128-input blocks in LDS at a time */
+    int ksplit; /* direct form: waves of a workgroup that share a row tile, each taking a part of the inputs */
     q4_shape s;
 };
 
-/* The exponent a row is scaled by, from the largest of its absolute values' bits; 0x7fffffff: not finite. */
-__device__ __forceinline__ int q4_row_shift(unsigned largest)
+/* The exponent that values are scaled by, from the largest of their absolute values' bits, and the factor that undoes
+ * it: a power of two, NaN if a value is not finite. */
+__device__ __forceinline__ int q4_shift(unsigned largest, float &factor)
 {
-    if (largest >= 0x7f800000u) return 0x7fffffff;
-    if (largest == 0) return 0;
-    int e;
-    (void)frexpf(__uint_as_float(largest), &e); /* largest < 2^e */
-    return 15 - e;
+    int e = 15;
+    if (largest - 1u < 0x7f7fffffu) (void)frexpf(__uint_as_float(largest), &e); /* largest < 2^e */
+    const int shift = min(15 - e, 126);                                        /* 2^-126: the factor is not rounded */
+    factor = largest < 0x7f800000u ? ldexpf(1.f, -shift) : __uint_as_float(0x7fc00000u);
+    return shift;
 }
 
-__device__ __forceinline__ float q4_row_factor(int shift)
-{
-    return shift == 0x7fffffff ? __uint_as_float(0x7fc00000u) : 1.f;
-}
-
-/* Four inputs from k on (zeros behind the row's end). */
+/* Four inputs from k on (zeros behind the row's end), in one access where they exist, whatever their alignment. */
 template <int TI>
-__device__ __forceinline__ void q4_load4(const void *row, int k, int inputs, bool vectors, float x[4])
+__device__ __forceinline__ void q4_load4(const void *row, int k, int inputs, float x[4])
 {
     typedef typename dn_elt<TI>::store E;
     typedef E E4 __attribute__((ext_vector_type(4)));
+    typedef E4 E4U __attribute__((aligned(sizeof(E))));
     const E *p = (const E *)row + k;
-    if (vectors && k + 4 <= inputs) {
-        const E4 v = *(const E4 *)p;
+    if (k + 4 <= inputs) {
+        const E4 v = *(const E4U *)p;
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = (float)v[i];
     } else {
@@ -265,31 +260,36 @@ __device__ __forceinline__ void q4_split4(const float x[4], int shift, half4_t &
 template <int PER>
 struct q4_tile {
     uint4 code;
-    float4_t scale[PER]; /* of the lane's four outputs of the result */
-    unsigned zero;       /* of the lane's output of the operand, a byte for each group */
+    float scale[PER];
+    unsigned zero; /* a byte for each group */
 };
 
 template <int PER>
 __device__ __forceinline__ q4_tile<PER> q4_load_tile(const q4_args &a, int tile, int kb, int lane)
 {
+    typedef float scales_t __attribute__((ext_vector_type(PER)));
     q4_tile<PER> t;
-    const long at = (long)tile * a.s.kblocks + kb;
+    const long at = (long)tile * a.s.kblocks + kb, own = (at * 16 + (lane & 15)) * PER;
     t.code = ((const uint4 *)a.packed)[at * 64 + lane];
+    const float *scale = (const float *)(a.packed + a.s.scales_at) + own;
+    const unsigned char *z = a.packed + a.s.zeros_at + own;
+    if constexpr (PER == 1) {
+        t.scale[0] = *scale;
+        t.zero = *z;
+    } else {
+        const scales_t v = *(const scales_t *)scale;
 #pragma unroll
-    for (int g = 0; g < PER; ++g)
-        t.scale[g] = ((const float4_t *)(a.packed + a.s.scales_at))[(at * PER + g) * 4 + (lane >> 4)];
-    const unsigned char *z = a.packed + a.s.zeros_at + (at * 16 + (lane & 15)) * PER;
-    t.zero = PER == 4 ? *(const unsigned *)z : PER == 2 ? *(const unsigned short *)z : *z;
+        for (int g = 0; g < PER; ++g) t.scale[g] = v[g];
+        t.zero = PER == 4 ? *(const unsigned *)z : *(const unsigned short *)z;
+    }
     return t;
 }
 
 __device__ __forceinline__ half2_t q4_as_half2(unsigned v) { return __builtin_bit_cast(half2_t, v); }
 
 /* Eight codes less their zero as fp16: 0x6400 | c is 1024 + c, and with the code four bits up 1024 + 16 c. */
-__device__ __forceinline__ half8_t q4_unpack8(unsigned v, unsigned zero)
+__device__ __forceinline__ half8_t q4_unpack8(unsigned v, half2_t z1024, half2_t z64)
 {
-    const unsigned z2 = zero | zero << 16;
-    const half2_t z1024 = q4_as_half2(0xe400e400u | z2), z64 = q4_as_half2(0xd400d400u | z2 << 4); /* -(1024 + z), -(64 + z) */
     const half2_t sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
     const unsigned w = v >> 8;
     const half2_t a = q4_as_half2((v & 0x000f000fu) | 0x64006400u) + z1024;
@@ -299,219 +299,211 @@ __device__ __forceinline__ half8_t q4_unpack8(unsigned v, unsigned zero)
     return (half8_t){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-__device__ __forceinline__ float4_t q4_mfma(half8_t a, half8_t b, float4_t c)
+/* Adds the products of R tiles of outputs with T tiles of 16 input rows.  operand(t, piece, step): the lane's eight
+ * inputs of a row; x_scale(t, g): the factors of its four rows of results, where they change along the row (XS). */
+template <int T, int R, int PIECES, int PER, bool XS, class Operand, class Scale>
+__device__ __forceinline__ void q4_multiply(const q4_tile<PER> (&w)[R], float4_t (&sum)[R][T], Operand operand, Scale x_scale)
 {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-
-/* Adds the products of one tile with T tiles of 16 input rows.  operand(t, piece, step): the lane's eight
- * inputs; x_scale(t, g): the input's own scale of the group, where it has one (XG). */
-template <int T, int PIECES, int PER, bool XG, class Operand, class Scale>
-__device__ __forceinline__ void q4_multiply(const q4_tile<PER> &w, float4_t (&sum)[T], Operand operand, Scale x_scale)
-{
-    const unsigned code[4] = {w.code.x, w.code.y, w.code.z, w.code.w};
 #pragma unroll
     for (int g = 0; g < PER; ++g) {
-        float4_t acc[T];
-        const unsigned zero = (w.zero >> (8 * g)) & 0xff;
+        float4_t acc[R][T];
+        half2_t z1024[R], z64[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const unsigned z = (w[r].zero >> (8 * g)) & 0xff, z2 = z | z << 16;
+            z1024[r] = q4_as_half2(0xe400e400u | z2); /* -(1024 + z), -(64 + z) */
+            z64[r] = q4_as_half2(0xd400d400u | z2 << 4);
+        }
 #pragma unroll
         for (int i = 0; i < 4 / PER; ++i) {
             const int step = g * (4 / PER) + i;
-            const half8_t av = q4_unpack8(code[step], zero);
+            half8_t wv[R];
 #pragma unroll
-            for (int t = 0; t < T; ++t) {
-                acc[t] = q4_mfma(av, operand(t, 0, step), i ? acc[t] : (float4_t){0, 0, 0, 0});
-                if (PIECES == 2) acc[t] = q4_mfma(av, operand(t, 1, step), acc[t]);
+            for (int r = 0; r < R; ++r) {
+                const unsigned code = step == 0 ? w[r].code.x : step == 1 ? w[r].code.y : step == 2 ? w[r].code.z : w[r].code.w;
+                wv[r] = q4_unpack8(code, z1024[r], z64[r]);
             }
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+#pragma unroll
+                for (int p = 0; p < PIECES; ++p) {
+                    const half8_t x = operand(t, p, step);
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+                        acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            x, wv[r], i || p ? acc[r][t] : (float4_t){0, 0, 0, 0}, 0, 0, 0);
+                }
         }
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            const float4_t f = XG ? w.scale[g] * x_scale(t, g) : w.scale[g];
-            sum[t] = __builtin_elementwise_fma(acc[t], f, sum[t]);
+            float4_t f = {1, 1, 1, 1};
+            if (XS) f = x_scale(t, g);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float4_t scale = {w[r].scale[g], w[r].scale[g], w[r].scale[g], w[r].scale[g]};
+                sum[r][t] = __builtin_elementwise_fma(acc[r][t], XS ? f * scale : scale, sum[r][t]);
+            }
         }
     }
 }
 
-/* Four neighbouring outputs of one input row: undoes the row's scaling, bias, activation, rounding, store. */
-__device__ __forceinline__ void q4_store4(const q4_args &a, int b, int o, float4_t v, int shift, float factor)
+/* An output: bias, activation, rounding, store. */
+__device__ __forceinline__ void q4_store(const q4_args &a, int b, int o, float y, float bias)
 {
-    if (b >= a.batch) return;
+    y += bias;
+    y = a.activation == DN_LINEAR ? y : dn_activate(y, a.activation);
     const long at = (long)b * a.s.outputs + o;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float y = ldexpf(v[i], -shift) * factor;
-        if (o + i >= a.s.outputs) continue;
-        if (a.biases) y += a.biases[o + i];
-        y = a.activation == DN_LINEAR ? y : dn_activate(y, a.activation);
-        if (a.output_type == DN_F32) ((float *)a.output)[at + i] = y;
-        else if (a.output_type == DN_F16) ((_Float16 *)a.output)[at + i] = (_Float16)y;
-        else ((__bf16 *)a.output)[at + i] = (__bf16)y;
-    }
+    if (a.output_type == DN_F32) ((float *)a.output)[at] = y;
+    else if (a.output_type == DN_F16) ((_Float16 *)a.output)[at] = (_Float16)y;
+    else ((__bf16 *)a.output)[at] = (__bf16)y;
 }
 
-/* Adds what the waves of a row tile have, in the order of the waves, and stores it.  `red`: 8 KB. */
-__device__ __forceinline__ void q4_join(const q4_args &a, float4_t (*red)[64], float4_t own, int tile, int b0, int shift, float factor)
-{
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    if (a.ksplit > 1) {
-        __syncthreads();
-        red[wave][lane] = own;
-        __syncthreads();
-        if (wave % a.ksplit) return;
-        for (int q = 1; q < a.ksplit; ++q) own += red[wave + q][lane];
-    }
-    if (tile < a.s.tiles) q4_store4(a, b0 + (lane & 15), tile * 16 + (lane >> 4) * 4, own, shift, factor);
-}
+__device__ __forceinline__ float q4_bias(const q4_args &a, int o) { return a.biases && o < a.s.outputs ? a.biases[o] : 0.f; }
 
-/* Small input (the whole of it in LDS, at most 16 rows): each workgroup scales and splits the input itself and
- * then streams row tiles of the weights, the next tiles' loads in flight over the current ones' products. */
+/* ---- small input: at most 16 rows that fit into LDS whole.  Each workgroup scales and splits the input itself, block
+ * by block of 128 values, and then streams row tiles of the weights, AHEAD blocks of a wave in flight. */
 template <int TI, int PER, bool XG>
 __global__ __launch_bounds__(Q4_THREADS) void q4_direct_kernel(q4_args a)
 {
     constexpr int PIECES = TI == DN_F32 ? 2 : 1;
-    constexpr int AHEAD = 4; /* blocks in flight */
+    constexpr int AHEAD = PER == 4 ? 6 : 8;
     extern __shared__ char lds[];
-    __shared__ unsigned s_largest[16][Q4_WAVES];
-    __shared__ float4_t s_red[Q4_WAVES][64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ float s_red[Q4_WAVES][16][17];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kpad = a.s.kblocks * 128, pitch = kpad * 2 * PIECES + 16; /* bytes of a row: 16 more, for the banks */
-    const int part = wave % a.ksplit, rows_per = Q4_WAVES / a.ksplit;
+    const int part = wave % a.ksplit, own_tile = wave / a.ksplit, rows_per = Q4_WAVES / a.ksplit;
     const int mine = (a.s.kblocks - part + a.ksplit - 1) / a.ksplit; /* this wave's blocks: part, part + ksplit, ... */
     const int stride = gridDim.x * rows_per;
-    int tile = blockIdx.x * rows_per + wave / a.ksplit;
+    int tile0 = blockIdx.x * rows_per;
 
-    /* block n of this wave in a row tile; one behind the last counts nothing */
-    auto fetch = [&](int t, int n) {
-        q4_tile<PER> w = q4_load_tile<PER>(a, min(t, a.s.tiles - 1), part + a.ksplit * min(n, mine - 1), lane);
-        if (n >= mine)
-#pragma unroll
-            for (int g = 0; g < PER; ++g) w.scale[g] = (float4_t){0, 0, 0, 0};
-        return w;
-    };
+    auto fetch = [&](int t, int n) { return q4_load_tile<PER>(a, min(t, a.s.tiles - 1), part + a.ksplit * n, lane); };
     q4_tile<PER> w[AHEAD];
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) w[u] = fetch(tile, u);
+    for (int u = 0; u < AHEAD; ++u)
+        if (u < mine) w[u] = fetch(tile0 + own_tile, u);
 
+    /* the input: [row][pitch] halves, and [block (8-bit input with groups: group)][16 rows] factors behind them */
     const size_t row_bytes = (size_t)a.s.inputs * (TI == DN_F32 ? 4 : TI == DN_I8 ? 1 : 2);
-    const bool vectors = ((uintptr_t)a.input & 15) == 0 && (row_bytes & 15) == 0;
-    if (TI != DN_I8) {
-        for (int b = 0; b < a.batch; ++b) {
-            unsigned m = 0;
-            for (int k = tid * 4; k < a.s.inputs; k += Q4_THREADS * 4) {
-                float x[4];
-                q4_load4<TI>((const char *)a.input + b * row_bytes, k, a.s.inputs, vectors, x);
-                m = q4_largest4(m, x);
-            }
-            m = dn_wave_max(m);
-            if (lane == 0) s_largest[b][wave] = m;
-        }
-        __syncthreads();
-    }
-    auto shift_of = [&](int b) {
-        if (TI == DN_I8) return 0;
-        unsigned m = s_largest[b][0];
-#pragma unroll
-        for (int w = 1; w < Q4_WAVES; ++w) m = max(m, s_largest[b][w]);
-        return q4_row_shift(m);
-    };
+    float *factors = (float *)(lds + a.batch * pitch);
+    const int quads = kpad / 4;
     for (int b = 0; b < a.batch; ++b) {
-        const int sh = shift_of(b);
-        for (int k = tid * 4; k < kpad; k += Q4_THREADS * 4) {
-            float x[4];
+        const char *row = (const char *)a.input + b * row_bytes;
+#pragma unroll 4
+        for (int q = tid; q < quads; q += Q4_THREADS) { /* 32 lanes have a block */
+            float x[4], factor = 1;
             half4_t hi, lo;
-            q4_load4<TI>((const char *)a.input + b * row_bytes, k, a.s.inputs, vectors, x);
-            q4_split4(x, sh == 0x7fffffff ? 0 : sh, hi, lo);
-            *(half4_t *)(lds + b * pitch + k * 2) = hi;
-            if (PIECES == 2) *(half4_t *)(lds + b * pitch + kpad * 2 + k * 2) = lo;
+            int shift = 0;
+            q4_load4<TI>(row, q * 4, a.s.inputs, x);
+            if (TI != DN_I8) {
+                unsigned m = q4_largest4(0, x);
+                m = max(m, dn_move<0xb1, 0xf>(m, m));
+                m = max(m, dn_move<0x4e, 0xf>(m, m));
+                m = max(m, dn_move<0x141, 0xf>(m, m));
+                m = max(m, dn_move<0x140, 0xf>(m, m));
+                m = max(m, (unsigned)__shfl_xor((int)m, 16, 64));
+                shift = q4_shift(m, factor);
+                if ((tid & 31) == 0) factors[(q >> 5) * 16 + b] = factor;
+            }
+            q4_split4(x, shift, hi, lo);
+            *(half4_t *)(lds + b * pitch + q * 8) = hi;
+            if (PIECES == 2) *(half4_t *)(lds + b * pitch + kpad * 2 + q * 8) = lo;
+        }
+        if (XG) {
+            const int x_groups = (a.s.inputs + a.x_group - 1) / a.x_group;
+            for (int g = tid; g < a.s.groups; g += Q4_THREADS)
+                factors[g * 16 + b] = g < x_groups ? a.input_scales[(long)b * x_groups + g] : 0.f;
         }
     }
-    const int x_groups = XG ? (a.s.inputs + a.x_group - 1) / a.x_group : 1;
-    float *x_scales = (float *)(lds + a.batch * pitch); /* [row][group], only XG */
-    if (XG)
-        for (int i = tid; i < a.batch * a.s.groups; i += Q4_THREADS) {
-            const int b = i / a.s.groups, g = i % a.s.groups;
-            x_scales[i] = g < x_groups ? a.input_scales[(long)b * x_groups + g] : 0.f;
-        }
-    const int col = min(lane & 15, a.batch - 1);
-    int shift = shift_of(col);
-    float factor = TI == DN_I8 ? (XG ? 1.f : a.input_scales[col]) : q4_row_factor(shift);
-    if (shift == 0x7fffffff) shift = 0;
     __syncthreads();
 
-    const char *base = lds + col * pitch + (lane >> 4) * 16;
-    for (; tile - wave / a.ksplit < a.s.tiles; tile += stride) {
-        float4_t sum[1] = {{0, 0, 0, 0}};
+    constexpr bool XS = TI != DN_I8 || XG;
+    const char *base = lds + min(lane & 15, a.batch - 1) * pitch + (lane >> 4) * 16;
+    const float *row_factors = factors + (lane >> 4) * 4;
+    for (; tile0 < a.s.tiles; tile0 += stride) {
+        const int tile = tile0 + own_tile;
+        float4_t sum[1][1] = {{{0, 0, 0, 0}}};
         for (int n = 0; n < mine; n += AHEAD) {
             const bool last = n + AHEAD >= mine; /* what comes next is of the next row tile */
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                const int kb = part + a.ksplit * min(n + u, mine - 1);
-                q4_multiply<1, PIECES, PER, XG>(
-                    w[u], sum,
-                    [&](int, int piece, int step) { return *(const half8_t *)(base + piece * kpad * 2 + kb * 256 + step * 64); },
-                    [&](int, int g) { return x_scales[col * a.s.groups + kb * PER + g]; });
-                w[u] = fetch(last ? tile + stride : tile, last ? u : n + AHEAD + u);
+                if (n + u < mine) {
+                    const int kb = part + a.ksplit * (n + u);
+                    const q4_tile<PER> one[1] = {w[u]};
+                    q4_multiply<1, 1, PIECES, PER, XS>(
+                        one, sum,
+                        [&](int, int piece, int step) { return *(const half8_t *)(base + piece * kpad * 2 + kb * 256 + step * 64); },
+                        [&](int, int g) { return *(const float4_t *)(row_factors + (XG ? kb * PER + g : kb) * 16); });
+                }
+                if (last ? u < mine && tile0 + stride < a.s.tiles : n + AHEAD + u < mine)
+                    w[u] = fetch(last ? tile + stride : tile, last ? u : n + AHEAD + u);
             }
         }
-        q4_join(a, s_red, sum[0], tile, 0, shift, factor);
+        /* what the waves of a row tile have, added in their order; a thread for each output of each row */
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s_red[wave][(lane >> 4) * 4 + i][lane & 15] = sum[0][0][i];
+        __syncthreads();
+        for (int i = tid; i < rows_per * a.batch * 16; i += Q4_THREADS) {
+            const int r = i / (a.batch * 16), b = (i >> 4) % a.batch, o = (tile0 + r) * 16 + (i & 15);
+            if (o >= a.s.outputs) continue;
+            const float bias = q4_bias(a, o);
+            float y = 0;
+#pragma unroll
+            for (int q = 0; q < Q4_WAVES; ++q)
+                if (q < a.ksplit) y += s_red[r * a.ksplit + q][b][i & 15];
+            if (TI == DN_I8 && !XG) y *= a.input_scales[b];
+            q4_store(a, b, o, y, bias);
+        }
     }
 }
 
-/* Larger input, first pass: one workgroup for each row scales it and writes it in the order in which the second
- * pass feeds it to the matrix instruction: [row / 16][inputs / 128][piece][step][lane][8 halves].  Behind that
- * [row] factors and shifts and, for 8-bit input with groups, [row / 16][groups][16] scales. */
-struct q4_space {
-    size_t rows_at, scales_at, bytes;
-};
-
-__host__ __device__ static inline q4_space q4_space_of(const q4_shape &s, int pieces, int batch, bool groups)
+/* ---- larger input, first pass: one workgroup for each row scales it and writes it in the order in which the second
+ * pass feeds it to the matrix instruction: [row / 16][inputs / 128] blocks of [piece][step][lane][8 halves] and, for
+ * 8-bit input with groups, [group in 128][16] factors.  Behind the blocks a factor for each row. */
+__host__ __device__ static inline int q4_block_bytes(const q4_shape &s, int pieces, bool groups)
 {
-    q4_space w;
-    const size_t tiles = ((size_t)batch + 15) / 16;
-    w.rows_at = tiles * s.kblocks * pieces * 4096;
-    w.scales_at = w.rows_at + tiles * 16 * 8;
-    w.bytes = w.scales_at + (groups ? tiles * s.groups * 64 : 0);
-    return w;
+    return pieces * 4096 + (groups ? 128 / s.group * 64 : 0);
 }
 
-template <int TI>
+__host__ __device__ static inline size_t q4_rows_at(const q4_shape &s, int pieces, int batch, bool groups)
+{
+    return ((size_t)batch + 15) / 16 * s.kblocks * q4_block_bytes(s, pieces, groups);
+}
+
+template <int TI, bool XG>
 __global__ __launch_bounds__(256) void q4_prepare_kernel(q4_args a)
 {
     constexpr int PIECES = TI == DN_F32 ? 2 : 1;
     __shared__ unsigned s_largest[4];
-    const int tid = threadIdx.x, b = blockIdx.x;
-    const bool xg = TI == DN_I8 && a.x_group;
-    const q4_space ws = q4_space_of(a.s, PIECES, a.batch, xg);
+    const int tid = threadIdx.x, b = blockIdx.x, block = q4_block_bytes(a.s, PIECES, XG);
     const size_t row_bytes = (size_t)a.s.inputs * (TI == DN_F32 ? 4 : TI == DN_I8 ? 1 : 2);
-    const bool vectors = ((uintptr_t)a.input & 15) == 0 && (row_bytes & 15) == 0;
     const char *row = (const char *)a.input + b * row_bytes;
     int shift = 0;
+    float factor = 1;
     if (TI != DN_I8) {
         unsigned m = 0;
+#pragma unroll 4
         for (int k = tid * 4; k < a.s.inputs; k += 1024) {
             float x[4];
-            q4_load4<TI>(row, k, a.s.inputs, vectors, x);
+            q4_load4<TI>(row, k, a.s.inputs, x);
             m = q4_largest4(m, x);
         }
         m = dn_wave_max(m);
         if ((tid & 63) == 0) s_largest[tid >> 6] = m;
         __syncthreads();
-        shift = q4_row_shift(max(max(s_largest[0], s_largest[1]), max(s_largest[2], s_largest[3])));
+        shift = q4_shift(max(max(s_largest[0], s_largest[1]), max(s_largest[2], s_largest[3])), factor);
     }
-    if (tid == 0) {
-        ((float *)(a.workspace + ws.rows_at))[2 * b] = TI == DN_I8 ? (xg ? 1.f : a.input_scales[b]) : q4_row_factor(shift);
-        ((int *)(a.workspace + ws.rows_at))[2 * b + 1] = shift == 0x7fffffff ? 0 : shift;
-    }
-    if (shift == 0x7fffffff) shift = 0;
-    unsigned char *out = a.workspace + (size_t)(b >> 4) * a.s.kblocks * PIECES * 4096 + (b & 15) * 16;
+    if (tid == 0)
+        ((float *)(a.workspace + q4_rows_at(a.s, PIECES, a.batch, XG)))[b] = TI == DN_I8 ? (XG ? 1.f : a.input_scales[b]) : factor;
+    unsigned char *out = a.workspace + (size_t)(b >> 4) * a.s.kblocks * block + (b & 15) * 16;
     for (int k = tid * 8; k < a.s.kblocks * 128; k += 2048) {
         float x[8];
         half4_t hi[2], lo[2];
-        q4_load4<TI>(row, k, a.s.inputs, vectors, x);
-        q4_load4<TI>(row, k + 4, a.s.inputs, vectors, x + 4);
+        q4_load4<TI>(row, k, a.s.inputs, x);
+        q4_load4<TI>(row, k + 4, a.s.inputs, x + 4);
         q4_split4(x, shift, hi[0], lo[0]);
         q4_split4(x + 4, shift, hi[1], lo[1]);
-        unsigned char *to = out + (size_t)(k >> 7) * PIECES * 4096 + ((k >> 5) & 3) * 1024 + ((k >> 3) & 3) * 256;
+        unsigned char *to = out + (size_t)(k >> 7) * block + ((k >> 5) & 3) * 1024 + ((k >> 3) & 3) * 256;
         ((half4_t *)to)[0] = hi[0];
         ((half4_t *)to)[1] = hi[1];
         if (PIECES == 2) {
@@ -519,140 +511,200 @@ __global__ __launch_bounds__(256) void q4_prepare_kernel(q4_args a)
             ((half4_t *)(to + 4096))[1] = lo[1];
         }
     }
-    if (xg) {
-        const int x_groups = (a.s.inputs + a.x_group - 1) / a.x_group;
-        float *to = (float *)(a.workspace + ws.scales_at) + ((size_t)(b >> 4) * a.s.groups) * 16 + (b & 15);
-        for (int g = tid; g < a.s.groups; g += 256) to[g * 16] = g < x_groups ? a.input_scales[(long)b * x_groups + g] : 0.f;
+    if (XG) {
+        const int x_groups = (a.s.inputs + a.x_group - 1) / a.x_group, per = 128 / a.s.group;
+        unsigned char *to = a.workspace + (size_t)(b >> 4) * a.s.kblocks * block + PIECES * 4096 + (b & 15) * 4;
+        for (int g = tid; g < a.s.groups; g += 256)
+            *(float *)(to + (size_t)(g / per) * block + g % per * 64) = g < x_groups ? a.input_scales[(long)b * x_groups + g] : 0.f;
     }
 }
 
-/* Second pass: a workgroup takes 8 / ksplit * R row tiles and T tiles of 16 input rows.  The input goes through
- * LDS in chunks that all its waves read; each wave's own weights come straight from memory, a chunk ahead. */
-__host__ __device__ constexpr int q4_units(int r, int per) /* blocks of a wave in a chunk, at most */
+/* A lane's results of one tile of outputs and 16 rows, with the rows' own factors. */
+__device__ __forceinline__ void q4_store_tile(const q4_args &a, const float *row_factors, int tile, int b0, float4_t v)
 {
-    return per == 4 ? 2 / r : 4 / r;
+    const int lane = threadIdx.x & 63, o = tile * 16 + (lane & 15);
+    if (o >= a.s.outputs) return;
+    const float bias = q4_bias(a, o);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int b = b0 + (lane >> 4) * 4 + i;
+        if (b < a.batch) q4_store(a, b, o, v[i] * row_factors[b], bias);
+    }
 }
 
+/* ---- second pass, few outputs: a workgroup takes R row tiles and T tiles of input rows, its eight waves an eighth of
+ * the inputs each.  No two waves read the same input, so that it comes straight into registers like the weights, both
+ * a block ahead, and nothing waits for another wave before the end. */
+template <int T, int R, int PIECES, int PER, bool XG>
+__global__ __launch_bounds__(Q4_THREADS) void q4_stream_kernel(q4_args a)
+{
+    __shared__ float4_t s_red[Q4_WAVES][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int block = q4_block_bytes(a.s, PIECES, XG), x_tiles = (a.batch + 15) / 16, x0 = blockIdx.y * T, tile0 = blockIdx.x * R;
+    const int mine = (a.s.kblocks - wave + Q4_WAVES - 1) / Q4_WAVES;
+    struct block_data {
+        q4_tile<PER> w[R];
+        half8_t x[T][PIECES][4];
+        float4_t f[T][PER];
+    };
+    auto fetch = [&](int n, block_data &d) {
+        const int kb = wave + n * Q4_WAVES;
+#pragma unroll
+        for (int r = 0; r < R; ++r) d.w[r] = q4_load_tile<PER>(a, min(tile0 + r, a.s.tiles - 1), kb, lane);
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const unsigned char *p = a.workspace + ((size_t)min(x0 + t, x_tiles - 1) * a.s.kblocks + kb) * block;
+#pragma unroll
+            for (int i = 0; i < 4 * PIECES; ++i) d.x[t][i / 4][i % 4] = *(const half8_t *)(p + i * 1024 + lane * 16);
+            if (XG)
+#pragma unroll
+                for (int g = 0; g < PER; ++g) d.f[t][g] = *(const float4_t *)(p + PIECES * 4096 + g * 64 + (lane >> 4) * 16);
+        }
+    };
+    float4_t sum[R][T];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int t = 0; t < T; ++t) sum[r][t] = (float4_t){0, 0, 0, 0};
+    auto multiply = [&](const block_data &d) {
+        q4_multiply<T, R, PIECES, PER, XG>(
+            d.w, sum, [&](int t, int piece, int step) { return d.x[t][piece][step]; }, [&](int t, int g) { return d.f[t][g]; });
+    };
+    block_data one, two;
+    if (mine > 0) fetch(0, one);
+    for (int n = 0; n < mine; n += 2) {
+        if (n + 1 < mine) fetch(n + 1, two);
+        multiply(one);
+        if (n + 2 < mine) fetch(n + 2, one);
+        if (n + 1 < mine) multiply(two);
+    }
+    /* the waves' sums, in their order; each wave joins what falls to it */
+    const float *row_factors = (const float *)(a.workspace + q4_rows_at(a.s, PIECES, a.batch, XG));
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            __syncthreads();
+            s_red[wave][lane] = sum[r][t];
+            __syncthreads();
+            if (wave == (r * T + t) % Q4_WAVES && tile0 + r < a.s.tiles && x0 + t < x_tiles) {
+                float4_t v = s_red[0][lane];
+#pragma unroll
+                for (int q = 1; q < Q4_WAVES; ++q) v += s_red[q][lane];
+                q4_store_tile(a, row_factors, tile0 + r, (x0 + t) * 16, v);
+            }
+        }
+}
+
+/* ---- second pass, many outputs: a workgroup takes 8 * R row tiles, R for each wave, and T tiles of input rows.  The
+ * input goes through LDS in chunks that all waves read, the next chunk on its way (through registers) during the
+ * products of the present one; each wave's weights come straight from memory, a chunk ahead as well. */
 template <int T, int R, int PIECES, int PER, bool XG>
 __global__ __launch_bounds__(Q4_THREADS) void q4_staged_kernel(q4_args a)
 {
-    constexpr int UNITS = q4_units(R, PER);
-    extern __shared__ char lds[];
-    __shared__ float4_t s_red[Q4_WAVES][64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const q4_space ws = q4_space_of(a.s, PIECES, a.batch, XG);
-    const int part = wave % a.ksplit, x_tiles = (a.batch + 15) / 16, x0 = blockIdx.y * T;
-    const int tile0 = (blockIdx.x * (Q4_WAVES / a.ksplit) + wave / a.ksplit) * R;
-    const int units = a.chunk / a.ksplit, chunks = (a.s.kblocks + a.chunk - 1) / a.chunk;
-    const float *x_scales = (const float *)(a.workspace + ws.scales_at);
+    constexpr int UNITS = 4 / (T * PIECES > 4 ? 4 : T * PIECES); /* blocks of a chunk */
+    constexpr int BLOCK = PIECES * 4096 + (XG ? PER * 64 : 0), SPAN = UNITS * BLOCK, CHUNK = T * SPAN;
+    constexpr int MOVES = (CHUNK + Q4_THREADS * 16 - 1) / (Q4_THREADS * 16);
+    __shared__ uint4 s_input[2][CHUNK / 16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int x_tiles = (a.batch + 15) / 16, x0 = blockIdx.y * T, tile0 = (blockIdx.x * Q4_WAVES + wave) * R;
+    const int kblocks = a.s.kblocks, chunks = (kblocks + UNITS - 1) / UNITS;
     float4_t sum[R][T];
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int t = 0; t < T; ++t) sum[r][t] = (float4_t){0, 0, 0, 0};
 
-    auto fetch = [&](int c, int u, int r) {
-        const int kb = c * a.chunk + part + u * a.ksplit;
-        q4_tile<PER> w = q4_load_tile<PER>(a, min(tile0 + r, a.s.tiles - 1), min(kb, a.s.kblocks - 1), lane);
-        if (kb >= a.s.kblocks)
+    uint4 moved[MOVES];
+    auto input_of = [&](int c) {
 #pragma unroll
-            for (int g = 0; g < PER; ++g) w.scale[g] = (float4_t){0, 0, 0, 0};
-        return w;
+        for (int m = 0; m < MOVES; ++m) { /* what lies behind the last block or tile is read at its place, and not multiplied */
+            const int i = min((m * Q4_THREADS + tid) * 16, CHUNK - 16), t = i / SPAN, in = i % SPAN;
+            const int kb = min(c * UNITS + in / BLOCK, kblocks - 1);
+            moved[m] = *(const uint4 *)(a.workspace + ((size_t)min(x0 + t, x_tiles - 1) * kblocks + kb) * BLOCK + in % BLOCK);
+        }
+    };
+    auto keep_input = [&](int buffer) {
+#pragma unroll
+        for (int m = 0; m < MOVES; ++m)
+            if ((m * Q4_THREADS + tid) * 16 < CHUNK) s_input[buffer][m * Q4_THREADS + tid] = moved[m];
     };
     q4_tile<PER> w[UNITS][R];
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u)
+    auto fetch = [&](int c, int u) {
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            if (u < units) w[u][r] = fetch(0, u, r);
-    const int block = PIECES * 4096, span = a.chunk * block; /* bytes of one input tile's block, and of its chunk */
+            w[u][r] = q4_load_tile<PER>(a, min(tile0 + r, a.s.tiles - 1), min(c * UNITS + u, kblocks - 1), lane);
+    };
+    input_of(0);
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) fetch(0, u);
+    keep_input(0);
+    __syncthreads();
     for (int c = 0; c < chunks; ++c) {
-        /* stage chunk c: blocks behind the last are not read by a product with a scale, but must be finite */
-        __syncthreads();
-        for (int i = tid * 16; i < T * span; i += Q4_THREADS * 16) {
-            const int t = i / span, in = i % span, kb = c * a.chunk + in / block;
-            uint4 v = {0, 0, 0, 0};
-            if (x0 + t < x_tiles && kb < a.s.kblocks)
-                v = *(const uint4 *)(a.workspace + ((size_t)(x0 + t) * a.s.kblocks + c * a.chunk) * block + in);
-            *(uint4 *)(lds + i) = v;
-        }
-        __syncthreads();
+        if (c + 1 < chunks) input_of(c + 1);
+        const char *base = (const char *)s_input[c & 1];
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
-            if (u >= units) break;
-            const int at = part + u * a.ksplit, kb = min(c * a.chunk + at, a.s.kblocks - 1);
-            const char *base = lds + at * block + lane * 16;
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                q4_multiply<T, PIECES, PER, XG>(
-                    w[u][r], sum[r],
-                    [&](int t, int piece, int step) { return *(const half8_t *)(base + t * span + piece * 4096 + step * 1024); },
-                    [&](int t, int g) {
-                        return x_scales[((size_t)min(x0 + t, x_tiles - 1) * a.s.groups + kb * PER + g) * 16 + (lane & 15)];
-                    });
-                w[u][r] = fetch(c + 1, u, r);
-            }
+            if (c * UNITS + u < kblocks)
+                q4_multiply<T, R, PIECES, PER, XG>(
+                    w[u], sum,
+                    [&](int t, int piece, int step) {
+                        return *(const half8_t *)(base + t * SPAN + u * BLOCK + piece * 4096 + step * 1024 + lane * 16);
+                    },
+                    [&](int t, int g) { return *(const float4_t *)(base + t * SPAN + u * BLOCK + PIECES * 4096 + g * 64 + (lane >> 4) * 16); });
+            if (c + 1 < chunks) fetch(c + 1, u);
         }
+        if (c + 1 < chunks) keep_input((c + 1) & 1); /* the buffer that all waves have left at the last barrier */
+        __syncthreads();
     }
+    const float *row_factors = (const float *)(a.workspace + q4_rows_at(a.s, PIECES, a.batch, XG));
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
-        const int b0 = (x0 + t) * 16, b = min(b0 + (lane & 15), a.batch - 1);
-        const float factor = ((const float *)(a.workspace + ws.rows_at))[2 * b];
-        const int shift = ((const int *)(a.workspace + ws.rows_at))[2 * b + 1];
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int r = 0; r < R; ++r) q4_join(a, s_red, sum[r][t], tile0 + r, b0, shift, factor);
-    }
+        for (int t = 0; t < T; ++t)
+            if (tile0 + r < a.s.tiles && x0 + t < x_tiles) q4_store_tile(a, row_factors, tile0 + r, (x0 + t) * 16, sum[r][t]);
 }
 
-/* Which form a product takes.  Direct: up to 16 rows and 16384 inputs in all (what a workgroup can scale while its
- * first weights arrive). */
+/* Which form a product takes.
+ *   direct  up to 16 rows and 16384 inputs in all: what a workgroup can scale while its first weights arrive
+ *   staged  so many outputs that workgroups of 128 (R = 1) or 256 (R = 2) of them fill the chip
+ *   stream  the others */
 struct q4_plan {
-    bool direct;
-    int pieces, ksplit, t, r, chunk;
+    enum { DIRECT, STREAM, STAGED } form;
+    int ksplit, t, r;
     unsigned gx, gy;
     size_t lds;
 };
 
-static q4_plan q4_plan_of(const q4_shape &s, int type, int batch, bool xg)
+static q4_plan q4_plan_of(const q4_shape &s, int type, int batch)
 {
     q4_plan p;
-    p.pieces = type == DN_F32 ? 2 : 1;
-    p.t = p.r = p.chunk = 1;
+    const int pieces = type == DN_F32 ? 2 : 1, x_tiles = (batch + 15) / 16;
+    p.ksplit = p.t = p.r = 1;
     p.gy = 1;
-    const size_t pitch = (size_t)s.kblocks * 256 * p.pieces + 16, need = batch * (pitch + (xg ? (size_t)s.groups * 4 : 0));
-    p.direct = batch <= 16 && (long)batch * s.inputs <= 16384 && need <= 128 << 10;
-    if (p.direct) {
-        p.lds = need;
-        /* waves share a row tile as long as that leaves each of them a block and the chip is not full */
-        p.ksplit = 1;
+    p.lds = batch * ((size_t)s.kblocks * 256 * pieces + 16) + (size_t)(type == DN_I8 ? s.groups : s.kblocks) * 64;
+    if (batch <= 16 && (long)batch * s.inputs <= 16384 && p.lds <= 120 << 10) {
+        p.form = q4_plan::DIRECT;
+        /* waves share a row tile as long as each has a block and the chip is not full */
         while (p.ksplit < 8 && (long)s.tiles * p.ksplit < 256 * Q4_WAVES && p.ksplit * 2 <= s.kblocks) p.ksplit *= 2;
-        const int groups = (s.tiles * p.ksplit + Q4_WAVES - 1) / Q4_WAVES;
-        p.gx = groups < 512 ? groups : 512;
+        const long groups = ((long)s.tiles * p.ksplit + Q4_WAVES - 1) / Q4_WAVES;
+        p.gx = (unsigned)(groups < 512 ? groups : 512);
         return p;
     }
-    const int x_tiles = (batch + 15) / 16, passes = (x_tiles + 3) / 4;
-    auto grid = [&]() {
-        const int per = Q4_WAVES / p.ksplit * p.r;
-        p.gx = (unsigned)((s.tiles + per - 1) / per);
-        p.gy = (unsigned)((x_tiles + p.t - 1) / p.t);
-        return (long)p.gx * p.gy;
-    };
-    p.t = (x_tiles + passes - 1) / passes;
-    p.ksplit = 1;
-    p.r = 2;
-    if (grid() < 256) p.r = 1;
-    while (grid() < 256 && p.ksplit < 8) {
-        if (p.t * p.pieces * p.ksplit * 2 <= 16) p.ksplit *= 2;
-        else if (p.t > 1) p.t = (p.t + 1) / 2;
-        else break;
+    p.lds = 0;
+    const int passes = (x_tiles + 3) / 4;
+    if (s.tiles >= 8 * 192) {
+        p.form = q4_plan::STAGED;
+        p.t = (x_tiles + passes - 1) / passes;
+        p.r = s.tiles >= 16 * 192 ? 2 : 1;
+        p.gx = (unsigned)((s.tiles + Q4_WAVES * p.r - 1) / (Q4_WAVES * p.r));
+    } else {
+        p.form = q4_plan::STREAM;
+        p.t = pieces == 1 && x_tiles > 1 ? 2 : 1;
+        p.r = s.tiles >= 2 * 192 ? 2 : 1;
+        p.gx = (unsigned)((s.tiles + p.r - 1) / p.r);
     }
-    grid();
-    const int most = 16 / (p.t * p.pieces) > 0 ? 16 / (p.t * p.pieces) : 1; /* blocks in 64 KB */
-    p.chunk = most / p.ksplit * p.ksplit;
-    if (p.chunk < p.ksplit) p.chunk = p.ksplit;
-    const int units = q4_units(p.r, 128 / s.group);
-    if (p.chunk > units * p.ksplit) p.chunk = units * p.ksplit;
-    p.lds = (size_t)p.t * p.chunk * p.pieces * 4096;
+    p.gy = (unsigned)((x_tiles + p.t - 1) / p.t);
     return p;
 }
 
@@ -660,37 +712,38 @@ extern "C" size_t connected_q4_workspace_bytes(int input_type, int batch, int in
 {
     if (!q4_shape_ok(inputs, outputs, group) || batch < 1) return 0;
     const q4_shape s = q4_shape_of(inputs, outputs, group);
-    if (q4_plan_of(s, input_type, batch, input_type == DN_I8).direct) return 0;
-    return q4_space_of(s, input_type == DN_F32 ? 2 : 1, batch, input_type == DN_I8).bytes;
+    if (q4_plan_of(s, input_type, batch).form == q4_plan::DIRECT) return 0;
+    return q4_rows_at(s, input_type == DN_F32 ? 2 : 1, batch, input_type == DN_I8) + (size_t)batch * 4;
 }
 
-template <int TI, int PER, bool XG>
-static void q4_launch_direct(const q4_args &a, const q4_plan &p)
-{
-    hipLaunchKernelGGL((q4_direct_kernel<TI, PER, XG>), dim3(p.gx), dim3(Q4_THREADS), p.lds, dn_stream(), a);
-}
-
-template <int T, int PIECES, int PER, bool XG>
-static void q4_launch_staged(const q4_args &a, const q4_plan &p)
+template <int T, int R, int PIECES, int PER, bool XG>
+static void q4_launch_second(const q4_args &a, const q4_plan &p)
 {
     const dim3 grid(p.gx, p.gy), block(Q4_THREADS);
-    if (p.r == 2) hipLaunchKernelGGL((q4_staged_kernel<T, 2, PIECES, PER, XG>), grid, block, p.lds, dn_stream(), a);
-    else hipLaunchKernelGGL((q4_staged_kernel<T, 1, PIECES, PER, XG>), grid, block, p.lds, dn_stream(), a);
+    if (p.form == q4_plan::STAGED) hipLaunchKernelGGL((q4_staged_kernel<T, R, PIECES, PER, XG>), grid, block, 0, dn_stream(), a);
+    else if constexpr (T * PIECES <= 2) hipLaunchKernelGGL((q4_stream_kernel<T, R, PIECES, PER, XG>), grid, block, 0, dn_stream(), a);
 }
 
 template <int TI, int PER, bool XG>
 static void q4_launch(const q4_args &a, const q4_plan &p)
 {
     constexpr int PIECES = TI == DN_F32 ? 2 : 1;
-    if (p.direct) {
-        q4_launch_direct<TI, PER, XG>(a, p);
+    if (p.form == q4_plan::DIRECT) {
+        hipLaunchKernelGGL((q4_direct_kernel<TI, PER, XG>), dim3(p.gx), dim3(Q4_THREADS), p.lds, dn_stream(), a);
         return;
     }
-    hipLaunchKernelGGL((q4_prepare_kernel<TI>), dim3((unsigned)a.batch), dim3(256), 0, dn_stream(), a);
-    if (p.t == 1) q4_launch_staged<1, PIECES, PER, XG>(a, p);
-    else if (p.t == 2) q4_launch_staged<2, PIECES, PER, XG>(a, p);
-    else if (p.t == 3) q4_launch_staged<3, PIECES, PER, XG>(a, p);
-    else q4_launch_staged<4, PIECES, PER, XG>(a, p);
+    hipLaunchKernelGGL((q4_prepare_kernel<TI, XG>), dim3((unsigned)a.batch), dim3(256), 0, dn_stream(), a);
+    if (p.r == 2) {
+        if (p.t == 1) q4_launch_second<1, 2, PIECES, PER, XG>(a, p);
+        else if (p.t == 2) q4_launch_second<2, 2, PIECES, PER, XG>(a, p);
+        else if (p.t == 3) q4_launch_second<3, 2, PIECES, PER, XG>(a, p);
+        else q4_launch_second<4, 2, PIECES, PER, XG>(a, p);
+    } else {
+        if (p.t == 1) q4_launch_second<1, 1, PIECES, PER, XG>(a, p);
+        else if (p.t == 2) q4_launch_second<2, 1, PIECES, PER, XG>(a, p);
+        else if (p.t == 3) q4_launch_second<3, 1, PIECES, PER, XG>(a, p);
+        else q4_launch_second<4, 1, PIECES, PER, XG>(a, p);
+    }
 }
 
 template <int TI, bool XG>
@@ -720,12 +773,12 @@ extern "C" int forward_connected_q4_gpu(const void *input, int input_type, const
     if (batch == 0) return 0;
     const q4_shape s = q4_shape_of(inputs, outputs, group);
     const bool xg = input_type == DN_I8 && input_group != 0;
-    const q4_plan p = q4_plan_of(s, input_type, batch, input_type == DN_I8);
-    if (!p.direct && !workspace) return dn_refuse(me, "the workspace is missing");
+    const q4_plan p = q4_plan_of(s, input_type, batch);
+    if (p.form != q4_plan::DIRECT && !workspace) return dn_refuse(me, "the workspace is missing");
     if (p.gx > 0x7fffffu || p.gy > 65535u) return dn_refuse(me, "too many outputs or rows for one call");
     hip_require_device(me);
     const q4_args a = {input, input_scales, (const unsigned char *)packed, biases, output, (unsigned char *)workspace,
-                       input_type, output_type, batch, xg ? input_group : 0, activation, p.ksplit, p.chunk, s};
+                       output_type, batch, xg ? input_group : 0, activation, p.ksplit, s};
     if (input_type == DN_F32) q4_launch_group<DN_F32, false>(a, p);
     else if (input_type == DN_F16) q4_launch_group<DN_F16, false>(a, p);
     else if (input_type == DN_BF16) q4_launch_group<DN_BF16, false>(a, p);
