@@ -191,6 +191,7 @@ typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef unsigned uint4_t __attribute__((ext_vector_type(4)));
 
 #define Q4_THREADS 512 /* 8 waves */
 #define Q4_WAVES 8
@@ -259,7 +260,7 @@ __device__ __forceinline__ void q4_split4(const float x[4], int shift, half4_t &
 /* One tile of 16 outputs x 128 inputs as a lane holds it; PER groups in 128 inputs. */
 template <int PER>
 struct q4_tile {
-    uint4 code;
+    uint4_t code;
     float scale[PER];
     unsigned zero; /* a byte for each group */
 };
@@ -270,7 +271,7 @@ __device__ __forceinline__ q4_tile<PER> q4_load_tile(const q4_args &a, int tile,
     typedef float scales_t __attribute__((ext_vector_type(PER)));
     q4_tile<PER> t;
     const long at = (long)tile * a.s.kblocks + kb, own = (at * 16 + (lane & 15)) * PER;
-    t.code = ((const uint4 *)a.packed)[at * 64 + lane];
+    t.code = ((const uint4_t *)a.packed)[at * 64 + lane];
     const float *scale = (const float *)(a.packed + a.s.scales_at) + own;
     const unsigned char *z = a.packed + a.s.zeros_at + own;
     if constexpr (PER == 1) {
@@ -287,15 +288,23 @@ __device__ __forceinline__ q4_tile<PER> q4_load_tile(const q4_args &a, int tile,
 
 __device__ __forceinline__ half2_t q4_as_half2(unsigned v) { return __builtin_bit_cast(half2_t, v); }
 
+/* (v & mask) | 0x64006400 in one instruction, which takes no two constants: the second comes in a register. */
+__device__ __forceinline__ half2_t q4_pick(unsigned v, unsigned mask, unsigned magic)
+{
+    unsigned d;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(d) : "v"(v), "s"(mask), "v"(magic));
+    return q4_as_half2(d);
+}
+
 /* Eight codes less their zero as fp16: 0x6400 | c is 1024 + c, and with the code four bits up 1024 + 16 c. */
-__device__ __forceinline__ half8_t q4_unpack8(unsigned v, half2_t z1024, half2_t z64)
+__device__ __forceinline__ half8_t q4_unpack8(unsigned v, half2_t z1024, half2_t z64, unsigned magic)
 {
     const half2_t sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
     const unsigned w = v >> 8;
-    const half2_t a = q4_as_half2((v & 0x000f000fu) | 0x64006400u) + z1024;
-    const half2_t b = __builtin_elementwise_fma(q4_as_half2((v & 0x00f000f0u) | 0x64006400u), sixteenth, z64);
-    const half2_t c = q4_as_half2((w & 0x000f000fu) | 0x64006400u) + z1024;
-    const half2_t d = __builtin_elementwise_fma(q4_as_half2((w & 0x00f000f0u) | 0x64006400u), sixteenth, z64);
+    const half2_t a = q4_pick(v, 0x000f000fu, magic) + z1024;
+    const half2_t b = __builtin_elementwise_fma(q4_pick(v, 0x00f000f0u, magic), sixteenth, z64);
+    const half2_t c = q4_pick(w, 0x000f000fu, magic) + z1024;
+    const half2_t d = __builtin_elementwise_fma(q4_pick(w, 0x00f000f0u, magic), sixteenth, z64);
     return (half8_t){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
@@ -304,6 +313,8 @@ __device__ __forceinline__ half8_t q4_unpack8(unsigned v, half2_t z1024, half2_t
 template <int T, int R, int PIECES, int PER, bool XS, class Operand, class Scale>
 __device__ __forceinline__ void q4_multiply(const q4_tile<PER> (&w)[R], float4_t (&sum)[R][T], Operand operand, Scale x_scale)
 {
+    unsigned magic = 0x64006400u;
+    asm("" : "+v"(magic));
 #pragma unroll
     for (int g = 0; g < PER; ++g) {
         float4_t acc[R][T];
@@ -321,7 +332,7 @@ __device__ __forceinline__ void q4_multiply(const q4_tile<PER> (&w)[R], float4_t
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 const unsigned code = step == 0 ? w[r].code.x : step == 1 ? w[r].code.y : step == 2 ? w[r].code.z : w[r].code.w;
-                wv[r] = q4_unpack8(code, z1024[r], z64[r]);
+                wv[r] = q4_unpack8(code, z1024[r], z64[r], magic);
             }
 #pragma unroll
             for (int t = 0; t < T; ++t)
@@ -388,7 +399,6 @@ __global__ __launch_bounds__(Q4_THREADS) void q4_direct_kernel(q4_args a)
     const int quads = kpad / 4;
     for (int b = 0; b < a.batch; ++b) {
         const char *row = (const char *)a.input + b * row_bytes;
-#pragma unroll 4
         for (int q = tid; q < quads; q += Q4_THREADS) { /* 32 lanes have a block */
             float x[4], factor = 1;
             half4_t hi, lo;
@@ -525,10 +535,11 @@ __device__ __forceinline__ void q4_store_tile(const q4_args &a, const float *row
     const int lane = threadIdx.x & 63, o = tile * 16 + (lane & 15);
     if (o >= a.s.outputs) return;
     const float bias = q4_bias(a, o);
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < 4; ++i) {
         const int b = b0 + (lane >> 4) * 4 + i;
-        if (b < a.batch) q4_store(a, b, o, v[i] * row_factors[b], bias);
+        const float y = i == 0 ? v[0] : i == 1 ? v[1] : i == 2 ? v[2] : v[3];
+        if (b < a.batch) q4_store(a, b, o, y * row_factors[b], bias);
     }
 }
 
@@ -580,34 +591,49 @@ __global__ __launch_bounds__(Q4_THREADS) void q4_stream_kernel(q4_args a)
     }
     /* the waves' sums, in their order; each wave joins what falls to it */
     const float *row_factors = (const float *)(a.workspace + q4_rows_at(a.s, PIECES, a.batch, XG));
+#pragma unroll 1
+    for (int k = 0; k < R * T; ++k) {
+        float4_t v = sum[0][0];
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+        for (int m = 1; m < R * T; ++m) v = k == m ? sum[m / T][m % T] : v;
+        __syncthreads();
+        s_red[wave][lane] = v;
+        __syncthreads();
+        if (wave == k && tile0 + k / T < a.s.tiles && x0 + k % T < x_tiles) { /* R * T <= 8 */
+            v = s_red[0][lane];
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
-            __syncthreads();
-            s_red[wave][lane] = sum[r][t];
-            __syncthreads();
-            if (wave == (r * T + t) % Q4_WAVES && tile0 + r < a.s.tiles && x0 + t < x_tiles) {
-                float4_t v = s_red[0][lane];
-#pragma unroll
-                for (int q = 1; q < Q4_WAVES; ++q) v += s_red[q][lane];
-                q4_store_tile(a, row_factors, tile0 + r, (x0 + t) * 16, v);
-            }
+            for (int q = 1; q < Q4_WAVES; ++q) v += s_red[q][lane];
+            q4_store_tile(a, row_factors, tile0 + k / T, (x0 + k % T) * 16, v);
         }
+    }
 }
 
-/* ---- second pass, many outputs: a workgroup takes 8 * R row tiles, R for each wave, and T tiles of input rows.  The
+/* Stores 16 rows of WIDTH outputs from LDS. */
+template <int THREADS, int WIDTH, int PITCH>
+__device__ __forceinline__ void q4_store_rows(const q4_args &a, const float *s_sum, const float *row_factors, int b0, int o0)
+{
+    const int rows = min(16, a.batch - b0);
+#pragma unroll 2
+    for (int i = threadIdx.x; i < rows * WIDTH; i += THREADS) {
+        const int row = i / WIDTH, o = o0 + i % WIDTH;
+        if (o < a.s.outputs) q4_store(a, b0 + row, o, s_sum[row * PITCH + i % WIDTH] * row_factors[b0 + row], q4_bias(a, o));
+    }
+}
+
+/* ---- second pass, many outputs: a workgroup takes 4 * R row tiles, R for each wave, and T tiles of input rows.  The
  * input goes through LDS in chunks that all waves read, the next chunk on its way (through registers) during the
  * products of the present one; each wave's weights come straight from memory, a chunk ahead as well. */
+#define Q4_STAGED_WAVES 4
 template <int T, int R, int PIECES, int PER, bool XG>
-__global__ __launch_bounds__(Q4_THREADS) void q4_staged_kernel(q4_args a)
+__global__ __launch_bounds__(Q4_STAGED_WAVES * 64, 2) void q4_staged_kernel(q4_args a)
 {
+    constexpr int THREADS = Q4_STAGED_WAVES * 64;
     constexpr int UNITS = 4 / (T * PIECES > 4 ? 4 : T * PIECES); /* blocks of a chunk */
     constexpr int BLOCK = PIECES * 4096 + (XG ? PER * 64 : 0), SPAN = UNITS * BLOCK, CHUNK = T * SPAN;
-    constexpr int MOVES = (CHUNK + Q4_THREADS * 16 - 1) / (Q4_THREADS * 16);
-    __shared__ uint4 s_input[2][CHUNK / 16];
+    constexpr int MOVES = (CHUNK + THREADS * 16 - 1) / (THREADS * 16);
+    __shared__ uint4_t s_input[2][CHUNK / 16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int x_tiles = (a.batch + 15) / 16, x0 = blockIdx.y * T, tile0 = (blockIdx.x * Q4_WAVES + wave) * R;
+    const int x_tiles = (a.batch + 15) / 16, x0 = blockIdx.y * T, tile0 = (blockIdx.x * Q4_STAGED_WAVES + wave) * R;
     const int kblocks = a.s.kblocks, chunks = (kblocks + UNITS - 1) / UNITS;
     float4_t sum[R][T];
 #pragma unroll
@@ -615,19 +641,19 @@ __global__ __launch_bounds__(Q4_THREADS) void q4_staged_kernel(q4_args a)
 #pragma unroll
         for (int t = 0; t < T; ++t) sum[r][t] = (float4_t){0, 0, 0, 0};
 
-    uint4 moved[MOVES];
+    uint4_t moved[MOVES];
     auto input_of = [&](int c) {
 #pragma unroll
         for (int m = 0; m < MOVES; ++m) { /* what lies behind the last block or tile is read at its place, and not multiplied */
-            const int i = min((m * Q4_THREADS + tid) * 16, CHUNK - 16), t = i / SPAN, in = i % SPAN;
+            const int i = min((m * THREADS + tid) * 16, CHUNK - 16), t = i / SPAN, in = i % SPAN;
             const int kb = min(c * UNITS + in / BLOCK, kblocks - 1);
-            moved[m] = *(const uint4 *)(a.workspace + ((size_t)min(x0 + t, x_tiles - 1) * kblocks + kb) * BLOCK + in % BLOCK);
+            moved[m] = *(const uint4_t *)(a.workspace + ((size_t)min(x0 + t, x_tiles - 1) * kblocks + kb) * BLOCK + in % BLOCK);
         }
     };
     auto keep_input = [&](int buffer) {
 #pragma unroll
         for (int m = 0; m < MOVES; ++m)
-            if ((m * Q4_THREADS + tid) * 16 < CHUNK) s_input[buffer][m * Q4_THREADS + tid] = moved[m];
+            if ((m * THREADS + tid) * 16 < CHUNK) s_input[buffer][m * THREADS + tid] = moved[m];
     };
     q4_tile<PER> w[UNITS][R];
     auto fetch = [&](int c, int u) {
@@ -657,17 +683,32 @@ __global__ __launch_bounds__(Q4_THREADS) void q4_staged_kernel(q4_args a)
         if (c + 1 < chunks) keep_input((c + 1) & 1); /* the buffer that all waves have left at the last barrier */
         __syncthreads();
     }
+    /* The sums go through LDS, a tile of input rows at a time, so that neighbouring lanes store neighbouring outputs
+     * (16 of a row alone are half a line) and there is one copy of the activation's code. */
     const float *row_factors = (const float *)(a.workspace + q4_rows_at(a.s, PIECES, a.batch, XG));
+    constexpr int WIDTH = Q4_STAGED_WAVES * R * 16, PITCH = WIDTH + 4;
+    static_assert(sizeof s_input >= 16 * PITCH * 4, "room for a tile's sums");
+    float *s_sum = (float *)s_input;
+    const int o0 = blockIdx.x * WIDTH;
+#pragma unroll 1
+    for (int x = 0; x < T; ++x) {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+        for (int r = 0; r < R; ++r) {
+            float4_t v = sum[r][0];
 #pragma unroll
-        for (int t = 0; t < T; ++t)
-            if (tile0 + r < a.s.tiles && x0 + t < x_tiles) q4_store_tile(a, row_factors, tile0 + r, (x0 + t) * 16, sum[r][t]);
+            for (int m = 1; m < T; ++m) v = x == m ? sum[r][m] : v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s_sum[((lane >> 4) * 4 + i) * PITCH + (wave * R + r) * 16 + (lane & 15)] = v[i];
+        }
+        __syncthreads();
+        q4_store_rows<THREADS, WIDTH, PITCH>(a, s_sum, row_factors, (x0 + x) * 16, o0);
+        __syncthreads();
+    }
 }
 
 /* Which form a product takes.
  *   direct  up to 16 rows and 16384 inputs in all: what a workgroup can scale while its first weights arrive
- *   staged  so many outputs that workgroups of 128 (R = 1) or 256 (R = 2) of them fill the chip
+ *   staged  so many outputs that workgroups of 64 (R = 1) or 128 (R = 2) of them fill the chip
  *   stream  the others */
 struct q4_plan {
     enum { DIRECT, STREAM, STAGED } form;
@@ -693,15 +734,16 @@ static q4_plan q4_plan_of(const q4_shape &s, int type, int batch)
     }
     p.lds = 0;
     const int passes = (x_tiles + 3) / 4;
-    if (s.tiles >= 8 * 192) {
+    if (s.tiles >= Q4_STAGED_WAVES * 384) {
         p.form = q4_plan::STAGED;
         p.t = (x_tiles + passes - 1) / passes;
-        p.r = s.tiles >= 16 * 192 ? 2 : 1;
-        p.gx = (unsigned)((s.tiles + Q4_WAVES * p.r - 1) / (Q4_WAVES * p.r));
+        p.r = s.group > 32 && s.tiles >= Q4_STAGED_WAVES * 2 * 384 ? 2 : 1;
+        if (s.group == 128 && type != DN_F32 && type != DN_I8 && s.tiles >= Q4_STAGED_WAVES * 4 * 384) p.r = 4;
+        p.gx = (unsigned)((s.tiles + Q4_STAGED_WAVES * p.r - 1) / (Q4_STAGED_WAVES * p.r));
     } else {
         p.form = q4_plan::STREAM;
         p.t = pieces == 1 && x_tiles > 1 ? 2 : 1;
-        p.r = s.tiles >= 2 * 192 ? 2 : 1;
+        p.r = s.group > 32 && s.tiles >= 2 * 192 ? 2 : 1;
         p.gx = (unsigned)((s.tiles + p.r - 1) / p.r);
     }
     p.gy = (unsigned)((x_tiles + p.t - 1) / p.t);
@@ -719,9 +761,11 @@ extern "C" size_t connected_q4_workspace_bytes(int input_type, int batch, int in
 template <int T, int R, int PIECES, int PER, bool XG>
 static void q4_launch_second(const q4_args &a, const q4_plan &p)
 {
-    const dim3 grid(p.gx, p.gy), block(Q4_THREADS);
-    if (p.form == q4_plan::STAGED) hipLaunchKernelGGL((q4_staged_kernel<T, R, PIECES, PER, XG>), grid, block, 0, dn_stream(), a);
-    else if constexpr (T * PIECES <= 2) hipLaunchKernelGGL((q4_stream_kernel<T, R, PIECES, PER, XG>), grid, block, 0, dn_stream(), a);
+    const dim3 grid(p.gx, p.gy);
+    if (p.form == q4_plan::STAGED)
+        hipLaunchKernelGGL((q4_staged_kernel<T, R, PIECES, PER, XG>), grid, dim3(Q4_STAGED_WAVES * 64), 0, dn_stream(), a);
+    else if constexpr (T * PIECES <= 2 && R <= 2)
+        hipLaunchKernelGGL((q4_stream_kernel<T, R, PIECES, PER, XG>), grid, dim3(Q4_THREADS), 0, dn_stream(), a);
 }
 
 template <int TI, int PER, bool XG>
@@ -733,17 +777,26 @@ static void q4_launch(const q4_args &a, const q4_plan &p)
         return;
     }
     hipLaunchKernelGGL((q4_prepare_kernel<TI, XG>), dim3((unsigned)a.batch), dim3(256), 0, dn_stream(), a);
-    if (p.r == 2) {
-        if (p.t == 1) q4_launch_second<1, 2, PIECES, PER, XG>(a, p);
-        else if (p.t == 2) q4_launch_second<2, 2, PIECES, PER, XG>(a, p);
-        else if (p.t == 3) q4_launch_second<3, 2, PIECES, PER, XG>(a, p);
-        else q4_launch_second<4, 2, PIECES, PER, XG>(a, p);
-    } else {
-        if (p.t == 1) q4_launch_second<1, 1, PIECES, PER, XG>(a, p);
-        else if (p.t == 2) q4_launch_second<2, 1, PIECES, PER, XG>(a, p);
-        else if (p.t == 3) q4_launch_second<3, 1, PIECES, PER, XG>(a, p);
-        else q4_launch_second<4, 1, PIECES, PER, XG>(a, p);
-    }
+    if constexpr (PER == 1 && PIECES == 1 && !XG) /* (what the registers hold) */
+        if (p.r == 4) {
+            if (p.t == 1) q4_launch_second<1, 4, PIECES, PER, XG>(a, p);
+            else if (p.t == 2) q4_launch_second<2, 4, PIECES, PER, XG>(a, p);
+            else if (p.t == 3) q4_launch_second<3, 4, PIECES, PER, XG>(a, p);
+            else q4_launch_second<4, 4, PIECES, PER, XG>(a, p);
+            return;
+        }
+    if constexpr (PER < 4) /* four groups in a block fill the registers with R = 1 */
+        if (p.r == 2) {
+            if (p.t == 1) q4_launch_second<1, 2, PIECES, PER, XG>(a, p);
+            else if (p.t == 2) q4_launch_second<2, 2, PIECES, PER, XG>(a, p);
+            else if (p.t == 3) q4_launch_second<3, 2, PIECES, PER, XG>(a, p);
+            else q4_launch_second<4, 2, PIECES, PER, XG>(a, p);
+            return;
+        }
+    if (p.t == 1) q4_launch_second<1, 1, PIECES, PER, XG>(a, p);
+    else if (p.t == 2) q4_launch_second<2, 1, PIECES, PER, XG>(a, p);
+    else if (p.t == 3) q4_launch_second<3, 1, PIECES, PER, XG>(a, p);
+    else q4_launch_second<4, 1, PIECES, PER, XG>(a, p);
 }
 
 template <int TI, bool XG>
