@@ -110,14 +110,6 @@ __device__ __forceinline__ void store_run(E *p, int i, int n, const float *v)
     }
 }
 
-/* max(a, |b|); the language's fmax takes two instructions for it, to quiet signalling NaNs. */
-__device__ __forceinline__ double max_abs(double a, double b)
-{
-    double d;
-    asm("v_max_f64 %0, %1, |%2|" : "=v"(d) : "v"(a), "v"(b));
-    return d;
-}
-
 /* One workgroup for each row, which it holds in registers: RUNS runs of V neighbouring values a lane, the runs of
  * the lanes next to each other (lane t, run j: values (j * THREADS + t) * V on).  Every buffer is read and written once.
  * RUNS = 0: as many runs as the row has, read again for each step (from the stored sum, if there is one).
@@ -211,7 +203,7 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_kernel(norm_args a)
                 for (int e = 0; e < V; ++e) {
                     p[e] = (double)v[e] * (double)g[e];
                     poison = fmaf(g[e], 0.f, poison);
-                    largest = max_abs(largest, p[e]);
+                    largest = fmax(largest, fabs(p[e]));
                 }
                 if (!finite)
 #pragma unroll

@@ -39,7 +39,8 @@ static q4_shape q4_shape_of(int inputs, int outputs, int group)
 
 static bool q4_shape_ok(int inputs, int outputs, int group)
 {
-    return inputs >= 1 && outputs >= 1 && inputs <= 0x7fffff80 && (group == 32 || group == 64 || group == 128);
+    /* what is below 2^31 by more than a launch's stride: loops and filled-up tiles stay within an int */
+    return inputs >= 1 && outputs >= 1 && inputs <= 0x7fff0000 && outputs <= 0x7fff0000 && (group == 32 || group == 64 || group == 128);
 }
 
 extern "C" size_t q4_packed_bytes(int inputs, int outputs, int group)
@@ -288,40 +289,42 @@ __device__ __forceinline__ q4_tile<PER> q4_load_tile(const q4_args &a, int tile,
 
 __device__ __forceinline__ half2_t q4_as_half2(unsigned v) { return __builtin_bit_cast(half2_t, v); }
 
-/* (v & mask) | 0x64006400 in one instruction, which takes no two constants: the second comes in a register. */
-__device__ __forceinline__ half2_t q4_pick(unsigned v, unsigned mask, unsigned magic)
-{
-    unsigned d;
-    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(d) : "v"(v), "s"(mask), "v"(magic));
-    return q4_as_half2(d);
-}
+/* The constants of the unpacking, held in registers that the compiler does not see through: it then masks and merges
+ * in one instruction, which takes no two literals. */
+struct q4_masks {
+    unsigned low, high, magic;
+    __device__ q4_masks() : low(0x000f000fu), high(0x00f000f0u), magic(0x64006400u)
+    {
+        asm("" : "+s"(low), "+s"(high), "+v"(magic));
+    }
+};
 
 /* Eight codes less their zero as fp16: 0x6400 | c is 1024 + c, and with the code four bits up 1024 + 16 c. */
-__device__ __forceinline__ half8_t q4_unpack8(unsigned v, half2_t z1024, half2_t z64, unsigned magic)
+__device__ __forceinline__ half8_t q4_unpack8(unsigned v, half2_t z1024, half2_t z64, const q4_masks &k)
 {
     const half2_t sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
     const unsigned w = v >> 8;
-    const half2_t a = q4_pick(v, 0x000f000fu, magic) + z1024;
-    const half2_t b = __builtin_elementwise_fma(q4_pick(v, 0x00f000f0u, magic), sixteenth, z64);
-    const half2_t c = q4_pick(w, 0x000f000fu, magic) + z1024;
-    const half2_t d = __builtin_elementwise_fma(q4_pick(w, 0x00f000f0u, magic), sixteenth, z64);
+    const half2_t a = q4_as_half2((v & k.low) | k.magic) + z1024;
+    const half2_t b = __builtin_elementwise_fma(q4_as_half2((v & k.high) | k.magic), sixteenth, z64);
+    const half2_t c = q4_as_half2((w & k.low) | k.magic) + z1024;
+    const half2_t d = __builtin_elementwise_fma(q4_as_half2((w & k.high) | k.magic), sixteenth, z64);
     return (half8_t){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
 /* Adds the products of R tiles of outputs with T tiles of 16 input rows.  operand(t, piece, step): the lane's eight
- * inputs of a row; x_scale(t, g): the factors of its four rows of results, where they change along the row (XS). */
-template <int T, int R, int PIECES, int PER, bool XS, class Operand, class Scale>
-__device__ __forceinline__ void q4_multiply(const q4_tile<PER> (&w)[R], float4_t (&sum)[R][T], Operand operand, Scale x_scale)
+ * inputs of a row; x_scale(t, g): the factors of its four rows of results, where they change along the row (XS).  ONE:
+ * there is one input row, and only the first result of a lane counts. */
+template <int T, int R, int PIECES, int PER, bool XS, bool ONE = false, class Operand, class Scale>
+__device__ __forceinline__ void q4_multiply(const q4_masks &masks, const q4_tile<PER> (&w)[R], float4_t (&sum)[R][T],
+                                            Operand operand, Scale x_scale)
 {
-    unsigned magic = 0x64006400u;
-    asm("" : "+v"(magic));
 #pragma unroll
     for (int g = 0; g < PER; ++g) {
         float4_t acc[R][T];
         half2_t z1024[R], z64[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const unsigned z = (w[r].zero >> (8 * g)) & 0xff, z2 = z | z << 16;
+            const unsigned z2 = __builtin_amdgcn_perm(0, w[r].zero, 0x0c000c00u + 0x00010001u * g); /* the byte in both halves */
             z1024[r] = q4_as_half2(0xe400e400u | z2); /* -(1024 + z), -(64 + z) */
             z64[r] = q4_as_half2(0xd400d400u | z2 << 4);
         }
@@ -332,7 +335,7 @@ __device__ __forceinline__ void q4_multiply(const q4_tile<PER> (&w)[R], float4_t
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 const unsigned code = step == 0 ? w[r].code.x : step == 1 ? w[r].code.y : step == 2 ? w[r].code.z : w[r].code.w;
-                wv[r] = q4_unpack8(code, z1024[r], z64[r], magic);
+                wv[r] = q4_unpack8(code, z1024[r], z64[r], masks);
             }
 #pragma unroll
             for (int t = 0; t < T; ++t)
@@ -351,6 +354,10 @@ __device__ __forceinline__ void q4_multiply(const q4_tile<PER> (&w)[R], float4_t
             if (XS) f = x_scale(t, g);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
+                if (ONE) {
+                    sum[r][t][0] = fmaf(acc[r][t][0], XS ? f[0] * w[r].scale[g] : w[r].scale[g], sum[r][t][0]);
+                    continue;
+                }
                 const float4_t scale = {w[r].scale[g], w[r].scale[g], w[r].scale[g], w[r].scale[g]};
                 sum[r][t] = __builtin_elementwise_fma(acc[r][t], XS ? f * scale : scale, sum[r][t]);
             }
@@ -373,21 +380,23 @@ __device__ __forceinline__ float q4_bias(const q4_args &a, int o) { return a.bia
 
 /* ---- small input: at most 16 rows that fit into LDS whole.  Each workgroup scales and splits the input itself, block
  * by block of 128 values, and then streams row tiles of the weights, AHEAD blocks of a wave in flight. */
-template <int TI, int PER, bool XG>
+template <int TI, int PER, bool XG, bool ONE>
 __global__ __launch_bounds__(Q4_THREADS) void q4_direct_kernel(q4_args a)
 {
+    constexpr int THREADS = Q4_THREADS, WAVES = Q4_WAVES;
     constexpr int PIECES = TI == DN_F32 ? 2 : 1;
-    constexpr int AHEAD = PER == 4 ? 6 : 8;
+    constexpr int AHEAD = PER == 4 ? 6 : 8, MOVES = 4;
     extern __shared__ char lds[];
-    __shared__ float s_red[Q4_WAVES][16][17];
+    __shared__ float s_red[WAVES][16][17];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kpad = a.s.kblocks * 128, pitch = kpad * 2 * PIECES + 16; /* bytes of a row: 16 more, for the banks */
-    const int part = wave % a.ksplit, own_tile = wave / a.ksplit, rows_per = Q4_WAVES / a.ksplit;
+    const int part = wave % a.ksplit, own_tile = wave / a.ksplit, rows_per = WAVES / a.ksplit;
     const int mine = (a.s.kblocks - part + a.ksplit - 1) / a.ksplit; /* this wave's blocks: part, part + ksplit, ... */
     const int stride = gridDim.x * rows_per;
     int tile0 = blockIdx.x * rows_per;
 
     auto fetch = [&](int t, int n) { return q4_load_tile<PER>(a, min(t, a.s.tiles - 1), part + a.ksplit * n, lane); };
+    const q4_masks masks;
     q4_tile<PER> w[AHEAD];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
@@ -397,38 +406,55 @@ __global__ __launch_bounds__(Q4_THREADS) void q4_direct_kernel(q4_args a)
     const size_t row_bytes = (size_t)a.s.inputs * (TI == DN_F32 ? 4 : TI == DN_I8 ? 1 : 2);
     float *factors = (float *)(lds + a.batch * pitch);
     const int quads = kpad / 4;
-    for (int b = 0; b < a.batch; ++b) {
-        const char *row = (const char *)a.input + b * row_bytes;
-        for (int q = tid; q < quads; q += Q4_THREADS) { /* 32 lanes have a block */
-            float x[4], factor = 1;
+    for (int b = 0, q = tid; b < a.batch;) {
+        float x[MOVES][4];
+        int of[MOVES], at[MOVES]; /* row and four of the next items of this lane, whose loads go together */
+#pragma unroll
+        for (int m = 0; m < MOVES; ++m) {
+            const bool in = q < quads; /* (a row shorter than the workgroup leaves some lanes out) */
+            of[m] = in ? b : a.batch;
+            at[m] = q;
+            q4_load4<TI>((const char *)a.input + min(b, a.batch - 1) * row_bytes, min(q, quads - 1) * 4, a.s.inputs, x[m]);
+            q += THREADS;
+            if (q >= quads) {
+                q = tid;
+                ++b;
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < MOVES; ++m) { /* 32 lanes have a block */
+            if (of[m] >= a.batch) continue;
+            float factor = 1;
             half4_t hi, lo;
             int shift = 0;
-            q4_load4<TI>(row, q * 4, a.s.inputs, x);
             if (TI != DN_I8) {
-                unsigned m = q4_largest4(0, x);
-                m = max(m, dn_move<0xb1, 0xf>(m, m));
-                m = max(m, dn_move<0x4e, 0xf>(m, m));
-                m = max(m, dn_move<0x141, 0xf>(m, m));
-                m = max(m, dn_move<0x140, 0xf>(m, m));
-                m = max(m, (unsigned)__shfl_xor((int)m, 16, 64));
-                shift = q4_shift(m, factor);
-                if ((tid & 31) == 0) factors[(q >> 5) * 16 + b] = factor;
+                unsigned m4 = q4_largest4(0, x[m]);
+                m4 = max(m4, dn_move<0xb1, 0xf>(m4, m4));
+                m4 = max(m4, dn_move<0x4e, 0xf>(m4, m4));
+                m4 = max(m4, dn_move<0x141, 0xf>(m4, m4));
+                m4 = max(m4, dn_move<0x140, 0xf>(m4, m4));
+                m4 = max(m4, (unsigned)__shfl_xor((int)m4, 16, 64));
+                shift = q4_shift(m4, factor);
+                if ((tid & 31) == 0) factors[(at[m] >> 5) * 16 + of[m]] = factor;
             }
-            q4_split4(x, shift, hi, lo);
-            *(half4_t *)(lds + b * pitch + q * 8) = hi;
-            if (PIECES == 2) *(half4_t *)(lds + b * pitch + kpad * 2 + q * 8) = lo;
+            q4_split4(x[m], shift, hi, lo);
+            char *to = lds + of[m] * pitch + at[m] * 8;
+            *(half4_t *)to = hi;
+            if (PIECES == 2) *(half4_t *)(to + kpad * 2) = lo;
         }
-        if (XG) {
-            const int x_groups = (a.s.inputs + a.x_group - 1) / a.x_group;
-            for (int g = tid; g < a.s.groups; g += Q4_THREADS)
-                factors[g * 16 + b] = g < x_groups ? a.input_scales[(long)b * x_groups + g] : 0.f;
+    }
+    if (XG) {
+        const int x_groups = (a.s.inputs + a.x_group - 1) / a.x_group;
+        for (int i = tid; i < a.batch * a.s.groups; i += THREADS) {
+            const int b = i / a.s.groups, g = i - b * a.s.groups;
+            factors[g * 16 + b] = g < x_groups ? a.input_scales[(long)b * x_groups + g] : 0.f;
         }
     }
     __syncthreads();
 
     constexpr bool XS = TI != DN_I8 || XG;
     const char *base = lds + min(lane & 15, a.batch - 1) * pitch + (lane >> 4) * 16;
-    const float *row_factors = factors + (lane >> 4) * 4;
+    const float *row_factors = factors + (ONE ? 0 : (lane >> 4) * 4);
     for (; tile0 < a.s.tiles; tile0 += stride) {
         const int tile = tile0 + own_tile;
         float4_t sum[1][1] = {{{0, 0, 0, 0}}};
@@ -439,10 +465,13 @@ __global__ __launch_bounds__(Q4_THREADS) void q4_direct_kernel(q4_args a)
                 if (n + u < mine) {
                     const int kb = part + a.ksplit * (n + u);
                     const q4_tile<PER> one[1] = {w[u]};
-                    q4_multiply<1, 1, PIECES, PER, XS>(
-                        one, sum,
+                    q4_multiply<1, 1, PIECES, PER, XS, ONE>(
+                        masks, one, sum,
                         [&](int, int piece, int step) { return *(const half8_t *)(base + piece * kpad * 2 + kb * 256 + step * 64); },
-                        [&](int, int g) { return *(const float4_t *)(row_factors + (XG ? kb * PER + g : kb) * 16); });
+                        [&](int, int g) {
+                            const float *f = row_factors + (XG ? kb * PER + g : kb) * 16;
+                            return ONE ? (float4_t){*f, 0, 0, 0} : *(const float4_t *)f;
+                        });
                 }
                 if (last ? u < mine && tile0 + stride < a.s.tiles : n + AHEAD + u < mine)
                     w[u] = fetch(last ? tile + stride : tile, last ? u : n + AHEAD + u);
@@ -451,15 +480,15 @@ __global__ __launch_bounds__(Q4_THREADS) void q4_direct_kernel(q4_args a)
         /* what the waves of a row tile have, added in their order; a thread for each output of each row */
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s_red[wave][(lane >> 4) * 4 + i][lane & 15] = sum[0][0][i];
+        for (int i = 0; i < (ONE ? 1 : 4); ++i) s_red[wave][(lane >> 4) * 4 + i][lane & 15] = sum[0][0][i];
         __syncthreads();
-        for (int i = tid; i < rows_per * a.batch * 16; i += Q4_THREADS) {
+        for (int i = tid; i < rows_per * a.batch * 16; i += THREADS) {
             const int r = i / (a.batch * 16), b = (i >> 4) % a.batch, o = (tile0 + r) * 16 + (i & 15);
             if (o >= a.s.outputs) continue;
             const float bias = q4_bias(a, o);
             float y = 0;
 #pragma unroll
-            for (int q = 0; q < Q4_WAVES; ++q)
+            for (int q = 0; q < WAVES; ++q)
                 if (q < a.ksplit) y += s_red[r * a.ksplit + q][b][i & 15];
             if (TI == DN_I8 && !XG) y *= a.input_scales[b];
             q4_store(a, b, o, y, bias);
@@ -577,9 +606,10 @@ __global__ __launch_bounds__(Q4_THREADS) void q4_stream_kernel(q4_args a)
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int t = 0; t < T; ++t) sum[r][t] = (float4_t){0, 0, 0, 0};
+    const q4_masks masks;
     auto multiply = [&](const block_data &d) {
         q4_multiply<T, R, PIECES, PER, XG>(
-            d.w, sum, [&](int t, int piece, int step) { return d.x[t][piece][step]; }, [&](int t, int g) { return d.f[t][g]; });
+            masks, d.w, sum, [&](int t, int piece, int step) { return d.x[t][piece][step]; }, [&](int t, int g) { return d.f[t][g]; });
     };
     block_data one, two;
     if (mine > 0) fetch(0, one);
@@ -641,6 +671,7 @@ __global__ __launch_bounds__(Q4_STAGED_WAVES * 64, 2) void q4_staged_kernel(q4_a
 #pragma unroll
         for (int t = 0; t < T; ++t) sum[r][t] = (float4_t){0, 0, 0, 0};
 
+    const q4_masks masks;
     uint4_t moved[MOVES];
     auto input_of = [&](int c) {
 #pragma unroll
@@ -673,7 +704,7 @@ __global__ __launch_bounds__(Q4_STAGED_WAVES * 64, 2) void q4_staged_kernel(q4_a
         for (int u = 0; u < UNITS; ++u) {
             if (c * UNITS + u < kblocks)
                 q4_multiply<T, R, PIECES, PER, XG>(
-                    w[u], sum,
+                    masks, w[u], sum,
                     [&](int t, int piece, int step) {
                         return *(const half8_t *)(base + t * SPAN + u * BLOCK + piece * 4096 + step * 1024 + lane * 16);
                     },
@@ -707,7 +738,9 @@ __global__ __launch_bounds__(Q4_STAGED_WAVES * 64, 2) void q4_staged_kernel(q4_a
 }
 
 /* Which form a product takes.
- *   direct  up to 16 rows and 16384 inputs in all: what a workgroup can scale while its first weights arrive
+ *   direct  at most 16 rows that are short enough for every workgroup to scale them while its first weights arrive: a
+ *           second launch and the way of the input through memory cost more.  Longer ones (25088 values in two rows)
+ *           are better scaled once.
  *   staged  so many outputs that workgroups of 64 (R = 1) or 128 (R = 2) of them fill the chip
  *   stream  the others */
 struct q4_plan {
@@ -720,14 +753,14 @@ struct q4_plan {
 static q4_plan q4_plan_of(const q4_shape &s, int type, int batch)
 {
     q4_plan p;
-    const int pieces = type == DN_F32 ? 2 : 1, x_tiles = (batch + 15) / 16;
+    const int pieces = type == DN_F32 ? 2 : 1, x_tiles = (int)(((long)batch + 15) / 16);
     p.ksplit = p.t = p.r = 1;
     p.gy = 1;
     p.lds = batch * ((size_t)s.kblocks * 256 * pieces + 16) + (size_t)(type == DN_I8 ? s.groups : s.kblocks) * 64;
-    if (batch <= 16 && (long)batch * s.inputs <= 16384 && p.lds <= 120 << 10) {
+    if (batch <= 16 && (long)batch * s.inputs <= (batch == 1 ? 28672 : pieces == 2 ? 20480 : 12288) && p.lds <= 120 << 10) {
         p.form = q4_plan::DIRECT;
         /* waves share a row tile as long as each has a block and the chip is not full */
-        while (p.ksplit < 8 && (long)s.tiles * p.ksplit < 256 * Q4_WAVES && p.ksplit * 2 <= s.kblocks) p.ksplit *= 2;
+        while (p.ksplit < Q4_WAVES && (long)s.tiles * p.ksplit < 256 * Q4_WAVES && p.ksplit * 2 <= s.kblocks) p.ksplit *= 2;
         const long groups = ((long)s.tiles * p.ksplit + Q4_WAVES - 1) / Q4_WAVES;
         p.gx = (unsigned)(groups < 512 ? groups : 512);
         return p;
@@ -738,7 +771,6 @@ static q4_plan q4_plan_of(const q4_shape &s, int type, int batch)
         p.form = q4_plan::STAGED;
         p.t = (x_tiles + passes - 1) / passes;
         p.r = s.group > 32 && s.tiles >= Q4_STAGED_WAVES * 2 * 384 ? 2 : 1;
-        if (s.group == 128 && type != DN_F32 && type != DN_I8 && s.tiles >= Q4_STAGED_WAVES * 4 * 384) p.r = 4;
         p.gx = (unsigned)((s.tiles + Q4_STAGED_WAVES * p.r - 1) / (Q4_STAGED_WAVES * p.r));
     } else {
         p.form = q4_plan::STREAM;
@@ -764,7 +796,7 @@ static void q4_launch_second(const q4_args &a, const q4_plan &p)
     const dim3 grid(p.gx, p.gy);
     if (p.form == q4_plan::STAGED)
         hipLaunchKernelGGL((q4_staged_kernel<T, R, PIECES, PER, XG>), grid, dim3(Q4_STAGED_WAVES * 64), 0, dn_stream(), a);
-    else if constexpr (T * PIECES <= 2 && R <= 2)
+    else if constexpr (T * PIECES <= 2)
         hipLaunchKernelGGL((q4_stream_kernel<T, R, PIECES, PER, XG>), grid, dim3(Q4_THREADS), 0, dn_stream(), a);
 }
 
@@ -773,18 +805,11 @@ static void q4_launch(const q4_args &a, const q4_plan &p)
 {
     constexpr int PIECES = TI == DN_F32 ? 2 : 1;
     if (p.form == q4_plan::DIRECT) {
-        hipLaunchKernelGGL((q4_direct_kernel<TI, PER, XG>), dim3(p.gx), dim3(Q4_THREADS), p.lds, dn_stream(), a);
+        if (a.batch == 1) hipLaunchKernelGGL((q4_direct_kernel<TI, PER, XG, true>), dim3(p.gx), dim3(Q4_THREADS), p.lds, dn_stream(), a);
+        else hipLaunchKernelGGL((q4_direct_kernel<TI, PER, XG, false>), dim3(p.gx), dim3(Q4_THREADS), p.lds, dn_stream(), a);
         return;
     }
     hipLaunchKernelGGL((q4_prepare_kernel<TI, XG>), dim3((unsigned)a.batch), dim3(256), 0, dn_stream(), a);
-    if constexpr (PER == 1 && PIECES == 1 && !XG) /* (what the registers hold) */
-        if (p.r == 4) {
-            if (p.t == 1) q4_launch_second<1, 4, PIECES, PER, XG>(a, p);
-            else if (p.t == 2) q4_launch_second<2, 4, PIECES, PER, XG>(a, p);
-            else if (p.t == 3) q4_launch_second<3, 4, PIECES, PER, XG>(a, p);
-            else q4_launch_second<4, 4, PIECES, PER, XG>(a, p);
-            return;
-        }
     if constexpr (PER < 4) /* four groups in a block fill the registers with R = 1 */
         if (p.r == 2) {
             if (p.t == 1) q4_launch_second<1, 2, PIECES, PER, XG>(a, p);
