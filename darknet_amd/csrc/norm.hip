@@ -250,13 +250,14 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_kernel(norm_args a)
         }
         if (a.output) {
             const float rf = (float)r;
+            const bool ordinary = r >= 0x1p-100 && r <= 0x1p100; /* else r itself may leave the range of 32 bits */
 #pragma unroll
             for (int j = 0; j < runs; ++j) {
                 float v[V], g[V];
                 values(j, v);
                 scales(j, g);
 #pragma unroll
-                for (int e = 0; e < V; ++e) v[e] = v[e] * rf * g[e];
+                for (int e = 0; e < V; ++e) v[e] = ordinary ? v[e] * rf * g[e] : (float)((double)v[e] * r * (double)g[e]);
                 store_run<E, V>((E *)a.output + row * n, at(j), n, v);
             }
         }
@@ -290,8 +291,9 @@ extern "C" int forward_rmsnorm_gpu(const void *input, const void *add, const flo
 {
     const char *me = "forward_rmsnorm_gpu";
     if (!dn_is_float_type(type)) return dn_refuse(me, "unknown element type");
-    if (rows < 0 || n < 1) return dn_refuse(me, "bad geometry");
+    if (rows < 0 || n < 1 || n > 0x7fff0000) return dn_refuse(me, "bad geometry"); /* indexes of a row stay within an int */
     if (!(eps >= 0) || !(eps <= 3.402823466e38f)) return dn_refuse(me, "eps must be a finite number that is not negative");
+    if (rows == 0) return 0;
     if (!input) return dn_refuse(me, "input is missing");
     if (!output && !q8_output) return dn_refuse(me, "neither output nor q8_output is given");
     if (!q8_output != !q8_scales) return dn_refuse(me, "q8_output and q8_scales come together");
@@ -303,7 +305,6 @@ extern "C" int forward_rmsnorm_gpu(const void *input, const void *add, const flo
     if (!dn_aligned(input, e) || !dn_aligned(add, e) || !dn_aligned(sum_output, e) || !dn_aligned(output, e) ||
         !dn_aligned(scales, 4) || !dn_aligned(q8_scales, 4))
         return dn_refuse(me, "a buffer is not aligned to its element type");
-    if (rows == 0) return 0;
     hip_require_device(me);
     const norm_args a = {input, add, scales, sum_output, output, q8_output, q8_scales, rows, n, q8_group, eps, 1. / n};
     if (type == DN_F32) q8_output ? norm_launch<DN_F32, true>(a) : norm_launch<DN_F32, false>(a);

@@ -757,7 +757,7 @@ static q4_plan q4_plan_of(const q4_shape &s, int type, int batch)
     p.ksplit = p.t = p.r = 1;
     p.gy = 1;
     p.lds = batch * ((size_t)s.kblocks * 256 * pieces + 16) + (size_t)(type == DN_I8 ? s.groups : s.kblocks) * 64;
-    if (batch <= 16 && (long)batch * s.inputs <= (batch == 1 ? 28672 : pieces == 2 ? 20480 : 12288) && p.lds <= 120 << 10) {
+    if (batch <= 4 && (long)batch * s.inputs <= 28672 && p.lds <= 120 << 10) {
         p.form = q4_plan::DIRECT;
         /* waves share a row tile as long as each has a block and the chip is not full */
         while (p.ksplit < Q4_WAVES && (long)s.tiles * p.ksplit < 256 * Q4_WAVES && p.ksplit * 2 <= s.kblocks) p.ksplit *= 2;
@@ -767,10 +767,10 @@ static q4_plan q4_plan_of(const q4_shape &s, int type, int batch)
     }
     p.lds = 0;
     const int passes = (x_tiles + 3) / 4;
-    if (s.tiles >= Q4_STAGED_WAVES * 384) {
+    if ((long)s.tiles * x_tiles >= 2800) {
         p.form = q4_plan::STAGED;
         p.t = (x_tiles + passes - 1) / passes;
-        p.r = s.group > 32 && s.tiles >= Q4_STAGED_WAVES * 2 * 384 ? 2 : 1;
+        p.r = s.group > 32 && (long)s.tiles * passes >= Q4_STAGED_WAVES * 2 * 384 ? 2 : 1;
         p.gx = (unsigned)((s.tiles + Q4_STAGED_WAVES * p.r - 1) / (Q4_STAGED_WAVES * p.r));
     } else {
         p.form = q4_plan::STREAM;
@@ -841,14 +841,14 @@ extern "C" int forward_connected_q4_gpu(const void *input, int input_type, const
     if (!dn_is_float_type(output_type)) return dn_refuse(me, "unknown output type");
     if (batch < 0 || !q4_shape_ok(inputs, outputs, group)) return dn_refuse(me, "bad geometry (group must be 32, 64 or 128)");
     if (activation < 0 || activation > DN_SELU) return dn_refuse(me, "unknown activation");
+    if (batch == 0) return 0;
     if (!input || !packed || !output) return dn_refuse(me, "a buffer is missing");
     if (input_type == DN_I8 && !input_scales) return dn_refuse(me, "8-bit input needs its scales");
     if (input_type == DN_I8 && input_group != 0 && input_group != group)
         return dn_refuse(me, "input_group must be 0 (the row) or the weights' group");
     if (!dn_aligned(input, dn_type_bytes(input_type)) || !dn_aligned(output, dn_type_bytes(output_type)) ||
-        !dn_aligned(input_scales, 4) || !dn_aligned(biases, 4) || !dn_aligned(packed, 16) || !dn_aligned(workspace, 16))
+        (input_type == DN_I8 && !dn_aligned(input_scales, 4)) || !dn_aligned(biases, 4) || !dn_aligned(packed, 16) || !dn_aligned(workspace, 16))
         return dn_refuse(me, "a buffer is not aligned to its element type, or packed or workspace not to 16 bytes");
-    if (batch == 0) return 0;
     const q4_shape s = q4_shape_of(inputs, outputs, group);
     const bool xg = input_type == DN_I8 && input_group != 0;
     const q4_plan p = q4_plan_of(s, input_type, batch);

@@ -241,7 +241,7 @@ __device__ __forceinline__ void find_border(sample_lds &s, const sample_row &r)
             u64 before;
             bin = counts.find(0, (u64)r.k, before);
             need = r.k - (int)before;
-            if (bin == SM_BINS) bin = -1; /* fewer than k tokens can be drawn at all */
+            if (bin >= SM_BINS - 1) bin = -1; /* all that weighs anything is among the first k */
         }
         if (lane == 0) {
             s.border.k_bin = bin;
@@ -882,12 +882,12 @@ extern "C" int sample_rows_gpu(const void *logits, int type, int rows, int n, lo
     if (!dn_is_float_type(type)) return dn_refuse(me, "unknown element type");
     if (rows < 0 || n < 1 || n > (1 << 24)) return dn_refuse(me, "bad geometry (1 to 2^24 tokens)");
     if (stride < n) return dn_refuse(me, "the stride is shorter than a row");
+    if (rows == 0) return 0;
     if (!logits || !uniform || !tokens) return dn_refuse(me, "a buffer is missing");
     if (!dn_aligned(logits, dn_type_bytes(type)) || !dn_aligned(temperature, 4) || !dn_aligned(top_k, 4) ||
         !dn_aligned(top_p, 4) || !dn_aligned(min_p, 4) || !dn_aligned(uniform, 4) || !dn_aligned(tokens, 4) ||
         !dn_aligned(probs, 4) || !dn_aligned(workspace, 16))
         return dn_refuse(me, "a buffer is not aligned to its element type, or the workspace not to 16 bytes");
-    if (rows == 0) return 0;
     if (!workspace && !sample_in_one(n)) return dn_refuse(me, "the workspace is missing");
     hip_require_device(me);
     sample_args a = {logits, temperature, top_p, min_p, uniform, top_k, tokens, probs, (unsigned char *)workspace,

@@ -448,7 +448,7 @@ void forward_crop_gpu(const float *input, float *output, int batch, int c, int h
  * stream capture is recorded like any other, and calls that overlap (two streams, two captured graphs) only need
  * workspaces and outputs of their own.  The workspace needs no initial contents and is aligned to 16 bytes.
  * They return 0, or -1 after a message on stderr when the arguments cannot be honoured: then nothing has
- * been launched.  No rows (rows or batch 0) is a call that does nothing.
+ * been launched.  No rows (rows or batch 0) is a call that does nothing, with buffers or without.
  * ---------------------------------------------------------------------------------------- */
 enum { DN_F32 = 0, DN_F16, DN_BF16, DN_I8 };
 
@@ -480,8 +480,8 @@ int forward_rmsnorm_gpu(const void *input, const void *add, const float *scales,
  * [batch][groups of input_group] (input_group: 0 = one scale a row, or `group`), as forward_rmsnorm_gpu
  * writes them; input_scales and input_group are read for DN_I8 only.  biases may be NULL.  output
  * [batch][outputs] is fp32, fp16 or bf16.  workspace: connected_q4_workspace_bytes() bytes (NULL if that
- * is 0).  Every output is the same in every run.  A row of the input that holds a value that is not finite
- * has NaN in all its outputs. */
+ * is 0).  Every output is the same in every run.  For a row of the input that holds a value that is not finite
+ * all the sums are NaN; the activation is applied to that. */
 size_t q4_packed_bytes(int inputs, int outputs, int group);
 int q4_pack_codes_gpu(const unsigned char *codes, const float *scales, const unsigned char *zeros, void *packed,
                       int inputs, int outputs, int group);
@@ -493,7 +493,7 @@ int forward_connected_q4_gpu(const void *input, int input_type, const float *inp
                              int inputs, int outputs, int group, int activation, void *workspace);
 
 /* One token for each row of logits [rows][stride], of which the first n (up to 2^24) count, from the
- * random number uniform[row] in [0, 1] (hip_random's are; one outside counts as the nearer end).  The tokens of
+ * random number uniform[row] in [0, 1] (hip_random's are; one outside counts as the nearer end, NaN as 0).  The tokens of
  * a row are ordered by (logit descending, index ascending), w = exp((logit - largest) / temperature):
  *   temperature   not above 0 (or NaN): the first token of the order; NULL: 1
  *   top_k         the first top_k of the order; NULL, or not above 0: all

@@ -106,3 +106,37 @@ def test_plain_forms():
     assert R.sample(l, 1, 0, 0.3, 0, 1.0)[0] == 1                # one four alone is 4/11
     assert R.sample(l, 1, 0, 1, 0.4, 1.0)[0] == 3 and R.sample(l, 0, 0, 1, 0, 0.9)[:2] == (1, 1.0)
     assert R.sample(np.float32([np.nan, -np.inf]), 1, 0, 1, 0, .5)[:2] == (-1, 0.0)
+
+
+def test_no_rows_need_no_buffers(L):
+    assert norm(L, rows=0, input=None, add=None, scales=None, sum=None, output=None) == 0
+    assert q4(L, batch=0, x=None, packed=None, y=None, ws=None) == 0
+    assert sample(L, rows=0, x=None, u=None, tok=None, ws=None) == 0
+
+
+def test_sizes_whose_indexes_leave_an_int_are_refused(L, capfd):
+    big = 0x7FFFFFFF
+    assert norm(L, n=big) == q4(L, k=big) == q4(L, n=big) == q4(L, batch=big, k=64, n=16) == -1
+    assert "geometry" in capfd.readouterr().err
+    assert L.q4_packed_bytes(big, 16, 32) == L.q4_packed_bytes(16, big, 32) == 0
+
+
+@pytest.mark.parametrize("batch,k,n", [(5, 64, 16), (64, 64, 16), (1, 40000, 16), (16, 128, 45000)])
+def test_q4_workspace(L, capfd, batch, k, n):
+    """Asked for and missing, or not aligned."""
+    assert L.connected_q4_workspace_bytes(R.F32, batch, k, n, 32) > 0
+    assert q4(L, batch=batch, k=k, n=n, ws=None) == -1 and "workspace is missing" in capfd.readouterr().err
+    assert q4(L, batch=batch, k=k, n=n, ws=P + 8) == -1 and "workspace" in capfd.readouterr().err
+
+
+def test_q4_workspace_not_needed(L):
+    assert L.connected_q4_workspace_bytes(R.F32, 1, 4096, 4096, 128) == 0
+    assert L.connected_q4_workspace_bytes(R.F32, 0, 4096, 4096, 128) == L.connected_q4_workspace_bytes(R.F32, 8, 4096, 4096, 5) == 0
+
+
+def test_sample_workspace(L, capfd):
+    assert L.sample_workspace_bytes(4, 8192) == 0 and L.sample_workspace_bytes(4, 8193) > 0
+    assert L.sample_workspace_bytes(0, 9000) == L.sample_workspace_bytes(1, (1 << 24) + 1) == 0
+    assert L.sample_workspace_bytes(100000, 1 << 17) > 1 << 32     # sizes are not cut to 32 bits
+    assert sample(L, n=9000, stride=9000, ws=None) == -1 and "workspace is missing" in capfd.readouterr().err
+    assert sample(L, n=9000, stride=9000, ws=P + 8) == -1 and "workspace" in capfd.readouterr().err
