@@ -11,16 +11,18 @@
  * lanes and atomics add them, so the same row gives the same token in every run, and a border between two
  * tokens lies where the formula puts it to within 2^-38 of the largest mass.
  *
- * No row is sorted.  The logits are counted and weighed in 512 bins, a sixteenth of T wide, below the largest (what is
- * further below weighs nothing); the
- * bin in which the order's prefix ends is known from the running sums, everything in the bins before it is
- * kept, and only that bin's tokens (the candidates) are looked at more closely: digit by digit of their places.
+ * No row is sorted.  The logits are counted and weighed in 512 bins below the largest, a sixteenth of T wide (what is
+ * further below weighs nothing) or, where the row's logits lie closer together, as much narrower.  The bin in which the
+ * order's prefix ends is known from the running sums, everything in the bins before it is kept, and only that
+ * bin's tokens (the candidates) are looked at more closely: digit by digit of their places.
  */
 #include <math.h>
 
 #include "row_types.h"
 
 typedef unsigned long long u64;
+
+typedef float float2_t __attribute__((ext_vector_type(2)));
 
 #define SM_BINS 512
 #define SM_PER_T 16
@@ -291,15 +293,35 @@ __device__ __forceinline__ u64 block_sum(u64 v, sample_lds &s)
 }
 
 template <int THREADS>
-__device__ __forceinline__ float block_largest(float v, sample_lds &s)
+__device__ __forceinline__ float2_t block_ends(float2_t v, sample_lds &s)
 {
-    v = dn_wave_max(v);
+    v = (float2_t){dn_wave_max(v.x), -dn_wave_max(-v.y)};
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) s.part[threadIdx.x >> 6] = __float_as_uint(v);
+    if ((threadIdx.x & 63) == 0) s.part[threadIdx.x >> 6] = __builtin_bit_cast(u64, v);
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) v = fmaxf(v, __uint_as_float((unsigned)s.part[w]));
+    for (int w = 0; w < THREADS / 64; ++w) {
+        const float2_t o = __builtin_bit_cast(float2_t, s.part[w]);
+        v = (float2_t){fmaxf(v.x, o.x), fminf(v.y, o.y)};
+    }
     return v;
+}
+
+/* A row's largest and least logit (of those above -inf), of four more. */
+__device__ __forceinline__ void widen(float2_t &ends, const float l[4])
+{
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        ends.x = l[e] > ends.x ? l[e] : ends.x;
+        ends.y = l[e] < ends.y && l[e] > -INFINITY ? l[e] : ends.y;
+    }
+}
+
+/* Where all logits lie closer to the largest than the bins reach, the bins are made as much narrower: the fewer
+ * tokens share the one that has to be looked at. */
+__device__ __forceinline__ void narrow_bins(sample_row &r, float2_t ends)
+{
+    r.bins_per_logit = fminf(fmaxf(r.bins_per_logit, (SM_BINS - 2) / (ends.x - ends.y)), 3.402823466e38f);
 }
 
 /* mass_of the weight, and in the top bit whether min-p keeps it. */
@@ -480,17 +502,15 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
     float *own_l = row_lds + tid * (E + 1);
     for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const S *x = (const S *)a.logits + row * a.stride;
-        const sample_row r = settings_of(a, row);
-        float largest = -INFINITY;
+        sample_row r = settings_of(a, row);
+        float2_t ends = {-INFINITY, INFINITY};
 #pragma unroll
         for (int e = 0; e < E; e += 4) {
             float l[4];
             load4<T>(x, tid * E + e, a.n, vectors, l);
+            widen(ends, l);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                own_l[e + i] = l[i];
-                largest = l[i] > largest ? l[i] : largest;
-            }
+            for (int i = 0; i < 4; ++i) own_l[e + i] = l[i];
         }
         if (r.k || r.p < 1)
             for (int i = tid; i < SM_SLOTS; i += THREADS) {
@@ -498,7 +518,9 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
                 s.mass[i] = 0;
             }
         if (tid == 0) s_count = 0;
-        largest = block_largest<THREADS>(largest, s);
+        ends = block_ends<THREADS>(ends, s);
+        narrow_bins(r, ends);
+        const float largest = ends.x;
         if (!(largest > -INFINITY)) {
             if (tid == 0) answer(a, row, -1, 0, 0);
             continue;
@@ -581,7 +603,7 @@ __host__ __device__ static inline sample_space space_of(int rows, int segments)
     w.list = w.border + (size_t)rows * sizeof(sample_border);
     w.bins_count = w.list + (size_t)rows * SM_LISTED * 8;
     w.largest = w.bins_count + (size_t)rows * SM_BINS * 4;
-    w.found = w.largest + all * 4;
+    w.found = w.largest + all * 8;
     w.bytes = w.found + (size_t)rows * 8;
     return w;
 }
@@ -590,25 +612,28 @@ template <int T>
 __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_largest_kernel(sample_args a)
 {
     typedef typename dn_elt<T>::store S;
-    __shared__ float part[SM_SPLIT_THREADS / 64];
+    __shared__ float2_t part[SM_SPLIT_THREADS / 64];
     const sample_space ws = space_of(a.rows, a.segments);
     const bool vectors = rows_aligned<T>(a);
     for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
         const S *x = (const S *)a.logits + row * a.stride;
         const int lo = blockIdx.x * a.length, hi = min(a.n, lo + a.length);
-        float m = -INFINITY;
+        float2_t ends = {-INFINITY, INFINITY};
         for (int i = lo + threadIdx.x * 8; i < hi; i += SM_STRIP) {
             float l[8];
             load8<T>(x, i, hi, vectors, l);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) m = l[e] > m ? l[e] : m;
+            widen(ends, l);
+            widen(ends, l + 4);
         }
-        m = dn_wave_max(m);
+        ends = (float2_t){dn_wave_max(ends.x), -dn_wave_max(-ends.y)};
         __syncthreads();
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = ends;
         __syncthreads();
-        if (threadIdx.x == 0)
-            ((float *)(a.workspace + ws.largest))[row * a.segments + blockIdx.x] = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+        if (threadIdx.x == 0) {
+            float2_t t = part[0];
+            for (int w = 1; w < SM_SPLIT_THREADS / 64; ++w) t = (float2_t){fmaxf(t.x, part[w].x), fminf(t.y, part[w].y)};
+            ((float2_t *)(a.workspace + ws.largest))[row * a.segments + blockIdx.x] = t;
+        }
         if (blockIdx.x == 0)
             for (int i = threadIdx.x; i < SM_BINS; i += SM_SPLIT_THREADS) {
                 ((u64 *)(a.workspace + ws.bins_mass))[row * SM_BINS + i] = 0;
@@ -618,11 +643,15 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_largest_kernel(sample
     }
 }
 
-__device__ __forceinline__ float row_largest(const sample_args &a, const sample_space &ws, long row)
+/* The row's largest logit, and the bins' width. */
+__device__ __forceinline__ float row_largest(const sample_args &a, const sample_space &ws, long row, sample_row &r)
 {
     const int lane = threadIdx.x & 63;
-    const float *m = (const float *)(a.workspace + ws.largest) + row * a.segments;
-    return dn_wave_max(lane < a.segments ? m[lane] : -INFINITY);
+    const float2_t *m = (const float2_t *)(a.workspace + ws.largest) + row * a.segments;
+    const float2_t own = lane < a.segments ? m[lane] : (float2_t){-INFINITY, INFINITY};
+    const float2_t ends = {dn_wave_max(own.x), -dn_wave_max(-own.y)};
+    narrow_bins(r, ends);
+    return ends.x;
 }
 
 template <int T>
@@ -635,9 +664,9 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_bins_kernel(sample_ar
     const bool vectors = rows_aligned<T>(a);
     const int tid = threadIdx.x;
     for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
-        const sample_row r = settings_of(a, row);
+        sample_row r = settings_of(a, row);
         if (!r.k && !(r.p < 1)) continue;
-        const float largest = row_largest(a, ws, row);
+        const float largest = row_largest(a, ws, row, r);
         const S *x = (const S *)a.logits + row * a.stride;
         const int lo = blockIdx.x * a.length, hi = min(a.n, lo + a.length);
         __syncthreads();
@@ -677,8 +706,8 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_kept_kernel(sample_ar
     const sample_places<T> places = {a.index_bits};
     const int tid = threadIdx.x;
     for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
-        const sample_row r = settings_of(a, row);
-        const float largest = row_largest(a, ws, row);
+        sample_row r = settings_of(a, row);
+        const float largest = row_largest(a, ws, row, r);
         __syncthreads();
         if (r.k || r.p < 1)
             for (int i = tid; i < SM_BINS; i += SM_SPLIT_THREADS) {
@@ -746,13 +775,13 @@ __global__ __launch_bounds__(SM_DRAW_THREADS) void sample_draw_kernel(sample_arg
     const int tid = threadIdx.x, blocks = (a.n + a.block - 1) / a.block;
     for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         /* all that the first steps read is asked for at once */
-        const sample_row r = settings_of(a, row);
+        sample_row r = settings_of(a, row);
         const sample_border b = ((const sample_border *)(a.workspace + ws.border))[row];
         const u64 *kept = (const u64 *)(a.workspace + ws.kept) + row * SM_BLOCKS;
         const u64 own_kept = tid < blocks ? kept[tid] : 0;
         const int count = ((const int *)(a.workspace + ws.found))[row * 2], lost = ((const int *)(a.workspace + ws.found))[row * 2 + 1];
         const u64 *in_memory = (const u64 *)(a.workspace + ws.list) + (size_t)row * SM_LISTED;
-        const float largest = row_largest(a, ws, row);
+        const float largest = row_largest(a, ws, row, r);
         const S *x = (const S *)a.logits + row * a.stride;
         if (!(largest > -INFINITY)) {
             if (tid == 0) answer(a, row, -1, 0, 0);
