@@ -189,7 +189,6 @@ extern "C" int q4_unpack_weights_gpu(const void *packed, float *weights, int inp
  * The input is the instruction's first operand and the weights the second, so that a lane's results are those
  * of one output, whose scale and zero it has read beside the codes. */
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
-typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef unsigned uint4_t __attribute__((ext_vector_type(4)));
@@ -211,48 +210,59 @@ struct q4_args {
     q4_shape s;
 };
 
-/* The exponent that values are scaled by, from the largest of their absolute values' bits, and the factor that undoes
+/* The power of two that values are scaled by, from the largest of their absolute values' bits, and the factor that undoes
  * it: a power of two, NaN if a value is not finite. */
-__device__ __forceinline__ int q4_shift(unsigned largest, float &factor)
+__device__ __forceinline__ float q4_scaling(unsigned largest, float &factor)
 {
     int e = 15;
     if (largest - 1u < 0x7f7fffffu) (void)frexpf(__uint_as_float(largest), &e); /* largest < 2^e */
     const int shift = min(15 - e, 126);                                        /* 2^-126: the factor is not rounded */
     factor = largest < 0x7f800000u ? ldexpf(1.f, -shift) : __uint_as_float(0x7fc00000u);
-    return shift;
+    return ldexpf(1.f, shift);
 }
 
-/* Four inputs from k on (zeros behind the row's end), in one access where they exist, whatever their alignment. */
+/* Eight inputs from k on, zeros behind the row's end, in one access (two of fp32) whatever their alignment: the run that
+ * the end cuts is read from eight before the end, and moved. */
 template <int TI>
-__device__ __forceinline__ void q4_load4(const void *row, int k, int inputs, float x[4])
+__device__ __forceinline__ void q4_load8(const void *row, int k, int inputs, float x[8])
 {
     typedef typename dn_elt<TI>::store E;
-    typedef E E4 __attribute__((ext_vector_type(4)));
-    typedef E4 E4U __attribute__((aligned(sizeof(E))));
-    const E *p = (const E *)row + k;
-    if (k + 4 <= inputs) {
-        const E4 v = *(const E4U *)p;
+    typedef E E8 __attribute__((ext_vector_type(8)));
+    typedef E8 E8U __attribute__((aligned(sizeof(E))));
+    const E *p = (const E *)row;
+    if (inputs < 8) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = (float)v[i];
-    } else {
+        for (int i = 0; i < 8; ++i) x[i] = k + i < inputs ? (float)p[k + i] : 0.f;
+        return;
+    }
+    const int from = min(k, inputs - 8), cut = k - from;
+    const E8 v = *(const E8U *)(p + from);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = k + i < inputs ? (float)p[i] : 0.f;
+    for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
+    if (cut > 0) {
+#pragma unroll
+        for (int d = 1; d <= 4; d *= 2)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = cut & d ? (i + d < 8 ? x[i + d] : 0.f) : x[i];
+        if (cut >= 8)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = 0;
     }
 }
 
-__device__ __forceinline__ unsigned q4_largest4(unsigned m, const float x[4])
+__device__ __forceinline__ unsigned q4_largest8(unsigned m, const float x[8])
 {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
     return m;
 }
 
-/* The operand form of four inputs: hi, and what it leaves of the value in lo. */
-__device__ __forceinline__ void q4_split4(const float x[4], int shift, half4_t &hi, half4_t &lo)
+/* The operand form of eight inputs, scaled by a power of two: hi, and what it leaves of the value in lo. */
+__device__ __forceinline__ void q4_split8(const float x[8], float scale, half8_t &hi, half8_t &lo)
 {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float v = ldexpf(x[i], shift);
+    for (int i = 0; i < 8; ++i) {
+        const float v = x[i] * scale;
         hi[i] = (_Float16)v;
         lo[i] = (_Float16)(v - (float)hi[i]);
     }
@@ -263,26 +273,27 @@ template <int PER>
 struct q4_tile {
     uint4_t code;
     float scale[PER];
-    unsigned zero; /* a byte for each group */
+    unsigned zero; /* a byte for each group, from byte zero_at(lane) on */
+    static __device__ unsigned zero_at(int lane) { return (unsigned)(lane * PER) & 3; }
 };
 
 template <int PER>
-__device__ __forceinline__ q4_tile<PER> q4_load_tile(const q4_args &a, int tile, int kb, int lane)
+__device__ __forceinline__ q4_tile<PER> q4_load_tile(const q4_args &a, int tile, int kb, int lane) /* lane: whose part */
 {
     typedef float scales_t __attribute__((ext_vector_type(PER)));
     q4_tile<PER> t;
     const long at = (long)tile * a.s.kblocks + kb, own = (at * 16 + (lane & 15)) * PER;
     t.code = ((const uint4_t *)a.packed)[at * 64 + lane];
     const float *scale = (const float *)(a.packed + a.s.scales_at) + own;
-    const unsigned char *z = a.packed + a.s.zeros_at + own;
+    /* a whole word: after a load of one or two bytes the compiler masks them at once, and so waits for a tile that
+     * is not wanted before the next round */
+    t.zero = *(const unsigned *)(a.packed + a.s.zeros_at + (own & ~3l));
     if constexpr (PER == 1) {
         t.scale[0] = *scale;
-        t.zero = *z;
     } else {
         const scales_t v = *(const scales_t *)scale;
 #pragma unroll
         for (int g = 0; g < PER; ++g) t.scale[g] = v[g];
-        t.zero = PER == 4 ? *(const unsigned *)z : *(const unsigned short *)z;
     }
     return t;
 }
@@ -311,10 +322,19 @@ __device__ __forceinline__ half8_t q4_unpack8(unsigned v, half2_t z1024, half2_t
     return (half8_t){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+/* The zero of group g of a tile in both halves, as -(1024 + z) and -(64 + z). */
+template <int PER>
+__device__ __forceinline__ void q4_zeros(const q4_tile<PER> &w, int g, half2_t &z1024, half2_t &z64)
+{
+    const unsigned select = 0x0c000c00u + 0x00010001u * (q4_tile<PER>::zero_at(threadIdx.x & 63) + g);
+    const unsigned z2 = __builtin_amdgcn_perm(0, w.zero, select);
+    z1024 = q4_as_half2(0xe400e400u | z2);
+    z64 = q4_as_half2(0xd400d400u | z2 << 4);
+}
+
 /* Adds the products of R tiles of outputs with T tiles of 16 input rows.  operand(t, piece, step): the lane's eight
- * inputs of a row; x_scale(t, g): the factors of its four rows of results, where they change along the row (XS).  ONE:
- * there is one input row, and only the first result of a lane counts. */
-template <int T, int R, int PIECES, int PER, bool XS, bool ONE = false, class Operand, class Scale>
+ * inputs of a row; x_scale(t, g): the factors of its four rows of results, where they change along the row (XS). */
+template <int T, int R, int PIECES, int PER, bool XS, class Operand, class Scale>
 __device__ __forceinline__ void q4_multiply(const q4_masks &masks, const q4_tile<PER> (&w)[R], float4_t (&sum)[R][T],
                                             Operand operand, Scale x_scale)
 {
@@ -323,20 +343,13 @@ __device__ __forceinline__ void q4_multiply(const q4_masks &masks, const q4_tile
         float4_t acc[R][T];
         half2_t z1024[R], z64[R];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const unsigned z2 = __builtin_amdgcn_perm(0, w[r].zero, 0x0c000c00u + 0x00010001u * g); /* the byte in both halves */
-            z1024[r] = q4_as_half2(0xe400e400u | z2); /* -(1024 + z), -(64 + z) */
-            z64[r] = q4_as_half2(0xd400d400u | z2 << 4);
-        }
+        for (int r = 0; r < R; ++r) q4_zeros(w[r], g, z1024[r], z64[r]);
 #pragma unroll
         for (int i = 0; i < 4 / PER; ++i) {
             const int step = g * (4 / PER) + i;
             half8_t wv[R];
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const unsigned code = step == 0 ? w[r].code.x : step == 1 ? w[r].code.y : step == 2 ? w[r].code.z : w[r].code.w;
-                wv[r] = q4_unpack8(code, z1024[r], z64[r], masks);
-            }
+            for (int r = 0; r < R; ++r) wv[r] = q4_unpack8(w[r].code[step], z1024[r], z64[r], masks);
 #pragma unroll
             for (int t = 0; t < T; ++t)
 #pragma unroll
@@ -354,10 +367,6 @@ __device__ __forceinline__ void q4_multiply(const q4_masks &masks, const q4_tile
             if (XS) f = x_scale(t, g);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                if (ONE) {
-                    sum[r][t][0] = fmaf(acc[r][t][0], XS ? f[0] * w[r].scale[g] : w[r].scale[g], sum[r][t][0]);
-                    continue;
-                }
                 const float4_t scale = {w[r].scale[g], w[r].scale[g], w[r].scale[g], w[r].scale[g]};
                 sum[r][t] = __builtin_elementwise_fma(acc[r][t], XS ? f * scale : scale, sum[r][t]);
             }
@@ -378,118 +387,134 @@ __device__ __forceinline__ void q4_store(const q4_args &a, int b, int o, float y
 
 __device__ __forceinline__ float q4_bias(const q4_args &a, int o) { return a.biases && o < a.s.outputs ? a.biases[o] : 0.f; }
 
-/* ---- small input: at most 16 rows that fit into LDS whole.  Each workgroup scales and splits the input itself, block
- * by block of 128 values, and then streams row tiles of the weights, AHEAD blocks of a wave in flight. */
-template <int TI, int PER, bool XG, bool ONE>
-__global__ __launch_bounds__(Q4_THREADS) void q4_direct_kernel(q4_args a)
+/* ---- small input: at most 4 rows that fit into LDS whole.  Each workgroup scales and splits the input itself, block
+ * by block of 128 values, and then streams the weights, AHEAD loads of a wave in flight.
+ *
+ * The matrix instruction has 16 rows, and the input at most 4: where there are fewer tiles of outputs than CUs, its rows
+ * are 4 rows of H neighbouring blocks, and its columns the weights of 16 / H outputs in these blocks.  A column's
+ * result with its own block is what counts.  So a workgroup has fewer outputs, and each operand that is read from LDS
+ * serves H blocks; but a wave then reads pieces of 256 / H bytes, which costs more than it gives with many tiles. */
+template <int TI, int PER, bool XG, int H>
+__global__ __launch_bounds__(Q4_THREADS, 4) void q4_direct_kernel(q4_args a)
 {
     constexpr int THREADS = Q4_THREADS, WAVES = Q4_WAVES;
-    constexpr int PIECES = TI == DN_F32 ? 2 : 1;
-    constexpr int AHEAD = PER == 4 ? 6 : 8, MOVES = 4;
+    constexpr int PIECES = TI == DN_F32 ? 2 : 1, WIDTH = 16 / H, BLOCK = H > 1 ? 272 : 256; /* (16 bytes more: the operand's blocks in other banks) */
+    constexpr int AHEAD = 4, MOVES = 2;
     extern __shared__ char lds[];
-    __shared__ float s_red[WAVES][16][17];
+    __shared__ float s_red[WAVES][4][WIDTH];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int kpad = a.s.kblocks * 128, pitch = kpad * 2 * PIECES + 16; /* bytes of a row: 16 more, for the banks */
-    const int part = wave % a.ksplit, own_tile = wave / a.ksplit, rows_per = WAVES / a.ksplit;
-    const int mine = (a.s.kblocks - part + a.ksplit - 1) / a.ksplit; /* this wave's blocks: part, part + ksplit, ... */
-    const int stride = gridDim.x * rows_per;
-    int tile0 = blockIdx.x * rows_per;
+    const int kblocks = a.s.kblocks, steps = (kblocks + H - 1) / H, kpad = steps * H * 128;
+    const int plane = kpad / 128 * BLOCK, pitch = plane * PIECES + 16; /* bytes of a row's halves, and of a row */
+    const int part = wave % a.ksplit, own_unit = wave / a.ksplit, units_per = WAVES / a.ksplit;
+    const int mine = (steps - part + a.ksplit - 1) / a.ksplit; /* this wave's steps of four blocks: part, part + ksplit, ... */
+    const int stride = gridDim.x * units_per, units = a.s.tiles * H;  /* a unit: four outputs */
+    const int own_block = (lane & 15) / WIDTH, own_row = lane >> 4;
+    int unit0 = blockIdx.x * units_per;
 
-    auto fetch = [&](int t, int n) { return q4_load_tile<PER>(a, min(t, a.s.tiles - 1), part + a.ksplit * n, lane); };
+    auto fetch = [&](int u, int n) {
+        const int unit = min(u, units - 1), kb = (part + a.ksplit * n) * H + own_block;
+        return q4_load_tile<PER>(a, unit / H, min(kb, kblocks - 1), (lane & 48) + unit % H * WIDTH + lane % WIDTH); /* (input behind the last block is 0) */
+    };
     const q4_masks masks;
     q4_tile<PER> w[AHEAD];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
-        if (u < mine) w[u] = fetch(tile0 + own_tile, u);
+        if (u < mine) w[u] = fetch(unit0 + own_unit, u);
 
-    /* the input: [row][pitch] halves, and [block (8-bit input with groups: group)][16 rows] factors behind them */
+    /* the input: [row][pitch] halves, and [block (8-bit input with groups: group)][4 rows] factors behind them */
     const size_t row_bytes = (size_t)a.s.inputs * (TI == DN_F32 ? 4 : TI == DN_I8 ? 1 : 2);
     float *factors = (float *)(lds + a.batch * pitch);
-    const int quads = kpad / 4;
+    const int eights = kpad / 8;
     for (int b = 0, q = tid; b < a.batch;) {
-        float x[MOVES][4];
-        int of[MOVES], at[MOVES]; /* row and four of the next items of this lane, whose loads go together */
+        float x[MOVES][8];
+        int of[MOVES], at[MOVES]; /* row and eight of the next items of this lane, whose loads go together */
 #pragma unroll
         for (int m = 0; m < MOVES; ++m) {
-            const bool in = q < quads; /* (a row shorter than the workgroup leaves some lanes out) */
+            const bool in = q < eights; /* (a row shorter than the workgroup leaves some lanes out) */
             of[m] = in ? b : a.batch;
             at[m] = q;
-            q4_load4<TI>((const char *)a.input + min(b, a.batch - 1) * row_bytes, min(q, quads - 1) * 4, a.s.inputs, x[m]);
+            q4_load8<TI>((const char *)a.input + min(b, a.batch - 1) * row_bytes, min(q, eights - 1) * 8, a.s.inputs, x[m]);
             q += THREADS;
-            if (q >= quads) {
+            if (q >= eights) {
                 q = tid;
                 ++b;
             }
         }
 #pragma unroll
-        for (int m = 0; m < MOVES; ++m) { /* 32 lanes have a block */
+        for (int m = 0; m < MOVES; ++m) { /* 16 lanes have a block */
             if (of[m] >= a.batch) continue;
-            float factor = 1;
-            half4_t hi, lo;
-            int shift = 0;
+            float factor = 1, scale = 1;
+            half8_t hi, lo;
             if (TI != DN_I8) {
-                unsigned m4 = q4_largest4(0, x[m]);
-                m4 = max(m4, dn_move<0xb1, 0xf>(m4, m4));
-                m4 = max(m4, dn_move<0x4e, 0xf>(m4, m4));
-                m4 = max(m4, dn_move<0x141, 0xf>(m4, m4));
-                m4 = max(m4, dn_move<0x140, 0xf>(m4, m4));
-                m4 = max(m4, (unsigned)__shfl_xor((int)m4, 16, 64));
-                shift = q4_shift(m4, factor);
-                if ((tid & 31) == 0) factors[(at[m] >> 5) * 16 + of[m]] = factor;
+                unsigned m8 = q4_largest8(0, x[m]);
+                m8 = max(m8, dn_move<0xb1, 0xf>(m8, m8));
+                m8 = max(m8, dn_move<0x4e, 0xf>(m8, m8));
+                m8 = max(m8, dn_move<0x141, 0xf>(m8, m8));
+                m8 = max(m8, dn_move<0x140, 0xf>(m8, m8));
+                scale = q4_scaling(m8, factor);
+                if ((tid & 15) == 0) factors[(at[m] >> 4) * 4 + of[m]] = factor;
             }
-            q4_split4(x[m], shift, hi, lo);
-            char *to = lds + of[m] * pitch + at[m] * 8;
-            *(half4_t *)to = hi;
-            if (PIECES == 2) *(half4_t *)(to + kpad * 2) = lo;
+            q4_split8(x[m], scale, hi, lo);
+            char *to = lds + of[m] * pitch + (at[m] >> 4) * BLOCK + (at[m] & 15) * 16;
+            *(half8_t *)to = hi;
+            if (PIECES == 2) *(half8_t *)(to + plane) = lo;
         }
     }
     if (XG) {
-        const int x_groups = (a.s.inputs + a.x_group - 1) / a.x_group;
-        for (int i = tid; i < a.batch * a.s.groups; i += THREADS) {
-            const int b = i / a.s.groups, g = i - b * a.s.groups;
-            factors[g * 16 + b] = g < x_groups ? a.input_scales[(long)b * x_groups + g] : 0.f;
+        const int x_groups = (a.s.inputs + a.x_group - 1) / a.x_group, groups = kpad / 128 * PER;
+        for (int i = tid; i < a.batch * groups; i += THREADS) {
+            const int b = i / groups, g = i - b * groups;
+            factors[g * 4 + b] = g < x_groups ? a.input_scales[(long)b * x_groups + g] : 0.f;
         }
     }
     __syncthreads();
 
-    constexpr bool XS = TI != DN_I8 || XG;
-    const char *base = lds + min(lane & 15, a.batch - 1) * pitch + (lane >> 4) * 16;
-    const float *row_factors = factors + (ONE ? 0 : (lane >> 4) * 4);
-    for (; tile0 < a.s.tiles; tile0 += stride) {
-        const int tile = tile0 + own_tile;
-        float4_t sum[1][1] = {{{0, 0, 0, 0}}};
+    const char *base = lds + min((lane & 15) >> 2, a.batch - 1) * pitch + (lane & 3) % H * BLOCK + (lane >> 4) * 16;
+    const float *own_factors = factors + own_block * (XG ? PER : 1) * 4 + own_row;
+    for (; unit0 < units; unit0 += stride) {
+        const int unit = unit0 + own_unit;
+        float sum = 0;
         for (int n = 0; n < mine; n += AHEAD) {
-            const bool last = n + AHEAD >= mine; /* what comes next is of the next row tile */
+            const bool last = n + AHEAD >= mine; /* what comes next is of the next unit */
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
                 if (n + u < mine) {
-                    const int kb = part + a.ksplit * (n + u);
-                    const q4_tile<PER> one[1] = {w[u]};
-                    q4_multiply<1, 1, PIECES, PER, XS, ONE>(
-                        masks, one, sum,
-                        [&](int, int piece, int step) { return *(const half8_t *)(base + piece * kpad * 2 + kb * 256 + step * 64); },
-                        [&](int, int g) {
-                            const float *f = row_factors + (XG ? kb * PER + g : kb) * 16;
-                            return ONE ? (float4_t){*f, 0, 0, 0} : *(const float4_t *)f;
-                        });
+                    const int kb = (part + a.ksplit * (n + u)) * H;
+#pragma unroll
+                    for (int g = 0; g < PER; ++g) {
+                        half2_t z1024, z64;
+                        q4_zeros(w[u], g, z1024, z64);
+                        float4_t acc = {0, 0, 0, 0};
+#pragma unroll
+                        for (int step = g * (4 / PER); step < (g + 1) * (4 / PER); ++step) {
+                            const half8_t wv = q4_unpack8(w[u].code[step], z1024, z64, masks);
+#pragma unroll
+                            for (int p = 0; p < PIECES; ++p)
+                                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const half8_t *)(base + p * plane + kb * BLOCK + step * 64), wv, acc, 0, 0, 0);
+                        }
+                        const float v = own_block == 0 ? acc[0] : own_block == 1 ? acc[1] : own_block == 2 ? acc[2] : acc[3];
+                        const float f = TI != DN_I8 || XG ? own_factors[(XG ? kb * PER + g : kb) * 4] : 1.f;
+                        sum = fmaf(v, f * w[u].scale[g], sum);
+                    }
                 }
-                if (last ? u < mine && tile0 + stride < a.s.tiles : n + AHEAD + u < mine)
-                    w[u] = fetch(last ? tile + stride : tile, last ? u : n + AHEAD + u);
+                if (last ? u < mine && unit0 + stride < units : n + AHEAD + u < mine)
+                    w[u] = fetch(last ? unit + stride : unit, last ? u : n + AHEAD + u);
             }
         }
-        /* what the waves of a row tile have, added in their order; a thread for each output of each row */
+        /* what the blocks and the waves of a unit have, added in their order; a thread for each output of each row */
+        if (H >= 2) sum += dn_move<0x128, 0xf>(sum, sum); /* the lane 8, then 4 on among 16 */
+        if (H == 4) sum += dn_move<0x124, 0xf>(sum, sum);
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < (ONE ? 1 : 4); ++i) s_red[wave][(lane >> 4) * 4 + i][lane & 15] = sum[0][0][i];
+        if (own_block == 0) s_red[wave][own_row][lane % WIDTH] = sum;
         __syncthreads();
-        for (int i = tid; i < rows_per * a.batch * 16; i += THREADS) {
-            const int r = i / (a.batch * 16), b = (i >> 4) % a.batch, o = (tile0 + r) * 16 + (i & 15);
+        for (int i = tid; i < units_per * a.batch * WIDTH; i += THREADS) {
+            const int r = i / (a.batch * WIDTH), b = i / WIDTH % a.batch, o = (unit0 + r) * WIDTH + i % WIDTH;
             if (o >= a.s.outputs) continue;
             const float bias = q4_bias(a, o);
             float y = 0;
 #pragma unroll
             for (int q = 0; q < WAVES; ++q)
-                if (q < a.ksplit) y += s_red[r * a.ksplit + q][b][i & 15];
+                if (q < a.ksplit) y += s_red[r * a.ksplit + q][b][i % WIDTH];
             if (TI == DN_I8 && !XG) y *= a.input_scales[b];
             q4_store(a, b, o, y, bias);
         }
@@ -517,38 +542,31 @@ __global__ __launch_bounds__(256) void q4_prepare_kernel(q4_args a)
     const int tid = threadIdx.x, b = blockIdx.x, block = q4_block_bytes(a.s, PIECES, XG);
     const size_t row_bytes = (size_t)a.s.inputs * (TI == DN_F32 ? 4 : TI == DN_I8 ? 1 : 2);
     const char *row = (const char *)a.input + b * row_bytes;
-    int shift = 0;
-    float factor = 1;
+    float factor = 1, scale = 1;
     if (TI != DN_I8) {
         unsigned m = 0;
 #pragma unroll 4
-        for (int k = tid * 4; k < a.s.inputs; k += 1024) {
-            float x[4];
-            q4_load4<TI>(row, k, a.s.inputs, x);
-            m = q4_largest4(m, x);
+        for (int k = tid * 8; k < a.s.inputs; k += 2048) {
+            float x[8];
+            q4_load8<TI>(row, k, a.s.inputs, x);
+            m = q4_largest8(m, x);
         }
         m = dn_wave_max(m);
         if ((tid & 63) == 0) s_largest[tid >> 6] = m;
         __syncthreads();
-        shift = q4_shift(max(max(s_largest[0], s_largest[1]), max(s_largest[2], s_largest[3])), factor);
+        scale = q4_scaling(max(max(s_largest[0], s_largest[1]), max(s_largest[2], s_largest[3])), factor);
     }
     if (tid == 0)
         ((float *)(a.workspace + q4_rows_at(a.s, PIECES, a.batch, XG)))[b] = TI == DN_I8 ? (XG ? 1.f : a.input_scales[b]) : factor;
     unsigned char *out = a.workspace + (size_t)(b >> 4) * a.s.kblocks * block + (b & 15) * 16;
     for (int k = tid * 8; k < a.s.kblocks * 128; k += 2048) {
         float x[8];
-        half4_t hi[2], lo[2];
-        q4_load4<TI>(row, k, a.s.inputs, x);
-        q4_load4<TI>(row, k + 4, a.s.inputs, x + 4);
-        q4_split4(x, shift, hi[0], lo[0]);
-        q4_split4(x + 4, shift, hi[1], lo[1]);
+        half8_t hi, lo;
+        q4_load8<TI>(row, k, a.s.inputs, x);
+        q4_split8(x, scale, hi, lo);
         unsigned char *to = out + (size_t)(k >> 7) * block + ((k >> 5) & 3) * 1024 + ((k >> 3) & 3) * 256;
-        ((half4_t *)to)[0] = hi[0];
-        ((half4_t *)to)[1] = hi[1];
-        if (PIECES == 2) {
-            ((half4_t *)(to + 4096))[0] = lo[0];
-            ((half4_t *)(to + 4096))[1] = lo[1];
-        }
+        *(half8_t *)to = hi;
+        if (PIECES == 2) *(half8_t *)(to + 4096) = lo;
     }
     if (XG) {
         const int x_groups = (a.s.inputs + a.x_group - 1) / a.x_group, per = 128 / a.s.group;
@@ -638,16 +656,35 @@ __global__ __launch_bounds__(Q4_THREADS) void q4_stream_kernel(q4_args a)
     }
 }
 
-/* Stores 16 rows of WIDTH outputs from LDS. */
-template <int THREADS, int WIDTH, int PITCH>
-__device__ __forceinline__ void q4_store_rows(const q4_args &a, const float *s_sum, const float *row_factors, int b0, int o0)
+/* Four neighbouring outputs of a row, in one access where they exist, whatever their alignment. */
+template <class E>
+__device__ __forceinline__ void q4_put4(E *p, int n, float4_t y)
 {
-    const int rows = min(16, a.batch - b0);
-#pragma unroll 2
-    for (int i = threadIdx.x; i < rows * WIDTH; i += THREADS) {
-        const int row = i / WIDTH, o = o0 + i % WIDTH;
-        if (o < a.s.outputs) q4_store(a, b0 + row, o, s_sum[row * PITCH + i % WIDTH] * row_factors[b0 + row], q4_bias(a, o));
+    typedef E E4 __attribute__((ext_vector_type(4)));
+    typedef E4 E4U __attribute__((aligned(sizeof(E))));
+    if (n >= 4) {
+        *(E4U *)p = __builtin_convertvector(y, E4);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (i < n) p[i] = (E)y[i];
     }
+}
+
+__device__ __forceinline__ void q4_store4(const q4_args &a, int b, int o, float4_t y)
+{
+    if (a.activation != DN_LINEAR)
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+            const float x = dn_activate(i == 0 ? y[0] : i == 1 ? y[1] : i == 2 ? y[2] : y[3], a.activation);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = i == e ? x : y[e];
+        }
+    const long at = (long)b * a.s.outputs + o;
+    const int n = a.s.outputs - o;
+    if (a.output_type == DN_F32) q4_put4((float *)a.output + at, n, y);
+    else if (a.output_type == DN_F16) q4_put4((_Float16 *)a.output + at, n, y);
+    else q4_put4((__bf16 *)a.output + at, n, y);
 }
 
 /* ---- second pass, many outputs: a workgroup takes 4 * R row tiles, R for each wave, and T tiles of input rows.  The
@@ -658,10 +695,11 @@ template <int T, int R, int PIECES, int PER, bool XG>
 __global__ __launch_bounds__(Q4_STAGED_WAVES * 64, 2) void q4_staged_kernel(q4_args a)
 {
     constexpr int THREADS = Q4_STAGED_WAVES * 64;
-    constexpr int UNITS = 4 / (T * PIECES > 4 ? 4 : T * PIECES); /* blocks of a chunk */
+    constexpr int UNITS = T * PIECES >= 2 ? 1 : 2; /* blocks of a chunk */
     constexpr int BLOCK = PIECES * 4096 + (XG ? PER * 64 : 0), SPAN = UNITS * BLOCK, CHUNK = T * SPAN;
     constexpr int MOVES = (CHUNK + THREADS * 16 - 1) / (THREADS * 16);
     __shared__ uint4_t s_input[2][CHUNK / 16];
+    __shared__ float s_factors[T * 16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int x_tiles = (a.batch + 15) / 16, x0 = blockIdx.y * T, tile0 = (blockIdx.x * Q4_STAGED_WAVES + wave) * R;
     const int kblocks = a.s.kblocks, chunks = (kblocks + UNITS - 1) / UNITS;
@@ -671,56 +709,70 @@ __global__ __launch_bounds__(Q4_STAGED_WAVES * 64, 2) void q4_staged_kernel(q4_a
 #pragma unroll
         for (int t = 0; t < T; ++t) sum[r][t] = (float4_t){0, 0, 0, 0};
 
+    if (tid < T * 16) s_factors[tid] = ((const float *)(a.workspace + q4_rows_at(a.s, PIECES, a.batch, XG)))[min(x0 * 16 + tid, a.batch - 1)];
     const q4_masks masks;
-    uint4_t moved[MOVES];
-    auto input_of = [&](int c) {
+    uint4_t moved[2][MOVES];
+    auto input_of = [&](int c, uint4_t (&to)[MOVES]) {
 #pragma unroll
         for (int m = 0; m < MOVES; ++m) { /* what lies behind the last block or tile is read at its place, and not multiplied */
-            const int i = min((m * THREADS + tid) * 16, CHUNK - 16), t = i / SPAN, in = i % SPAN;
+            const int at = (m * THREADS + tid) * 16, i = (m + 1) * THREADS * 16 <= CHUNK ? at : min(at, CHUNK - 16), t = i / SPAN, in = i % SPAN;
             const int kb = min(c * UNITS + in / BLOCK, kblocks - 1);
-            moved[m] = *(const uint4_t *)(a.workspace + ((size_t)min(x0 + t, x_tiles - 1) * kblocks + kb) * BLOCK + in % BLOCK);
+            to[m] = *(const uint4_t *)(a.workspace + ((size_t)min(x0 + t, x_tiles - 1) * kblocks + kb) * BLOCK + in % BLOCK);
         }
+        __builtin_amdgcn_sched_barrier(0);
     };
-    auto keep_input = [&](int buffer) {
+    auto keep_input = [&](int buffer, const uint4_t (&from)[MOVES]) {
 #pragma unroll
         for (int m = 0; m < MOVES; ++m)
-            if ((m * THREADS + tid) * 16 < CHUNK) s_input[buffer][m * THREADS + tid] = moved[m];
+            if ((m + 1) * THREADS * 16 <= CHUNK || (m * THREADS + tid) * 16 < CHUNK) s_input[buffer][m * THREADS + tid] = from[m];
     };
-    q4_tile<PER> w[UNITS][R];
-    auto fetch = [&](int c, int u) {
+    q4_tile<PER> w[2][UNITS][R];
+    auto fetch = [&](int c, int u, q4_tile<PER> (&to)[R]) {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            w[u][r] = q4_load_tile<PER>(a, min(tile0 + r, a.s.tiles - 1), min(c * UNITS + u, kblocks - 1), lane);
+            to[r] = q4_load_tile<PER>(a, min(tile0 + r, a.s.tiles - 1), min(c * UNITS + u, kblocks - 1), lane);
+        __builtin_amdgcn_sched_barrier(0);
     };
-    input_of(0);
+    /* Two chunks on their way, input and weights in turn: loads return in their order, so that a wait for input that was
+     * asked for behind weights would be a wait for those as well.  No load is conditional (behind the last chunk they
+     * repeat the last block): the compiler waits for every load that may have been left out. */
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) fetch(0, u);
-    keep_input(0);
+    for (int h = 0; h < 2; ++h) {
+        input_of(h, moved[h]);
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) fetch(h, u, w[h][u]);
+    }
+    keep_input(0, moved[0]);
     __syncthreads();
-    for (int c = 0; c < chunks; ++c) {
-        if (c + 1 < chunks) input_of(c + 1);
-        const char *base = (const char *)s_input[c & 1];
+    for (int c0 = 0; c0 < chunks; c0 += 2) {
 #pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-            if (c * UNITS + u < kblocks)
-                q4_multiply<T, R, PIECES, PER, XG>(
-                    masks, w[u], sum,
-                    [&](int t, int piece, int step) {
-                        return *(const half8_t *)(base + t * SPAN + u * BLOCK + piece * 4096 + step * 1024 + lane * 16);
-                    },
-                    [&](int t, int g) { return *(const float4_t *)(base + t * SPAN + u * BLOCK + PIECES * 4096 + g * 64 + (lane >> 4) * 16); });
-            if (c + 1 < chunks) fetch(c + 1, u);
+        for (int h = 0; h < 2; ++h) {
+            const int c = c0 + h;
+            input_of(c + 2, moved[h]);
+            const char *base = (const char *)s_input[h];
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) {
+                if (c * UNITS + u < kblocks)
+                    q4_multiply<T, R, PIECES, PER, XG>(
+                        masks, w[h][u], sum,
+                        [&](int t, int piece, int step) {
+                            return *(const half8_t *)(base + t * SPAN + u * BLOCK + piece * 4096 + step * 1024 + lane * 16);
+                        },
+                        [&](int t, int g) { return *(const float4_t *)(base + t * SPAN + u * BLOCK + PIECES * 4096 + g * 64 + (lane >> 4) * 16); });
+                fetch(c + 2, u, w[h][u]);
+            }
+            keep_input(h ^ 1, moved[h ^ 1]); /* the buffer that all waves have left at the last barrier */
+            __syncthreads();
         }
-        if (c + 1 < chunks) keep_input((c + 1) & 1); /* the buffer that all waves have left at the last barrier */
-        __syncthreads();
     }
     /* The sums go through LDS, a tile of input rows at a time, so that neighbouring lanes store neighbouring outputs
-     * (16 of a row alone are half a line) and there is one copy of the activation's code. */
-    const float *row_factors = (const float *)(a.workspace + q4_rows_at(a.s, PIECES, a.batch, XG));
+     * (16 of a row alone are half a line), four each, and there is one copy of the activation's code. */
     constexpr int WIDTH = Q4_STAGED_WAVES * R * 16, PITCH = WIDTH + 4;
     static_assert(sizeof s_input >= 16 * PITCH * 4, "room for a tile's sums");
     float *s_sum = (float *)s_input;
-    const int o0 = blockIdx.x * WIDTH;
+    const int column = tid % (WIDTH / 4) * 4, o = blockIdx.x * WIDTH + column;
+    const float4_t bias = {q4_bias(a, o), q4_bias(a, o + 1), q4_bias(a, o + 2), q4_bias(a, o + 3)};
 #pragma unroll 1
     for (int x = 0; x < T; ++x) {
 #pragma unroll
@@ -732,7 +784,13 @@ __global__ __launch_bounds__(Q4_STAGED_WAVES * 64, 2) void q4_staged_kernel(q4_a
             for (int i = 0; i < 4; ++i) s_sum[((lane >> 4) * 4 + i) * PITCH + (wave * R + r) * 16 + (lane & 15)] = v[i];
         }
         __syncthreads();
-        q4_store_rows<THREADS, WIDTH, PITCH>(a, s_sum, row_factors, (x0 + x) * 16, o0);
+#pragma unroll 1
+        for (int row = tid / (WIDTH / 4); row < 16; row += THREADS / (WIDTH / 4)) {
+            const int b = (x0 + x) * 16 + row;
+            const float f = s_factors[x * 16 + row];
+            const float4_t factor = {f, f, f, f};
+            if (b < a.batch && o < a.s.outputs) q4_store4(a, b, o, __builtin_elementwise_fma(*(const float4_t *)(s_sum + row * PITCH + column), factor, bias));
+        }
         __syncthreads();
     }
 }
@@ -745,7 +803,7 @@ __global__ __launch_bounds__(Q4_STAGED_WAVES * 64, 2) void q4_staged_kernel(q4_a
  *   stream  the others */
 struct q4_plan {
     enum { DIRECT, STREAM, STAGED } form;
-    int ksplit, t, r;
+    int ksplit, h, t, r;
     unsigned gx, gy;
     size_t lds;
 };
@@ -754,14 +812,16 @@ static q4_plan q4_plan_of(const q4_shape &s, int type, int batch)
 {
     q4_plan p;
     const int pieces = type == DN_F32 ? 2 : 1, x_tiles = (int)(((long)batch + 15) / 16);
-    p.ksplit = p.t = p.r = 1;
+    p.ksplit = p.h = p.t = p.r = 1;
     p.gy = 1;
-    p.lds = batch * ((size_t)s.kblocks * 256 * pieces + 16) + (size_t)(type == DN_I8 ? s.groups : s.kblocks) * 64;
+    while (p.h < 4 && (long)s.tiles * p.h <= 128 && s.kblocks > p.h) p.h *= 2;
+    const int steps = (s.kblocks + p.h - 1) / p.h;
+    p.lds = batch * ((size_t)steps * p.h * (p.h > 1 ? 272 : 256) * pieces + 16) + (size_t)steps * p.h * (type == DN_I8 ? 128 / s.group : 1) * 16;
     if (batch <= 4 && (long)batch * s.inputs <= 28672 && p.lds <= 120 << 10) {
         p.form = q4_plan::DIRECT;
-        /* waves share a row tile as long as each has a block and the chip is not full */
-        while (p.ksplit < Q4_WAVES && (long)s.tiles * p.ksplit < 256 * Q4_WAVES && p.ksplit * 2 <= s.kblocks) p.ksplit *= 2;
-        const long groups = ((long)s.tiles * p.ksplit + Q4_WAVES - 1) / Q4_WAVES;
+        /* waves share outputs as long as each has blocks and two workgroups a CU are not reached */
+        while (p.ksplit < Q4_WAVES && (long)s.tiles * p.h * p.ksplit <= 256 * Q4_WAVES && p.ksplit * 2 <= steps) p.ksplit *= 2;
+        const long groups = ((long)s.tiles * p.h * p.ksplit + Q4_WAVES - 1) / Q4_WAVES;
         p.gx = (unsigned)(groups < 512 ? groups : 512);
         return p;
     }
@@ -805,8 +865,10 @@ static void q4_launch(const q4_args &a, const q4_plan &p)
 {
     constexpr int PIECES = TI == DN_F32 ? 2 : 1;
     if (p.form == q4_plan::DIRECT) {
-        if (a.batch == 1) hipLaunchKernelGGL((q4_direct_kernel<TI, PER, XG, true>), dim3(p.gx), dim3(Q4_THREADS), p.lds, dn_stream(), a);
-        else hipLaunchKernelGGL((q4_direct_kernel<TI, PER, XG, false>), dim3(p.gx), dim3(Q4_THREADS), p.lds, dn_stream(), a);
+        const dim3 grid(p.gx), block(Q4_THREADS);
+        if (p.h == 1) hipLaunchKernelGGL((q4_direct_kernel<TI, PER, XG, 1>), grid, block, p.lds, dn_stream(), a);
+        else if (p.h == 2) hipLaunchKernelGGL((q4_direct_kernel<TI, PER, XG, 2>), grid, block, p.lds, dn_stream(), a);
+        else hipLaunchKernelGGL((q4_direct_kernel<TI, PER, XG, 4>), grid, block, p.lds, dn_stream(), a);
         return;
     }
     hipLaunchKernelGGL((q4_prepare_kernel<TI, XG>), dim3((unsigned)a.batch), dim3(256), 0, dn_stream(), a);

@@ -457,14 +457,15 @@ __device__ __forceinline__ void answer(const sample_args &a, long row, int token
     if (a.probs) a.probs[row] = total ? (float)((double)mass / (double)total) : 0.f;
 }
 
-/* Four (eight) neighbouring tokens from i on; -inf behind `end`. */
+/* Four (eight) neighbouring tokens from i on, in one access whatever their alignment; -inf behind `end`. */
 template <int T>
-__device__ __forceinline__ void load4(const typename dn_elt<T>::store *x, int i, int end, bool vectors, float *l)
+__device__ __forceinline__ void load4(const typename dn_elt<T>::store *x, int i, int end, float *l)
 {
     typedef typename dn_elt<T>::store S;
     typedef S S4 __attribute__((ext_vector_type(4)));
-    if (vectors && i + 4 <= end) {
-        const S4 u = *(const S4 *)(x + i);
+    typedef S4 S4U __attribute__((aligned(sizeof(S))));
+    if (i + 4 <= end) {
+        const S4 u = *(const S4U *)(x + i);
 #pragma unroll
         for (int e = 0; e < 4; ++e) l[e] = (float)u[e];
     } else {
@@ -474,17 +475,19 @@ __device__ __forceinline__ void load4(const typename dn_elt<T>::store *x, int i,
 }
 
 template <int T>
-__device__ __forceinline__ void load8(const typename dn_elt<T>::store *x, int i, int end, bool vectors, float l[8])
+__device__ __forceinline__ void load8(const typename dn_elt<T>::store *x, int i, int end, float l[8])
 {
-    load4<T>(x, i, end, vectors, l);
-    load4<T>(x, i + 4, end, vectors, l + 4);
-}
-
-template <int T>
-__device__ __forceinline__ bool rows_aligned(const sample_args &a)
-{
-    const int size = sizeof(typename dn_elt<T>::store);
-    return ((uintptr_t)a.logits & 15) == 0 && ((a.stride * size) & 15) == 0;
+    typedef typename dn_elt<T>::store S;
+    typedef S S8 __attribute__((ext_vector_type(8)));
+    typedef S8 S8U __attribute__((aligned(sizeof(S))));
+    if (i + 8 <= end) {
+        const S8 u = *(const S8U *)(x + i);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) l[e] = (float)u[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) l[e] = i + e < end ? (float)x[i + e] : -INFINITY;
+    }
 }
 
 /* ---- a row of up to 8192 tokens: one workgroup, the row in registers ---------------------------------- */
@@ -497,7 +500,6 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
     __shared__ float row_lds[THREADS * (E + 1)]; /* E neighbours a lane; the gap spreads them over the banks */
     __shared__ unsigned s_count;
     const int tid = threadIdx.x;
-    const bool vectors = rows_aligned<T>(a);
     const sample_places<T> places = {a.index_bits};
     float *own_l = row_lds + tid * (E + 1);
     for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -507,7 +509,7 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
 #pragma unroll
         for (int e = 0; e < E; e += 4) {
             float l[4];
-            load4<T>(x, tid * E + e, a.n, vectors, l);
+            load4<T>(x, tid * E + e, a.n, l);
             widen(ends, l);
 #pragma unroll
             for (int i = 0; i < 4; ++i) own_l[e + i] = l[i];
@@ -614,14 +616,13 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_largest_kernel(sample
     typedef typename dn_elt<T>::store S;
     __shared__ float2_t part[SM_SPLIT_THREADS / 64];
     const sample_space ws = space_of(a.rows, a.segments);
-    const bool vectors = rows_aligned<T>(a);
     for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
         const S *x = (const S *)a.logits + row * a.stride;
         const int lo = blockIdx.x * a.length, hi = min(a.n, lo + a.length);
         float2_t ends = {-INFINITY, INFINITY};
         for (int i = lo + threadIdx.x * 8; i < hi; i += SM_STRIP) {
             float l[8];
-            load8<T>(x, i, hi, vectors, l);
+            load8<T>(x, i, hi, l);
             widen(ends, l);
             widen(ends, l + 4);
         }
@@ -661,7 +662,6 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_bins_kernel(sample_ar
     __shared__ u64 mass[SM_BINS];
     __shared__ unsigned count[SM_BINS];
     const sample_space ws = space_of(a.rows, a.segments);
-    const bool vectors = rows_aligned<T>(a);
     const int tid = threadIdx.x;
     for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
         sample_row r = settings_of(a, row);
@@ -677,7 +677,7 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_bins_kernel(sample_ar
         __syncthreads();
         for (int i = lo + tid * 8; i < hi; i += SM_STRIP) {
             float l[8];
-            load8<T>(x, i, hi, vectors, l);
+            load8<T>(x, i, hi, l);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 if (!(l[e] > -INFINITY)) continue;
@@ -702,7 +702,6 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_kept_kernel(sample_ar
     __shared__ u64 s_list[SM_FOUND];
     __shared__ unsigned s_count, s_from;
     const sample_space ws = space_of(a.rows, a.segments);
-    const bool vectors = rows_aligned<T>(a);
     const sample_places<T> places = {a.index_bits};
     const int tid = threadIdx.x;
     for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
@@ -725,7 +724,7 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_kept_kernel(sample_ar
             const int to = min(hi, from + a.block);
             for (int i = from + tid * 8; i < to; i += SM_STRIP) {
                 float l[8];
-                load8<T>(x, i, to, vectors, l);
+                load8<T>(x, i, to, l);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     if (!(l[e] > -INFINITY)) continue;
@@ -770,7 +769,6 @@ __global__ __launch_bounds__(SM_DRAW_THREADS) void sample_draw_kernel(sample_arg
     __shared__ u64 s_before;
     __shared__ int s_block;
     const sample_space ws = space_of(a.rows, a.segments);
-    const bool vectors = rows_aligned<T>(a);
     const sample_places<T> places = {a.index_bits};
     const int tid = threadIdx.x, blocks = (a.n + a.block - 1) / a.block;
     for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -803,7 +801,7 @@ __global__ __launch_bounds__(SM_DRAW_THREADS) void sample_draw_kernel(sample_arg
             __syncthreads();
             auto strip_at = [&](int i) {
                 float l[8], *to = strip + tid * P;
-                load8<T>(x, i, a.n, vectors, l);
+                load8<T>(x, i, a.n, l);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) to[e] = l[e];
                 return to;
@@ -830,7 +828,7 @@ __global__ __launch_bounds__(SM_DRAW_THREADS) void sample_draw_kernel(sample_arg
         for (int from = lo; from < hi; from += SM_STRIP) {
             const int i = from + tid * 4;
             float l[4];
-            load4<T>(x, i, hi, vectors, l);
+            load4<T>(x, i, hi, l);
 #pragma unroll
             for (int e = 0; e < 4; ++e) strip[tid * P + e] = l[e];
             auto kept_mass = [&](int e) {
