@@ -817,7 +817,7 @@ static q4_plan q4_plan_of(const q4_shape &s, int type, int batch)
     while (p.h < 4 && (long)s.tiles * p.h <= 128 && s.kblocks > p.h) p.h *= 2;
     const int steps = (s.kblocks + p.h - 1) / p.h;
     p.lds = batch * ((size_t)steps * p.h * (p.h > 1 ? 272 : 256) * pieces + 16) + (size_t)steps * p.h * (type == DN_I8 ? 128 / s.group : 1) * 16;
-    if (batch <= 4 && (long)batch * s.inputs <= 28672 && p.lds <= 120 << 10) {
+    if (batch <= 4 && p.lds <= 150 << 10) {
         p.form = q4_plan::DIRECT;
         /* waves share outputs as long as each has blocks and two workgroups a CU are not reached */
         while (p.ksplit < Q4_WAVES && (long)s.tiles * p.h * p.ksplit <= 256 * Q4_WAVES && p.ksplit * 2 <= steps) p.ksplit *= 2;

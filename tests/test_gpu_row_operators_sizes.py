@@ -28,7 +28,8 @@ def test_q4_forms(dn, batch, k, n):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("batch,k", [(1, 26000), (1, 28672), (1, 30000), (2, 14336), (3, 9500), (4, 7168), (4, 7169)])
+@pytest.mark.parametrize("batch,k", [(1, 26000), (1, 28672), (1, 30000), (2, 14336), (3, 9500), (4, 7168), (4, 7169),
+                                     (1, 35000), (1, 37000), (1, 70000), (1, 74000), (2, 36700), (4, 9000), (4, 18300), (4, 19000)])
 def test_q4_long_rows(dn, kind, batch, k):
     tx, group, xg = kind
     Q4(dn, k + batch, k, 37, group).check(dn, k, batch, tx, F32, xg=xg)
