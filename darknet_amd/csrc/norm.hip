@@ -277,6 +277,7 @@ static void norm_launch(const norm_args &a)
     if (runs <= 64) NM_LAUNCH(64, 1);
     else if (runs <= 128) NM_LAUNCH(128, 1);
     else if (runs <= 256) NM_LAUNCH(256, 1);
+    else if (V == 8 && runs <= 512) NM_LAUNCH(512, 1);
     else if (runs <= 512) NM_LAUNCH(256, 2);
     else if (runs <= 1024) NM_LAUNCH(512, 2);
     else if (runs <= 2048) NM_LAUNCH(1024, 2);

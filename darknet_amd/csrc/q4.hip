@@ -590,44 +590,39 @@ __device__ __forceinline__ void q4_store_tile(const q4_args &a, const float *row
     }
 }
 
-/* ---- second pass, few outputs: a workgroup takes R row tiles and T tiles of input rows, its eight waves an eighth of
+/* ---- second pass, few outputs: a workgroup takes R row tiles and a tile of input rows, its eight waves an eighth of
  * the inputs each.  No two waves read the same input, so that it comes straight into registers like the weights, both
  * a block ahead, and nothing waits for another wave before the end. */
-template <int T, int R, int PIECES, int PER, bool XG>
+template <int R, int PIECES, int PER, bool XG>
 __global__ __launch_bounds__(Q4_THREADS) void q4_stream_kernel(q4_args a)
 {
     __shared__ float4_t s_red[Q4_WAVES][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int block = q4_block_bytes(a.s, PIECES, XG), x_tiles = (a.batch + 15) / 16, x0 = blockIdx.y * T, tile0 = blockIdx.x * R;
+    const int block = q4_block_bytes(a.s, PIECES, XG), x_tile = blockIdx.y, tile0 = blockIdx.x * R;
     const int mine = (a.s.kblocks - wave + Q4_WAVES - 1) / Q4_WAVES;
     struct block_data {
         q4_tile<PER> w[R];
-        half8_t x[T][PIECES][4];
-        float4_t f[T][PER];
+        half8_t x[PIECES][4];
+        float4_t f[PER];
     };
     auto fetch = [&](int n, block_data &d) {
         const int kb = wave + n * Q4_WAVES;
 #pragma unroll
         for (int r = 0; r < R; ++r) d.w[r] = q4_load_tile<PER>(a, min(tile0 + r, a.s.tiles - 1), kb, lane);
+        const unsigned char *p = a.workspace + ((size_t)x_tile * a.s.kblocks + kb) * block;
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
-            const unsigned char *p = a.workspace + ((size_t)min(x0 + t, x_tiles - 1) * a.s.kblocks + kb) * block;
+        for (int i = 0; i < 4 * PIECES; ++i) d.x[i / 4][i % 4] = *(const half8_t *)(p + i * 1024 + lane * 16);
+        if (XG)
 #pragma unroll
-            for (int i = 0; i < 4 * PIECES; ++i) d.x[t][i / 4][i % 4] = *(const half8_t *)(p + i * 1024 + lane * 16);
-            if (XG)
-#pragma unroll
-                for (int g = 0; g < PER; ++g) d.f[t][g] = *(const float4_t *)(p + PIECES * 4096 + g * 64 + (lane >> 4) * 16);
-        }
+            for (int g = 0; g < PER; ++g) d.f[g] = *(const float4_t *)(p + PIECES * 4096 + g * 64 + (lane >> 4) * 16);
     };
-    float4_t sum[R][T];
+    float4_t sum[R][1];
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int t = 0; t < T; ++t) sum[r][t] = (float4_t){0, 0, 0, 0};
+    for (int r = 0; r < R; ++r) sum[r][0] = (float4_t){0, 0, 0, 0};
     const q4_masks masks;
     auto multiply = [&](const block_data &d) {
-        q4_multiply<T, R, PIECES, PER, XG>(
-            masks, d.w, sum, [&](int t, int piece, int step) { return d.x[t][piece][step]; }, [&](int t, int g) { return d.f[t][g]; });
+        q4_multiply<1, R, PIECES, PER, XG>(
+            masks, d.w, sum, [&](int, int piece, int step) { return d.x[piece][step]; }, [&](int, int g) { return d.f[g]; });
     };
     block_data one, two;
     if (mine > 0) fetch(0, one);
@@ -640,18 +635,15 @@ __global__ __launch_bounds__(Q4_THREADS) void q4_stream_kernel(q4_args a)
     /* the waves' sums, in their order; each wave joins what falls to it */
     const float *row_factors = (const float *)(a.workspace + q4_rows_at(a.s, PIECES, a.batch, XG));
 #pragma unroll 1
-    for (int k = 0; k < R * T; ++k) {
-        float4_t v = sum[0][0];
-#pragma unroll
-        for (int m = 1; m < R * T; ++m) v = k == m ? sum[m / T][m % T] : v;
+    for (int k = 0; k < R; ++k) {
         __syncthreads();
-        s_red[wave][lane] = v;
+        s_red[wave][lane] = R > 1 && k == 1 ? sum[R - 1][0] : sum[0][0];
         __syncthreads();
-        if (wave == k && tile0 + k / T < a.s.tiles && x0 + k % T < x_tiles) { /* R * T <= 8 */
-            v = s_red[0][lane];
+        if (wave == k && tile0 + k < a.s.tiles) {
+            float4_t v = s_red[0][lane];
 #pragma unroll
             for (int q = 1; q < Q4_WAVES; ++q) v += s_red[q][lane];
-            q4_store_tile(a, row_factors, tile0 + k / T, (x0 + k % T) * 16, v);
+            q4_store_tile(a, row_factors, tile0 + k, x_tile * 16, v);
         }
     }
 }
@@ -827,14 +819,13 @@ static q4_plan q4_plan_of(const q4_shape &s, int type, int batch)
     }
     p.lds = 0;
     const int passes = (x_tiles + 3) / 4;
-    if ((long)s.tiles * x_tiles >= 2800) {
+    if ((long)s.tiles * x_tiles >= 2300) {
         p.form = q4_plan::STAGED;
         p.t = (x_tiles + passes - 1) / passes;
         p.r = s.group > 32 && (long)s.tiles * passes >= Q4_STAGED_WAVES * 2 * 384 ? 2 : 1;
         p.gx = (unsigned)((s.tiles + Q4_STAGED_WAVES * p.r - 1) / (Q4_STAGED_WAVES * p.r));
     } else {
         p.form = q4_plan::STREAM;
-        p.t = pieces == 1 && x_tiles > 1 ? 2 : 1;
         p.r = s.group > 32 && s.tiles >= 2 * 192 ? 2 : 1;
         p.gx = (unsigned)((s.tiles + p.r - 1) / p.r);
     }
@@ -856,8 +847,8 @@ static void q4_launch_second(const q4_args &a, const q4_plan &p)
     const dim3 grid(p.gx, p.gy);
     if (p.form == q4_plan::STAGED)
         hipLaunchKernelGGL((q4_staged_kernel<T, R, PIECES, PER, XG>), grid, dim3(Q4_STAGED_WAVES * 64), 0, dn_stream(), a);
-    else if constexpr (T * PIECES <= 2)
-        hipLaunchKernelGGL((q4_stream_kernel<T, R, PIECES, PER, XG>), grid, dim3(Q4_THREADS), 0, dn_stream(), a);
+    else if constexpr (T == 1)
+        hipLaunchKernelGGL((q4_stream_kernel<R, PIECES, PER, XG>), grid, dim3(Q4_THREADS), 0, dn_stream(), a);
 }
 
 template <int TI, int PER, bool XG>
