@@ -115,7 +115,11 @@ __device__ __forceinline__ void store_run(E *p, int i, int n, const float *v)
  * RUNS = 0: as many runs as the row has, read again for each step (from the stored sum, if there is one).
  * A group of 8-bit values is a power of two of neighbouring lanes' runs, so that its maximum takes lane moves only.
  *
- * The 8-bit form works on p = s * scales, exact in 64 bits: max|y| = max|p| * r, and code = rint(p * (r / c)). */
+ * The 8-bit form works on p = s * scales, exact in 64 bits: max|y| = max|p| * r, and code = rint(p * (r / c)).
+ *
+ * Bound by memory: 16384 x 4096 fp32 with residual, sum and output (1.07 GB) 187 us, 5.7 TB/s, where a copy reaches
+ * 5.1; 4096 x 8192 bf16 likewise 60 us, 4.5 TB/s.  With 8-bit output in groups of 128 (236 MB) 66 us, 3.6 TB/s: half
+ * the time is in its 600 vector instructions for 16 values a lane.  One row of 4096: 3 us, a launch. */
 template <int T, int THREADS, int RUNS, int V, bool Q8>
 __global__ __launch_bounds__(THREADS) void rmsnorm_kernel(norm_args a)
 {
@@ -265,7 +269,9 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_kernel(norm_args a)
 }
 
 /* Which form a row takes: one run a lane up to 256 lanes, then two, so that several rows share a CU and their loads
- * and stores overlap; a row of more than 16384 values is read again for each step. */
+ * and stores overlap (2048 fp32 to 8 bits: 47 us by 256 lanes, 55 by 512; 8192 bf16: 66 by 512, 69 by 1024, 90 by 256 with
+ * four), but for 16-bit rows of 257 to 512 runs of eight, whose two runs take the registers of a row more (4096 bf16: 27.7
+ * by 512, 29.7 by 256).  A row of more than 16384 values is read again for each step. */
 template <int T, bool Q8>
 static void norm_launch(const norm_args &a)
 {

@@ -187,7 +187,11 @@ extern "C" int q4_unpack_weights_gpu(const void *packed, float *weights, int inp
  * undoes the scaling is NaN.
  *
  * The input is the instruction's first operand and the weights the second, so that a lane's results are those
- * of one output, whose scale and zero it has read beside the codes. */
+ * of one output, whose scale and zero it has read beside the codes.
+ *
+ * What bounds it: the weights are read once, half a byte each, and up to some 64 rows nothing else takes as long.  The
+ * products take a quarter of that at 16 rows; unpacking (9 vector instructions for 8 codes of a lane) is shared
+ * by all rows of a workgroup.  So each form below is built around loads that stay in flight. */
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
@@ -393,12 +397,17 @@ __device__ __forceinline__ float q4_bias(const q4_args &a, int o) { return a.bia
  * The matrix instruction has 16 rows, and the input at most 4: where there are fewer tiles of outputs than CUs, its rows
  * are 4 rows of H neighbouring blocks, and its columns the weights of 16 / H outputs in these blocks.  A column's
  * result with its own block is what counts.  So a workgroup has fewer outputs, and each operand that is read from LDS
- * serves H blocks; but a wave then reads pieces of 256 / H bytes, which costs more than it gives with many tiles. */
+ * serves H blocks; but a wave then reads pieces of 256 / H bytes, which costs more than it gives with many tiles.
+ *
+ * Measured, fp32 input: 4096 -> 4096 in groups of 128 5.2 us (1.7 TB/s; a launch that does nothing 3), 12544 -> 1715 in
+ * groups of 32 8.4 us (1.7 TB/s), 25088 -> 4096 17.5 us (3.2 TB/s).  Of the second 4 us are the launch, the first loads
+ * and the join, 1.5 the scaling of the input, the rest the weights: few CUs, each at what it can have in flight. */
 template <int TI, int PER, bool XG, int H>
 __global__ __launch_bounds__(Q4_THREADS, 4) void q4_direct_kernel(q4_args a)
 {
     constexpr int THREADS = Q4_THREADS, WAVES = Q4_WAVES;
-    constexpr int PIECES = TI == DN_F32 ? 2 : 1, WIDTH = 16 / H, BLOCK = H > 1 ? 272 : 256; /* (16 bytes more: the operand's blocks in other banks) */
+    constexpr int PIECES = TI == DN_F32 ? 2 : 1, WIDTH = 16 / H;
+    constexpr int BLOCK = H > 1 ? 272 : 256; /* bytes of a block: 16 more put the blocks of an operand in other banks */
     constexpr int AHEAD = 4, MOVES = 2;
     extern __shared__ char lds[];
     __shared__ float s_red[WAVES][4][WIDTH];
@@ -406,14 +415,15 @@ __global__ __launch_bounds__(Q4_THREADS, 4) void q4_direct_kernel(q4_args a)
     const int kblocks = a.s.kblocks, steps = (kblocks + H - 1) / H, kpad = steps * H * 128;
     const int plane = kpad / 128 * BLOCK, pitch = plane * PIECES + 16; /* bytes of a row's halves, and of a row */
     const int part = wave % a.ksplit, own_unit = wave / a.ksplit, units_per = WAVES / a.ksplit;
-    const int mine = (steps - part + a.ksplit - 1) / a.ksplit; /* this wave's steps of four blocks: part, part + ksplit, ... */
-    const int stride = gridDim.x * units_per, units = a.s.tiles * H;  /* a unit: four outputs */
+    const int mine = (steps - part + a.ksplit - 1) / a.ksplit; /* this wave's steps of H blocks: part, part + ksplit, ... */
+    const int stride = gridDim.x * units_per, units = a.s.tiles * H; /* a unit: WIDTH outputs */
     const int own_block = (lane & 15) / WIDTH, own_row = lane >> 4;
     int unit0 = blockIdx.x * units_per;
 
     auto fetch = [&](int u, int n) {
         const int unit = min(u, units - 1), kb = (part + a.ksplit * n) * H + own_block;
-        return q4_load_tile<PER>(a, unit / H, min(kb, kblocks - 1), (lane & 48) + unit % H * WIDTH + lane % WIDTH); /* (input behind the last block is 0) */
+        /* behind the last block: its weights again, for input that is 0 */
+        return q4_load_tile<PER>(a, unit / H, min(kb, kblocks - 1), (lane & 48) + unit % H * WIDTH + lane % WIDTH);
     };
     const q4_masks masks;
     q4_tile<PER> w[AHEAD];
@@ -523,7 +533,10 @@ __global__ __launch_bounds__(Q4_THREADS, 4) void q4_direct_kernel(q4_args a)
 
 /* ---- larger input, first pass: one workgroup for each row scales it and writes it in the order in which the second
  * pass feeds it to the matrix instruction: [row / 16][inputs / 128] blocks of [piece][step][lane][8 halves] and, for
- * 8-bit input with groups, [group in 128][16] factors.  Behind the blocks a factor for each row. */
+ * 8-bit input with groups, [group in 128][16] factors.  Behind the blocks a factor for each row.  A pass over a few
+ * kilobytes, 3 to 5 us with its launch; it saves every workgroup of the second pass a scaling of its own (16 rows
+ * of 8192 values read as they are by that pass, without this one: the same time in groups of 128, 27 us against 20 in
+ * groups of 32). */
 __host__ __device__ static inline int q4_block_bytes(const q4_shape &s, int pieces, bool groups)
 {
     return pieces * 4096 + (groups ? 128 / s.group * 64 : 0);
@@ -592,7 +605,11 @@ __device__ __forceinline__ void q4_store_tile(const q4_args &a, const float *row
 
 /* ---- second pass, few outputs: a workgroup takes R row tiles and a tile of input rows, its eight waves an eighth of
  * the inputs each.  No two waves read the same input, so that it comes straight into registers like the weights, both
- * a block ahead, and nothing waits for another wave before the end. */
+ * a block ahead, and nothing waits for another wave before the end.
+ *
+ * Measured: 16 rows of 8-bit input, 8192 -> 8192 in groups of 128, 14.7 us for both passes, 11 for this one (3.3 TB/s);
+ * 16 x 4096 -> 32768 bf16 21.5 us (3.4 TB/s).  Two tiles of input rows in a workgroup took longer (64 x 4096 -> 8192:
+ * 23.7 against 20.4 us: fewer waves have the registers). */
 template <int R, int PIECES, int PER, bool XG>
 __global__ __launch_bounds__(Q4_THREADS) void q4_stream_kernel(q4_args a)
 {
@@ -680,8 +697,13 @@ __device__ __forceinline__ void q4_store4(const q4_args &a, int b, int o, float4
 }
 
 /* ---- second pass, many outputs: a workgroup takes 4 * R row tiles, R for each wave, and T tiles of input rows.  The
- * input goes through LDS in chunks that all waves read, the next chunk on its way (through registers) during the
- * products of the present one; each wave's weights come straight from memory, a chunk ahead as well. */
+ * input goes through LDS in chunks that all waves read; each wave's weights come straight from memory, as nobody else
+ * needs them.
+ *
+ * Measured: 64 x 4096 -> 131072 bf16, groups of 128, fp32 output: 100 us, 3.2 TB/s and 690 TFLOP/s; its bytes alone
+ * would take 64 us and its products 66.  A SIMD has two waves, and an instruction count of 40 us of vector and 27 us
+ * of matrix instructions, which overlap in part.  Four row tiles a wave or three workgroups a CU gave nothing
+ * (registers), one chunk on its way instead of two 117 us. */
 #define Q4_STAGED_WAVES 4
 template <int T, int R, int PIECES, int PER, bool XG>
 __global__ __launch_bounds__(Q4_STAGED_WAVES * 64, 2) void q4_staged_kernel(q4_args a)
@@ -787,12 +809,18 @@ __global__ __launch_bounds__(Q4_STAGED_WAVES * 64, 2) void q4_staged_kernel(q4_a
     }
 }
 
-/* Which form a product takes.
- *   direct  at most 16 rows that are short enough for every workgroup to scale them while its first weights arrive: a
- *           second launch and the way of the input through memory cost more.  Longer ones (25088 values in two rows)
- *           are better scaled once.
- *   staged  so many outputs that workgroups of 64 (R = 1) or 128 (R = 2) of them fill the chip
- *   stream  the others */
+/* Which form a product takes (times of both sides, groups of 128):
+ *   direct  at most 4 rows (the matrix instruction's rows and columns are laid out for that) which fit into LDS: one row
+ *           25088 -> 4096 fp32 17.5 us, by the second pass below 31; four rows 4096 -> 4096 bf16 6.4 us against 8.7.
+ *           The border is near: four rows of 18000 20.5 against 19.7.
+ *   staged  so many tiles that workgroups of 4 or 8 of them fill the chip: its time hardly depends on their number
+ *           up to there, while stream's grows with it.  64 x 4096 -> 11200 bf16 24.2 against 28.6 us, 8192 outputs
+ *           (2048 tiles) 20.4 by stream; 32 x 4096 -> 22400 21.8 against 28.3; fp32 input 36.6 against 41.5
+ *   stream  the others
+ * Blocks (H): 12544 -> 1715 (108 tiles) 7.9 us by two, 9.7 by one; 160 tiles 11.0 by two, 10.0 by one; 63 tiles of
+ * 8192 5.4 by four, 5.5 by two, 7.0 by one.
+ * Row tiles (R): staged 64 x 4096 -> 131072 100 us by two, 113 by one, no difference at 49152; stream 16 x 8192 -> 8192
+ * 15.0 and 15.4. */
 struct q4_plan {
     enum { DIRECT, STREAM, STAGED } form;
     int ksplit, h, t, r;

@@ -490,7 +490,9 @@ __device__ __forceinline__ void load8(const typename dn_elt<T>::store *x, int i,
     }
 }
 
-/* ---- a row of up to 8192 tokens: one workgroup, the row in registers ---------------------------------- */
+/* ---- a row of up to 8192 tokens: one workgroup, the row in LDS, one launch --------------------------------
+ * Bound by the latency of its steps (largest, bins, border, candidates, kept mass, token), each behind a barrier: 1000
+ * tokens 10 us, 8000 16 us, 256 rows of 8000 19 us. */
 template <int T, int E, int THREADS>
 __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
 {
@@ -585,7 +587,13 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
  * 1 largest of each segment (and the row's bins cleared)
  * 2 bins of the row, rows with top-k or top-p only: each segment's in LDS, then added to the row's
  * 3 borders from the bins; the kept mass of each block of tokens and each segment's candidates
- * 4 one workgroup a row: the prefix' end among the candidates, the block that the draw falls into, the token */
+ * 4 one workgroup a row: the prefix' end among the candidates, the block that the draw falls into, the token
+ *
+ * Measured: one row of 32768 fp32, top-k and top-p, 22 us (2, 4, 5 and 7 in the four); 64 rows of 131072 with settings of
+ * all kinds 51 us (6, 15, 17, 10), with top-k alone 36.  A pass over the logits is 6 us at the memory's
+ * rate; the second and third are bound by their instructions: a weight is 22 of 64 bits, the additions to 64-bit bins
+ * wait for each other, and a token of a bin that is kept is weighed twice rather than 8 bytes stored for each.  The
+ * fourth is a chain of latencies. */
 #define SM_SPLIT_THREADS 256
 #define SM_STRIP (SM_SPLIT_THREADS * 8) /* tokens that a workgroup takes at a time */
 #define SM_DRAW_THREADS 512
