@@ -243,7 +243,9 @@ __device__ __forceinline__ void find_border(sample_lds &s, const sample_row &r)
             u64 before;
             bin = counts.find(0, (u64)r.k, before);
             need = r.k - (int)before;
-            if (bin >= SM_BINS - 1) bin = -1; /* all that weighs anything is among the first k */
+            /* all that weighs anything is among the first k: what is in the last bin lies 31 T or more below the largest
+             * (but for a T next to which the difference of two logits is infinite) */
+            if (bin == SM_BINS || (bin == SM_BINS - 1 && r.bins_per_logit > 1e-30f)) bin = -1;
         }
         if (lane == 0) {
             s.border.k_bin = bin;
@@ -390,7 +392,8 @@ __device__ __forceinline__ u64 last_place(Each each, const sample_places<T> &pla
         const u64 target = by_mass ? share_of(r.p, mass_k) : (u64)b.k_need;
         u64 base = by_mass ? b.mass_lo : 0;
         /* logits of bins from .. to, a hundredth of a bin more on either side than the rounding of bin_of needs */
-        const float upper = fminf(largest, largest - (from - 0.01f) / r.bins_per_logit);
+        const float up = largest - (from - 0.01f) / r.bins_per_logit;
+        const float upper = up >= -3.402823466e38f && up < largest ? up : largest; /* (bins may be infinitely wide) */
         const float lower = to < SM_BINS - 1 ? largest - (to + 1.01f) / r.bins_per_logit : -INFINITY;
         const u64 most = places.of(upper, 0), least = places.of(lower, (1 << places.bits) - 1);
         int bit = most > least ? 64 - __clzll((long long)(most ^ least)) : 0, turn = 0;

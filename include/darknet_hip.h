@@ -446,7 +446,8 @@ void forward_crop_gpu(const float *input, float *output, int batch, int c, int h
  * (scales, biases, settings of the sampling) are fp32 or int as written.  All buffers lie on the current
  * device.  These calls allocate nothing and keep nothing from one call for the next: a call under
  * stream capture is recorded like any other, and calls that overlap (two streams, two captured graphs) only need
- * workspaces and outputs of their own.  The workspace needs no initial contents and is aligned to 16 bytes.
+ * workspaces and outputs of their own.  The workspace needs no initial contents and is aligned to 16 bytes.  Where
+ * nothing else is said a buffer that is written overlaps no other.
  * They return 0, or -1 after a message on stderr when the arguments cannot be honoured: then nothing has
  * been launched.  No rows (rows or batch 0) is a call that does nothing, with buffers or without.
  * ---------------------------------------------------------------------------------------- */

@@ -55,6 +55,61 @@ def test_sample_many_tokens_kept(dn, n):
     check_draw(dn, flat, BF16, r.random(4), top_p=np.full(4, 0.9), min_p=np.full(4, 0.95))
 
 
+@pytest.mark.parametrize("n", [6, 900, 30000])
+def test_sample_logits_at_the_ends_of_the_range(dn, n):
+    """Differences of two logits that leave 32 bits, under temperatures next to which they are small."""
+    r = np.random.default_rng(n)
+    x = (r.random((6, n)) * 3e38).astype(np.float32)
+    x[:, ::2] *= -1
+    x[:, 5] = -3e38
+    t = np.float32([1e38, np.inf, 3e37, 1e36, 1.0, 2e38])
+    u = np.linspace(0.02, 0.98, 6)
+    check_draw(dn, x, F32, u, t)
+    for k in (1, 2, n // 2, n - 1):
+        check_draw(dn, x, F32, u, t, top_k=np.full(6, k))
+        check_draw(dn, x, F32, u, t, top_k=np.full(6, k), top_p=np.full(6, 0.7), min_p=np.full(6, 0.01))
+    check_draw(dn, x, F32, u, t, top_p=np.full(6, 0.9))
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+@pytest.mark.parametrize("n", [300, 20000])
+def test_norm_scales_that_are_not_finite(dn, t, n):
+    """NaN and infinite scales: their outputs, and the 8-bit groups that hold them."""
+    c = Norm(n, 2, n, t, group=128)
+    c.g[5], c.g[200] = np.nan, np.inf
+    s, o, q, scales = c.run(dn)
+    with np.errstate(invalid="ignore"):
+        _, y = R.rmsnorm(c.x, c.add, c.g, 1e-5, t)
+        codes, want = R.q8(y, 128)
+    assert np.array_equal(scales, want, equal_nan=True) and np.array_equal(q, codes)
+    got = R.from_type(o, t)
+    assert np.isnan(got[:, 5]).all() and np.isinf(got[:, 200]).all()
+    rest = np.isfinite(y)
+    assert (np.abs(got - y)[rest] <= (np.abs(y) * (R.HALF_STEP[t] + 4 * 2.0 ** -24) + R.HALF_TINY[t])[rest]).all()
+
+
+@pytest.mark.parametrize("batch", [2, 20])
+def test_q4_activations(dn, batch):
+    """Every activation on what the product gives with none, by every way of storing: fp32 results differ from the
+    formula's in 64 bits by the sum's own error (no slope here is above 1.8) and one rounding."""
+    forms = {0: lambda v: 1 / (1 + np.exp(-v)), 1: lambda v: np.maximum(v, 0), 2: lambda v: np.where(v > 0, v, .01 * v), 3: lambda v: v,
+             4: lambda v: np.maximum(v, 0) + .1 * v, 5: np.tanh, 7: lambda v: np.where(v > 0, v, .1 * v),
+             8: lambda v: np.where(v >= 0, v, np.exp(np.minimum(v, 0)) - 1), 9: lambda v: 2 / (1 + np.exp(-v)) - 1, 11: lambda v: np.clip(v, -1, 1),
+             13: lambda v: np.where(v >= 0, 1.0507 * v, 1.0507 * 1.6732 * (np.exp(np.minimum(v, 0)) - 1))}
+    k = 256
+    for n in (50, 24000):
+        m = Q4(dn, n, k, n, 128)
+        x = (np.random.default_rng(n).standard_normal((batch, k)) * 0.1).astype(np.float32)
+        bx, out = Buffer(x), Buffer(shape=(batch, n), dtype=np.float32)
+        ws = m.workspace(dn, F32, batch)
+        v = x.astype(np.float64) @ m.w.T
+        tol = R.q4_bound(x.astype(np.float64), m.w, 128, F32, v)
+        for act, form in forms.items():
+            assert m.call(dn, bx, F32, None, 0, None, out, F32, batch, act, ws) == 0
+            dn.hip_synchronize()
+            assert (np.abs(out.get() - form(v)) <= 1.8 * tol + 2.0 ** -23 * np.abs(form(v))).all(), act
+
+
 def push(dn, ptr, a):
     dn.hip_push_array(ptr, np.ascontiguousarray(a, np.float32).ctypes.data_as(C.POINTER(C.c_float)), a.size)
 
