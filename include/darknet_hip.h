@@ -475,7 +475,7 @@ int forward_rmsnorm_gpu(const void *input, const void *add, const float *scales,
  *   q4_pack_codes_gpu     from weights that are 4-bit already: codes [outputs][(inputs + 1) / 2], the lower
  *                         half of a byte is the even input; scales [outputs][groups]; zeros the same in
  *                         bytes (0 .. 15), or NULL for 8 everywhere
- *   q4_pack_weights_gpu   from [outputs][inputs] floats: each group's range, widened to hold zero, in 15 steps
+ *   q4_pack_weights_gpu   from [outputs][inputs] finite floats: each group's range, widened to hold zero, in 15 steps
  *   q4_unpack_weights_gpu the values the packed copy stands for, [outputs][inputs] floats
  * packed is aligned to 16 bytes.  input [batch][inputs] is fp32, fp16, bf16, or 8 bits with input_scales
  * [batch][groups of input_group] (input_group: 0 = one scale a row, or `group`), as forward_rmsnorm_gpu
