@@ -211,6 +211,7 @@ struct q4_args {
     int batch, x_group; /* x_group: 0, or the inputs that share one of input_scales */
     int activation;
     int ksplit; /* direct form: waves of a workgroup that share a row tile, each taking a part of the inputs */
+    int run;    /* stream form: blocks of the inputs that a workgroup has */
     q4_shape s;
 };
 
@@ -536,7 +537,7 @@ __global__ __launch_bounds__(Q4_THREADS, 4) void q4_direct_kernel(q4_args a)
  * 8-bit input with groups, [group in 128][16] factors.  Behind the blocks a factor for each row.  A pass over a few
  * kilobytes, 3 to 5 us with its launch; it saves every workgroup of the second pass a scaling of its own (16 rows
  * of 8192 values read as they are by that pass, without this one: the same time in groups of 128, 27 us against 20 in
- * groups of 32). */
+ * groups of 32).  1024 threads for long rows: 8 rows of 20787 in all 17.8 us, 21 with 256. */
 __host__ __device__ static inline int q4_block_bytes(const q4_shape &s, int pieces, bool groups)
 {
     return pieces * 4096 + (groups ? 128 / s.group * 64 : 0);
@@ -547,11 +548,11 @@ __host__ __device__ static inline size_t q4_rows_at(const q4_shape &s, int piece
     return ((size_t)batch + 15) / 16 * s.kblocks * q4_block_bytes(s, pieces, groups);
 }
 
-template <int TI, bool XG>
-__global__ __launch_bounds__(256) void q4_prepare_kernel(q4_args a)
+template <int TI, bool XG, int THREADS>
+__global__ __launch_bounds__(THREADS) void q4_prepare_kernel(q4_args a)
 {
     constexpr int PIECES = TI == DN_F32 ? 2 : 1;
-    __shared__ unsigned s_largest[4];
+    __shared__ unsigned s_largest[THREADS / 64];
     const int tid = threadIdx.x, b = blockIdx.x, block = q4_block_bytes(a.s, PIECES, XG);
     const size_t row_bytes = (size_t)a.s.inputs * (TI == DN_F32 ? 4 : TI == DN_I8 ? 1 : 2);
     const char *row = (const char *)a.input + b * row_bytes;
@@ -559,7 +560,7 @@ __global__ __launch_bounds__(256) void q4_prepare_kernel(q4_args a)
     if (TI != DN_I8) {
         unsigned m = 0;
 #pragma unroll 4
-        for (int k = tid * 8; k < a.s.inputs; k += 2048) {
+        for (int k = tid * 8; k < a.s.inputs; k += THREADS * 8) {
             float x[8];
             q4_load8<TI>(row, k, a.s.inputs, x);
             m = q4_largest8(m, x);
@@ -567,12 +568,14 @@ __global__ __launch_bounds__(256) void q4_prepare_kernel(q4_args a)
         m = dn_wave_max(m);
         if ((tid & 63) == 0) s_largest[tid >> 6] = m;
         __syncthreads();
-        scale = q4_scaling(max(max(s_largest[0], s_largest[1]), max(s_largest[2], s_largest[3])), factor);
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; ++w) m = max(m, s_largest[w]);
+        scale = q4_scaling(m, factor);
     }
     if (tid == 0)
         ((float *)(a.workspace + q4_rows_at(a.s, PIECES, a.batch, XG)))[b] = TI == DN_I8 ? (XG ? 1.f : a.input_scales[b]) : factor;
     unsigned char *out = a.workspace + (size_t)(b >> 4) * a.s.kblocks * block + (b & 15) * 16;
-    for (int k = tid * 8; k < a.s.kblocks * 128; k += 2048) {
+    for (int k = tid * 8; k < a.s.kblocks * 128; k += THREADS * 8) {
         float x[8];
         half8_t hi, lo;
         q4_load8<TI>(row, k, a.s.inputs, x);
@@ -584,7 +587,7 @@ __global__ __launch_bounds__(256) void q4_prepare_kernel(q4_args a)
     if (XG) {
         const int x_groups = (a.s.inputs + a.x_group - 1) / a.x_group, per = 128 / a.s.group;
         unsigned char *to = a.workspace + (size_t)(b >> 4) * a.s.kblocks * block + PIECES * 4096 + (b & 15) * 4;
-        for (int g = tid; g < a.s.groups; g += 256)
+        for (int g = tid; g < a.s.groups; g += THREADS)
             *(float *)(to + (size_t)(g / per) * block + g % per * 64) = g < x_groups ? a.input_scales[(long)b * x_groups + g] : 0.f;
     }
 }
@@ -603,11 +606,42 @@ __device__ __forceinline__ void q4_store_tile(const q4_args &a, const float *row
     }
 }
 
+/* The same as one of several parts of the sums, which the next pass joins. */
+__host__ __device__ static inline size_t q4_parts_at(const q4_shape &s, int pieces, int batch, bool groups)
+{
+    return (q4_rows_at(s, pieces, batch, groups) + (size_t)batch * 4 + 15) / 16 * 16;
+}
+
+__device__ __forceinline__ void q4_store_part(const q4_args &a, size_t parts_at, int tile, int b0, float4_t v)
+{
+    const int lane = threadIdx.x & 63, o = tile * 16 + (lane & 15);
+    if (o >= a.s.outputs) return;
+    float *parts = (float *)(a.workspace + parts_at) + (size_t)blockIdx.z * a.batch * a.s.outputs;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int b = b0 + (lane >> 4) * 4 + i;
+        if (b < a.batch) parts[(size_t)b * a.s.outputs + o] = v[i];
+    }
+}
+
+/* Third pass, where the inputs were cut: the parts' sums of an output, in their order. */
+__global__ __launch_bounds__(256) void q4_join_kernel(q4_args a, size_t rows_at, size_t parts_at, int parts)
+{
+    const int o = blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
+    if (o >= a.s.outputs) return;
+    const float *part = (const float *)(a.workspace + parts_at) + (size_t)b * a.s.outputs + o;
+    const float bias = q4_bias(a, o), factor = ((const float *)(a.workspace + rows_at))[b];
+    float y = 0;
+#pragma unroll 4
+    for (int p = 0; p < parts; ++p) y += part[(size_t)p * a.batch * a.s.outputs];
+    q4_store(a, b, o, y * factor, bias);
+}
+
 /* ---- second pass, few outputs: a workgroup takes R row tiles and a tile of input rows, its eight waves an eighth of
  * the inputs each.  No two waves read the same input, so that it comes straight into registers like the weights, both
  * a block ahead, and nothing waits for another wave before the end.
  *
- * Measured: 16 rows of 8-bit input, 8192 -> 8192 in groups of 128, 14.7 us for both passes, 11 for this one (3.3 TB/s);
+ * Measured: 16 rows of 8-bit input, 8192 -> 8192 in groups of 128, 14.1 us for both passes, 11 for this one (3.3 TB/s);
  * 16 x 4096 -> 32768 bf16 21.5 us (3.4 TB/s).  Two tiles of input rows in a workgroup took longer (64 x 4096 -> 8192:
  * 23.7 against 20.4 us: fewer waves have the registers). */
 template <int R, int PIECES, int PER, bool XG>
@@ -616,14 +650,14 @@ __global__ __launch_bounds__(Q4_THREADS) void q4_stream_kernel(q4_args a)
     __shared__ float4_t s_red[Q4_WAVES][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int block = q4_block_bytes(a.s, PIECES, XG), x_tile = blockIdx.y, tile0 = blockIdx.x * R;
-    const int mine = (a.s.kblocks - wave + Q4_WAVES - 1) / Q4_WAVES;
+    const int kb0 = blockIdx.z * a.run, mine = (min(a.run, a.s.kblocks - kb0) - wave + Q4_WAVES - 1) / Q4_WAVES;
     struct block_data {
         q4_tile<PER> w[R];
         half8_t x[PIECES][4];
         float4_t f[PER];
     };
     auto fetch = [&](int n, block_data &d) {
-        const int kb = wave + n * Q4_WAVES;
+        const int kb = kb0 + wave + n * Q4_WAVES;
 #pragma unroll
         for (int r = 0; r < R; ++r) d.w[r] = q4_load_tile<PER>(a, min(tile0 + r, a.s.tiles - 1), kb, lane);
         const unsigned char *p = a.workspace + ((size_t)x_tile * a.s.kblocks + kb) * block;
@@ -660,7 +694,8 @@ __global__ __launch_bounds__(Q4_THREADS) void q4_stream_kernel(q4_args a)
             float4_t v = s_red[0][lane];
 #pragma unroll
             for (int q = 1; q < Q4_WAVES; ++q) v += s_red[q][lane];
-            q4_store_tile(a, row_factors, tile0 + k, x_tile * 16, v);
+            if (gridDim.z > 1) q4_store_part(a, q4_parts_at(a.s, PIECES, a.batch, XG), tile0 + k, x_tile * 16, v);
+            else q4_store_tile(a, row_factors, tile0 + k, x_tile * 16, v);
         }
     }
 }
@@ -823,8 +858,8 @@ __global__ __launch_bounds__(Q4_STAGED_WAVES * 64, 2) void q4_staged_kernel(q4_a
  * 15.0 and 15.4. */
 struct q4_plan {
     enum { DIRECT, STREAM, STAGED } form;
-    int ksplit, h, t, r;
-    unsigned gx, gy;
+    int ksplit, h, t, r, run;
+    unsigned gx, gy, gz;
     size_t lds;
 };
 
@@ -833,7 +868,8 @@ static q4_plan q4_plan_of(const q4_shape &s, int type, int batch)
     q4_plan p;
     const int pieces = type == DN_F32 ? 2 : 1, x_tiles = (int)(((long)batch + 15) / 16);
     p.ksplit = p.h = p.t = p.r = 1;
-    p.gy = 1;
+    p.gy = p.gz = 1;
+    p.run = s.kblocks;
     while (p.h < 4 && (long)s.tiles * p.h <= 128 && s.kblocks > p.h) p.h *= 2;
     const int steps = (s.kblocks + p.h - 1) / p.h;
     p.lds = batch * ((size_t)steps * p.h * (p.h > 1 ? 272 : 256) * pieces + 16) + (size_t)steps * p.h * (type == DN_I8 ? 128 / s.group : 1) * 16;
@@ -858,6 +894,15 @@ static q4_plan q4_plan_of(const q4_shape &s, int type, int batch)
         p.gx = (unsigned)((s.tiles + p.r - 1) / p.r);
     }
     p.gy = (unsigned)((x_tiles + p.t - 1) / p.t);
+    /* Far fewer workgroups than CUs, and long rows: the inputs are cut over workgroups.  The third launch costs some 3 us:
+     * 8 x 20787 -> 512 bf16 17.8 us uncut, 12.8 cut; 5 x 22144 -> 1778 19.2 and 16.4; 16 x 8192 -> 1000 10.4 and 10.0;
+     * below that nothing. */
+    if (p.form == q4_plan::STREAM && s.kblocks >= 64) {
+        while ((long)p.gx * p.gy * p.gz * 2 <= 256 && p.run >= 32) {
+            p.run = (p.run + 1) / 2;
+            p.gz = (unsigned)((s.kblocks + p.run - 1) / p.run);
+        }
+    }
     return p;
 }
 
@@ -865,18 +910,25 @@ extern "C" size_t connected_q4_workspace_bytes(int input_type, int batch, int in
 {
     if (!q4_shape_ok(inputs, outputs, group) || batch < 1) return 0;
     const q4_shape s = q4_shape_of(inputs, outputs, group);
-    if (q4_plan_of(s, input_type, batch).form == q4_plan::DIRECT) return 0;
-    return q4_rows_at(s, input_type == DN_F32 ? 2 : 1, batch, input_type == DN_I8) + (size_t)batch * 4;
+    const q4_plan p = q4_plan_of(s, input_type, batch);
+    if (p.form == q4_plan::DIRECT) return 0;
+    const int pieces = input_type == DN_F32 ? 2 : 1;
+    if (p.gz > 1) return q4_parts_at(s, pieces, batch, input_type == DN_I8) + (size_t)p.gz * batch * outputs * 4;
+    return q4_rows_at(s, pieces, batch, input_type == DN_I8) + (size_t)batch * 4;
 }
 
 template <int T, int R, int PIECES, int PER, bool XG>
 static void q4_launch_second(const q4_args &a, const q4_plan &p)
 {
-    const dim3 grid(p.gx, p.gy);
+    const dim3 grid(p.gx, p.gy, p.gz);
     if (p.form == q4_plan::STAGED)
         hipLaunchKernelGGL((q4_staged_kernel<T, R, PIECES, PER, XG>), grid, dim3(Q4_STAGED_WAVES * 64), 0, dn_stream(), a);
-    else if constexpr (T == 1)
+    else if constexpr (T == 1) {
         hipLaunchKernelGGL((q4_stream_kernel<R, PIECES, PER, XG>), grid, dim3(Q4_THREADS), 0, dn_stream(), a);
+        if (p.gz > 1)
+            hipLaunchKernelGGL(q4_join_kernel, dim3((unsigned)((a.s.outputs + 255) / 256), (unsigned)a.batch), dim3(256), 0, dn_stream(), a,
+                               q4_rows_at(a.s, PIECES, a.batch, XG), q4_parts_at(a.s, PIECES, a.batch, XG), (int)p.gz);
+    }
 }
 
 template <int TI, int PER, bool XG>
@@ -890,7 +942,8 @@ static void q4_launch(const q4_args &a, const q4_plan &p)
         else hipLaunchKernelGGL((q4_direct_kernel<TI, PER, XG, 4>), grid, block, p.lds, dn_stream(), a);
         return;
     }
-    hipLaunchKernelGGL((q4_prepare_kernel<TI, XG>), dim3((unsigned)a.batch), dim3(256), 0, dn_stream(), a);
+    if (a.s.inputs > 4096) hipLaunchKernelGGL((q4_prepare_kernel<TI, XG, 1024>), dim3((unsigned)a.batch), dim3(1024), 0, dn_stream(), a);
+    else hipLaunchKernelGGL((q4_prepare_kernel<TI, XG, 256>), dim3((unsigned)a.batch), dim3(256), 0, dn_stream(), a);
     if constexpr (PER < 4) /* four groups in a block fill the registers with R = 1 */
         if (p.r == 2) {
             if (p.t == 1) q4_launch_second<1, 2, PIECES, PER, XG>(a, p);
@@ -937,7 +990,7 @@ extern "C" int forward_connected_q4_gpu(const void *input, int input_type, const
     if (p.gx > 0x7fffffu || p.gy > 65535u) return dn_refuse(me, "too many outputs or rows for one call");
     hip_require_device(me);
     const q4_args a = {input, input_scales, (const unsigned char *)packed, biases, output, (unsigned char *)workspace,
-                       output_type, batch, xg ? input_group : 0, activation, p.ksplit, s};
+                       output_type, batch, xg ? input_group : 0, activation, p.ksplit, p.run, s};
     if (input_type == DN_F32) q4_launch_group<DN_F32, false>(a, p);
     else if (input_type == DN_F16) q4_launch_group<DN_F16, false>(a, p);
     else if (input_type == DN_BF16) q4_launch_group<DN_BF16, false>(a, p);

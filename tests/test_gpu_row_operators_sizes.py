@@ -35,6 +35,13 @@ def test_q4_long_rows(dn, kind, batch, k):
     Q4(dn, k + batch, k, 37, group).check(dn, k, batch, tx, F32, xg=xg)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("batch,k,n", [(5, 8064, 33), (5, 8065, 33), (16, 8192, 33), (17, 9001, 130), (33, 20787, 50), (5, 12545, 1700), (8, 16500, 2100)])
+def test_q4_inputs_cut_over_workgroups(dn, kind, batch, k, n):
+    tx, group, xg = kind
+    Q4(dn, k + n, k, n, group).check(dn, k, batch, tx, BF16 if batch == 17 else F32, xg=xg, act=7)
+
+
 def test_norm_rows_at_the_ends_of_the_range(dn):
     """Without eps the factor of a row leaves the range of 32 bits where the row is near its ends."""
     for size in (1e-42, 1e-39, 1e-36, 1e-30, 1e30, 3e37):
