@@ -271,7 +271,8 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_kernel(norm_args a)
 /* Which form a row takes: one run a lane up to 256 lanes, then two, so that several rows share a CU and their loads
  * and stores overlap (2048 fp32 to 8 bits: 47 us by 256 lanes, 55 by 512; 8192 bf16: 66 by 512, 69 by 1024, 90 by 256 with
  * four), but for 16-bit rows of 257 to 512 runs of eight, whose two runs take the registers of a row more (4096 bf16: 27.7
- * by 512, 29.7 by 256).  A row of more than 16384 values is read again for each step. */
+ * by 512, 29.7 by 256).  768 lanes for what leaves a third of 1024 idle (3795 x 6000 fp32 71 us, 79 by 1024; 384 below 512
+ * gave nothing).  A row of more than 16384 values is read again for each step. */
 template <int T, bool Q8>
 static void norm_launch(const norm_args &a)
 {
@@ -286,6 +287,7 @@ static void norm_launch(const norm_args &a)
     else if (V == 8 && runs <= 512) NM_LAUNCH(512, 1);
     else if (runs <= 512) NM_LAUNCH(256, 2);
     else if (runs <= 1024) NM_LAUNCH(512, 2);
+    else if (runs <= 1536) NM_LAUNCH(768, 2);
     else if (runs <= 2048) NM_LAUNCH(1024, 2);
     else if (V == 4 && runs <= 4096) NM_LAUNCH(1024, 16 / V);
     else NM_LAUNCH(1024, 0);

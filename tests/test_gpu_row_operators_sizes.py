@@ -42,6 +42,15 @@ def test_q4_inputs_cut_over_workgroups(dn, kind, batch, k, n):
     Q4(dn, k + n, k, n, group).check(dn, k, batch, tx, BF16 if batch == 17 else F32, xg=xg, act=7)
 
 
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("runs", [64, 128, 256, 512, 1024, 1536, 2048, 4096])
+def test_norm_widths_where_the_form_changes(dn, t, runs):
+    v = 4 if t == F32 else 8
+    for n in (runs * v, runs * v + 1):
+        Norm(n, 3, n, t, group=128).check(dn)
+        Norm(n + 1, 2, n, t, add=False, group=0).check(dn)
+
+
 def test_norm_rows_at_the_ends_of_the_range(dn):
     """Without eps the factor of a row leaves the range of 32 bits where the row is near its ends."""
     for size in (1e-42, 1e-39, 1e-36, 1e-30, 1e30, 3e37):
