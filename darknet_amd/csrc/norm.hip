@@ -118,8 +118,8 @@ __device__ __forceinline__ void store_run(E *p, int i, int n, const float *v)
  * The 8-bit form works on p = s * scales, exact in 64 bits: max|y| = max|p| * r, and code = rint(p * (r / c)).
  *
  * Bound by memory: 16384 x 4096 fp32 with residual, sum and output (1.07 GB) 187 us, 5.7 TB/s, where a copy reaches
- * 5.1; 4096 x 8192 bf16 likewise 60 us, 4.5 TB/s.  With 8-bit output in groups of 128 (236 MB) 66 us, 3.6 TB/s: half
- * the time is in its 600 vector instructions for 16 values a lane.  One row of 4096: 3 us, a launch. */
+ * 5.1; 4096 x 8192 bf16 likewise 60 us, 4.5 TB/s.  With 8-bit output in groups of 128 (236 MB) 54 us, 4.3 TB/s,
+ * beside 600 vector instructions for 16 values a lane.  One row of 4096: 3 us, a launch. */
 template <int T, int THREADS, int RUNS, int V, bool Q8>
 __global__ __launch_bounds__(THREADS) void rmsnorm_kernel(norm_args a)
 {
@@ -129,7 +129,11 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_kernel(norm_args a)
     for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const E *in = (const E *)a.input + row * n, *add = a.add ? (const E *)a.add + row * n : 0;
         E *sum = a.sum ? (E *)a.sum + row * n : 0;
-        auto at = [&](int j) { return (j * THREADS + tid) * V; };
+        /* Behind the empty statement the compiler knows nothing of where a run lies, and does not prepare the loads and
+         * stores of all runs beforehand: 58 registers instead of 95 with 8-bit output, and a third more waves. */
+        int first = tid * V;
+        asm("" : "+v"(first));
+        auto at = [&](int j) { return j * THREADS * V + first; };
         auto added = [&](float s[V], const float t[V]) {
 #pragma unroll
             for (int e = 0; e < V; ++e) s[e] = (float)(E)(s[e] + t[e]);
@@ -269,7 +273,7 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_kernel(norm_args a)
 }
 
 /* Which form a row takes: one run a lane up to 256 lanes, then two, so that several rows share a CU and their loads
- * and stores overlap (2048 fp32 to 8 bits: 47 us by 256 lanes, 55 by 512; 8192 bf16: 66 by 512, 69 by 1024, 90 by 256 with
+ * and stores overlap (2048 fp32 to 8 bits: 47 us by 256 lanes, 55 by 512; 8192 bf16: 60 by 512, 62 by 1024, 80 by 256 with
  * four), but for 16-bit rows of 257 to 512 runs of eight, whose two runs take the registers of a row more (4096 bf16: 27.7
  * by 512, 29.7 by 256).  768 lanes for what leaves a third of 1024 idle (3795 x 6000 fp32 71 us, 79 by 1024; 384 below 512
  * gave nothing).  A row of more than 16384 values is read again for each step. */
