@@ -179,12 +179,15 @@ extern "C" int q4_unpack_weights_gpu(const void *packed, float *weights, int inp
 }
 
 /* ---- the product --------------------------------------------------------------------------------------
- * On the fp16 matrix instruction: code - zero is a whole number of at most 15, exact in fp16.  The input is
- * scaled by a power of two that brings its largest value to 2^14 .. 2^15 and held as one fp16 value (8-bit, fp16
- * and bf16 input: exact, short of values 2^-29 below the largest) or as the sum of two (fp32 input: to
- * 2^-23 of each value).  Products are exact in the fp32 accumulators, which a group starts from zero; its sum
- * is then multiplied with the scale and added to the output's.  Where a value is not finite the factor that
- * undoes the scaling is NaN.
+ * On the fp16 matrix instruction: code - zero is a whole number of at most 15, exact in fp16.  8-bit and fp16 input is
+ * exact there.  fp32 and bf16 input is scaled by a power of two that brings the largest value (of the row, or of 128
+ * inputs) to 2^14 .. 2^15, and held as one fp16 value (bf16: exact from 2^-31 of the largest up) or as two, of which the
+ * second is the 2^12-fold of what the first leaves (fp32: to 2^-23 of each value from 2^-28 of the largest up; the weights
+ * that the second meets are 2^-12 times the others).  Values further below are left out there; each eight inputs that
+ * have some are marked, and their products are added to the output at the end, one by one: an ordinary row has hardly any,
+ * but an output whose weights avoid the large inputs would miss them.  Products are exact in the fp32 accumulators, which
+ * a group starts from zero; its sum is then multiplied with the scale and added to the output's.  Where a value is not
+ * finite the factor that undoes the scaling is NaN.
  *
  * The input is the instruction's first operand and the weights the second, so that a lane's results are those
  * of one output, whose scale and zero it has read beside the codes.
@@ -208,6 +211,7 @@ struct q4_args {
     void *output;
     unsigned char *workspace;
     int output_type;
+    bool ranged;        /* input whose values may be too far apart for the pieces */
     int batch, x_group; /* x_group: 0, or the inputs that share one of input_scales */
     int activation;
     int ksplit; /* direct form: waves of a workgroup that share a row tile, each taking a part of the inputs */
@@ -215,13 +219,25 @@ struct q4_args {
     q4_shape s;
 };
 
+/* Input types whose values may be too far apart for the pieces, and the least that these take: what is below would be
+ * subnormal in the first piece (fp32; the matrix instruction aligns its addends by their exponents, and takes that of a
+ * subnormal factor as 2^-14), or lose bits (bf16). */
+template <int TI> struct q4_range { static constexpr bool wide = TI == DN_F32 || TI == DN_BF16; };
+template <int TI>
+__device__ __forceinline__ unsigned q4_least_held(float factor) /* as bits of the value itself */
+{
+    return __float_as_uint((TI == DN_F32 ? 0x1p-14f : 0x1p-17f) * factor);
+}
+
 /* The power of two that values are scaled by, from the largest of their absolute values' bits, and the factor that undoes
- * it: a power of two, NaN if a value is not finite. */
+ * it: a power of two, NaN if a value is not finite.  fp16 input is not scaled down: it fits, and would lose its last bit. */
+template <int TI>
 __device__ __forceinline__ float q4_scaling(unsigned largest, float &factor)
 {
     int e = 15;
     if (largest - 1u < 0x7f7fffffu) (void)frexpf(__uint_as_float(largest), &e); /* largest < 2^e */
-    const int shift = min(15 - e, 126);                                        /* 2^-126: the factor is not rounded */
+    int shift = min(15 - e, 126);                                              /* 2^-126: the factor is not rounded */
+    if (TI == DN_F16) shift = max(shift, 0);
     factor = largest < 0x7f800000u ? ldexpf(1.f, -shift) : __uint_as_float(0x7fc00000u);
     return ldexpf(1.f, shift);
 }
@@ -262,15 +278,84 @@ __device__ __forceinline__ unsigned q4_largest8(unsigned m, const float x[8])
     return m;
 }
 
-/* The operand form of eight inputs, scaled by a power of two: hi, and what it leaves of the value in lo. */
-__device__ __forceinline__ void q4_split8(const float x[8], float scale, half8_t &hi, half8_t &lo)
+/* The least of eight absolute values that are not 0, as the maximum of 0 - its bits. */
+__device__ __forceinline__ unsigned q4_least8(unsigned m, const float x[8])
 {
 #pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, 0u - (__float_as_uint(x[i]) & 0x7fffffffu));
+    return m;
+}
+
+/* Whether a value that is not 0 lies below what the pieces hold (never where the factor is NaN). */
+template <int TI>
+__device__ __forceinline__ bool q4_below(unsigned least, float factor)
+{
+    return q4_range<TI>::wide && factor > 0 && least > 0u - q4_least_held<TI>(factor);
+}
+
+/* The operand form of eight inputs, scaled by a power of two: hi, and 2^12 times what it leaves of the value in lo.
+ * Returns the least of the scaled values (below what the pieces hold if one of them is, or is 0). */
+#define Q4_LO 0x1p-12f
+__device__ __forceinline__ float q4_split8(const float x[8], float scale, half8_t &hi, half8_t &lo)
+{
+    float least = 1, v[8];
+#pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float v = x[i] * scale;
-        hi[i] = (_Float16)v;
-        lo[i] = (_Float16)(v - (float)hi[i]);
+        v[i] = x[i] * scale;
+        least = fminf(least, fabsf(v[i]));
+        hi[i] = (_Float16)v[i];
     }
+    /* Behind the empty statements the compiler does not know where a half came from: it converts in pairs then, where it
+     * would else round each value again in a slower mixed instruction (12544 values 0.25 us). */
+    uint4_t w = __builtin_bit_cast(uint4_t, hi);
+    asm("" : "+v"(w));
+    hi = __builtin_bit_cast(half8_t, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float t = fmaf((float)hi[i], -1 / Q4_LO, v[i] * (1 / Q4_LO)); /* exact before it is rounded */
+        asm("" : "+v"(t));
+        lo[i] = (_Float16)t;
+    }
+    return least;
+}
+
+/* Of eight inputs those that the pieces take. */
+template <int TI>
+__device__ __forceinline__ void q4_drop_below(float x[8], float factor)
+{
+    const unsigned least = q4_least_held<TI>(factor);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (__float_as_uint(x[i]) & 0x7fffffffu) < least ? 0.f : x[i];
+}
+
+/* What the pieces leave of row b's sum with output o: the small values of the eights that are marked, 16 bits for each
+ * 128 inputs (eights without such values may be marked too).  mask(kb), factor(kb): of a block.  One thread's work, for the
+ * few rows that need it. */
+template <int TI, class Mask, class Factor>
+__device__ __forceinline__ float q4_left_out(const q4_args &a, int b, int o, Mask mask, Factor factor)
+{
+    typedef typename dn_elt<TI>::store E;
+    const E *row = (const E *)a.input + (long)b * a.s.inputs;
+    float sum = 0;
+#pragma unroll 1
+    for (int kb = 0; kb < a.s.kblocks; ++kb) {
+#pragma unroll 1
+        for (unsigned m = mask(kb); m; m &= m - 1) {
+            const int k = kb * 128 + (__ffs((int)m) - 1) * 8;
+            const unsigned least = q4_least_held<TI>(factor(kb));
+            float x[8];
+            q4_load8<TI>(row, k, a.s.inputs, x);
+            const unsigned codes = ((const unsigned *)a.packed)[q4_dword_at(a.s, o, k)];
+            const long g = q4_group_at(a.s, o, k / a.s.group);
+            const int zero = a.packed[a.s.zeros_at + g];
+            const float scale = ((const float *)(a.packed + a.s.scales_at))[g];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if ((__float_as_uint(x[i]) & 0x7fffffffu) < least)
+                    sum = fmaf(x[i], (float)((int)(codes >> q4_bit_of(i) & 15) - zero) * scale, sum);
+        }
+    }
+    return sum;
 }
 
 /* One tile of 16 outputs x 128 inputs as a lane holds it; PER groups in 128 inputs. */
@@ -352,9 +437,12 @@ __device__ __forceinline__ void q4_multiply(const q4_masks &masks, const q4_tile
 #pragma unroll
         for (int i = 0; i < 4 / PER; ++i) {
             const int step = g * (4 / PER) + i;
-            half8_t wv[R];
+            half8_t wv[R], wl[R];
 #pragma unroll
-            for (int r = 0; r < R; ++r) wv[r] = q4_unpack8(w[r].code[step], z1024[r], z64[r], masks);
+            for (int r = 0; r < R; ++r) {
+                wv[r] = q4_unpack8(w[r].code[step], z1024[r], z64[r], masks);
+                if (PIECES == 2) wl[r] = wv[r] * (_Float16)Q4_LO; /* exact: 15 * 2^-12 at most, 2^-12 at least */
+            }
 #pragma unroll
             for (int t = 0; t < T; ++t)
 #pragma unroll
@@ -363,7 +451,7 @@ __device__ __forceinline__ void q4_multiply(const q4_masks &masks, const q4_tile
 #pragma unroll
                     for (int r = 0; r < R; ++r)
                         acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            x, wv[r], i || p ? acc[r][t] : (float4_t){0, 0, 0, 0}, 0, 0, 0);
+                            x, p ? wl[r] : wv[r], i || p ? acc[r][t] : (float4_t){0, 0, 0, 0}, 0, 0, 0);
                 }
         }
 #pragma unroll
@@ -412,6 +500,7 @@ __global__ __launch_bounds__(Q4_THREADS, 4) void q4_direct_kernel(q4_args a)
     constexpr int AHEAD = 4, MOVES = 2;
     extern __shared__ char lds[];
     __shared__ float s_red[WAVES][4][WIDTH];
+    __shared__ unsigned s_below[WAVES]; /* whether a wave has met values below what the pieces hold */
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kblocks = a.s.kblocks, steps = (kblocks + H - 1) / H, kpad = steps * H * 128;
     const int plane = kpad / 128 * BLOCK, pitch = plane * PIECES + 16; /* bytes of a row's halves, and of a row */
@@ -432,9 +521,11 @@ __global__ __launch_bounds__(Q4_THREADS, 4) void q4_direct_kernel(q4_args a)
     for (int u = 0; u < AHEAD; ++u)
         if (u < mine) w[u] = fetch(unit0 + own_unit, u);
 
-    /* the input: [row][pitch] halves, and [block (8-bit input with groups: group)][4 rows] factors behind them */
+    /* the input: [row][pitch] halves, and [block (8-bit input with groups: group)][4 rows] factors behind them, negative
+     * (fp32 and bf16 input) where values lie below what the pieces hold */
     const size_t row_bytes = (size_t)a.s.inputs * (TI == DN_F32 ? 4 : TI == DN_I8 ? 1 : 2);
     float *factors = (float *)(lds + a.batch * pitch);
+    if (q4_range<TI>::wide && lane == 0) s_below[wave] = 0;
     const int eights = kpad / 8;
     for (int b = 0, q = tid; b < a.batch;) {
         float x[MOVES][8];
@@ -462,10 +553,17 @@ __global__ __launch_bounds__(Q4_THREADS, 4) void q4_direct_kernel(q4_args a)
                 m8 = max(m8, dn_move<0x4e, 0xf>(m8, m8));
                 m8 = max(m8, dn_move<0x141, 0xf>(m8, m8));
                 m8 = max(m8, dn_move<0x140, 0xf>(m8, m8));
-                scale = q4_scaling(m8, factor);
+                scale = q4_scaling<TI>(m8, factor);
                 if ((tid & 15) == 0) factors[(at[m] >> 4) * 4 + of[m]] = factor;
             }
-            q4_split8(x[m], scale, hi, lo);
+            const float least = q4_split8(x[m], scale, hi, lo);
+            if (q4_range<TI>::wide && least < 0x1p-14f && q4_below<TI>(q4_least8(0, x[m]), factor)) {
+                q4_drop_below<TI>(x[m], factor);
+                (void)q4_split8(x[m], scale, hi, lo);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); /* behind the write above, which is the same wave's */
+                factors[(at[m] >> 4) * 4 + of[m]] = -factor;
+                s_below[wave] = 1;
+            }
             char *to = lds + of[m] * pitch + (at[m] >> 4) * BLOCK + (at[m] & 15) * 16;
             *(half8_t *)to = hi;
             if (PIECES == 2) *(half8_t *)(to + plane) = lo;
@@ -495,17 +593,28 @@ __global__ __launch_bounds__(Q4_THREADS, 4) void q4_direct_kernel(q4_args a)
                     for (int g = 0; g < PER; ++g) {
                         half2_t z1024, z64;
                         q4_zeros(w[u], g, z1024, z64);
-                        float4_t acc = {0, 0, 0, 0};
+                        /* the second piece has a sum of its own (one or two instructions more for a group, not four for each 8
+                         * weights), or goes first where that would take more registers than there are (a group is one step there) */
+                        constexpr int SUMS = PIECES == 2 && (PER < 4 || H < 4) ? 2 : 1;
+                        float4_t acc[SUMS];
+#pragma unroll
+                        for (int p = 0; p < SUMS; ++p) acc[p] = (float4_t){0, 0, 0, 0};
 #pragma unroll
                         for (int step = g * (4 / PER); step < (g + 1) * (4 / PER); ++step) {
+                            half8_t x[PIECES];
+#pragma unroll
+                            for (int p = 0; p < PIECES; ++p) x[p] = *(const half8_t *)(base + p * plane + kb * BLOCK + step * 64);
                             const half8_t wv = q4_unpack8(w[u].code[step], z1024, z64, masks);
 #pragma unroll
-                            for (int p = 0; p < PIECES; ++p)
-                                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const half8_t *)(base + p * plane + kb * BLOCK + step * 64), wv, acc, 0, 0, 0);
+                            for (int p = PIECES - 1; p >= 0; --p) {
+                                acc[p % SUMS] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[p], wv, acc[p % SUMS], 0, 0, 0);
+                                if (SUMS == 1 && p == 1) acc[0] *= (float4_t){Q4_LO, Q4_LO, Q4_LO, Q4_LO};
+                            }
                         }
-                        const float v = own_block == 0 ? acc[0] : own_block == 1 ? acc[1] : own_block == 2 ? acc[2] : acc[3];
+                        auto own = [&](float4_t v) { return own_block == 0 ? v[0] : own_block == 1 ? v[1] : own_block == 2 ? v[2] : v[3]; };
+                        const float v = SUMS == 2 ? fmaf(own(acc[SUMS - 1]), Q4_LO, own(acc[0])) : own(acc[0]);
                         const float f = TI != DN_I8 || XG ? own_factors[(XG ? kb * PER + g : kb) * 4] : 1.f;
-                        sum = fmaf(v, f * w[u].scale[g], sum);
+                        sum = fmaf(v, (q4_range<TI>::wide ? fabsf(f) : f) * w[u].scale[g], sum);
                     }
                 }
                 if (last ? u < mine && unit0 + stride < units : n + AHEAD + u < mine)
@@ -527,6 +636,15 @@ __global__ __launch_bounds__(Q4_THREADS, 4) void q4_direct_kernel(q4_args a)
             for (int q = 0; q < WAVES; ++q)
                 if (q < a.ksplit) y += s_red[r * a.ksplit + q][b][i % WIDTH];
             if (TI == DN_I8 && !XG) y *= a.input_scales[b];
+            if constexpr (q4_range<TI>::wide) {
+                unsigned any = 0;
+#pragma unroll
+                for (int q = 0; q < WAVES; ++q) any |= s_below[q];
+                if (__builtin_expect(any != 0, 0)) {
+                    auto factor = [&](int kb) { return -factors[kb * 4 + b]; };
+                    y += q4_left_out<TI>(a, b, o, [&](int kb) { return factor(kb) > 0 ? 0xffffu : 0u; }, factor);
+                }
+            }
             q4_store(a, b, o, y, bias);
         }
     }
@@ -534,10 +652,12 @@ __global__ __launch_bounds__(Q4_THREADS, 4) void q4_direct_kernel(q4_args a)
 
 /* ---- larger input, first pass: one workgroup for each row scales it and writes it in the order in which the second
  * pass feeds it to the matrix instruction: [row / 16][inputs / 128] blocks of [piece][step][lane][8 halves] and, for
- * 8-bit input with groups, [group in 128][16] factors.  Behind the blocks a factor for each row.  A pass over a few
- * kilobytes, 3 to 5 us with its launch; it saves every workgroup of the second pass a scaling of its own (16 rows
- * of 8192 values read as they are by that pass, without this one: the same time in groups of 128, 27 us against 20 in
- * groups of 32).  1024 threads for long rows: 8 rows of 20787 in all 17.8 us, 21 with 256. */
+ * 8-bit input with groups, [group in 128][16] factors.  Behind the blocks a factor for each row, negative (fp32 and bf16
+ * input) where values lie below what the pieces hold; then [row][inputs / 128] the 16 bits of the eights that have
+ * such values, written for these rows only.  A pass over a few kilobytes, 3 to 5 us with its launch; it saves every
+ * workgroup of the second pass a scaling of its own (16 rows of 8192 values read as they are by that pass, without this
+ * one: the same time in groups of 128, 27 us against 20 in groups of 32).  1024 threads for long rows: 8 rows of 20787
+ * in all 17.8 us, 21 with 256. */
 __host__ __device__ static inline int q4_block_bytes(const q4_shape &s, int pieces, bool groups)
 {
     return pieces * 4096 + (groups ? 128 / s.group * 64 : 0);
@@ -548,37 +668,58 @@ __host__ __device__ static inline size_t q4_rows_at(const q4_shape &s, int piece
     return ((size_t)batch + 15) / 16 * s.kblocks * q4_block_bytes(s, pieces, groups);
 }
 
+__host__ __device__ static inline size_t q4_marks_at(const q4_shape &s, int pieces, int batch, bool groups)
+{
+    return q4_rows_at(s, pieces, batch, groups) + (size_t)batch * 4;
+}
+
 template <int TI, bool XG, int THREADS>
 __global__ __launch_bounds__(THREADS) void q4_prepare_kernel(q4_args a)
 {
     constexpr int PIECES = TI == DN_F32 ? 2 : 1;
-    __shared__ unsigned s_largest[THREADS / 64];
+    __shared__ unsigned s_largest[THREADS / 64], s_least[THREADS / 64];
     const int tid = threadIdx.x, b = blockIdx.x, block = q4_block_bytes(a.s, PIECES, XG);
     const size_t row_bytes = (size_t)a.s.inputs * (TI == DN_F32 ? 4 : TI == DN_I8 ? 1 : 2);
     const char *row = (const char *)a.input + b * row_bytes;
     float factor = 1, scale = 1;
+    bool below = false;
     if (TI != DN_I8) {
-        unsigned m = 0;
+        unsigned m = 0, least = 0;
 #pragma unroll 4
         for (int k = tid * 8; k < a.s.inputs; k += THREADS * 8) {
             float x[8];
             q4_load8<TI>(row, k, a.s.inputs, x);
             m = q4_largest8(m, x);
+            if (q4_range<TI>::wide) least = q4_least8(least, x);
         }
         m = dn_wave_max(m);
-        if ((tid & 63) == 0) s_largest[tid >> 6] = m;
+        if (q4_range<TI>::wide) least = dn_wave_max(least);
+        if ((tid & 63) == 0) {
+            s_largest[tid >> 6] = m;
+            s_least[tid >> 6] = least;
+        }
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < THREADS / 64; ++w) m = max(m, s_largest[w]);
-        scale = q4_scaling(m, factor);
+        for (int w = 0; w < THREADS / 64; ++w) {
+            m = max(m, s_largest[w]);
+            if (q4_range<TI>::wide) least = max(least, s_least[w]);
+        }
+        scale = q4_scaling<TI>(m, factor);
+        below = q4_below<TI>(least, factor);
     }
     if (tid == 0)
-        ((float *)(a.workspace + q4_rows_at(a.s, PIECES, a.batch, XG)))[b] = TI == DN_I8 ? (XG ? 1.f : a.input_scales[b]) : factor;
+        ((float *)(a.workspace + q4_rows_at(a.s, PIECES, a.batch, XG)))[b] = TI == DN_I8 ? (XG ? 1.f : a.input_scales[b]) : below ? -factor : factor;
     unsigned char *out = a.workspace + (size_t)(b >> 4) * a.s.kblocks * block + (b & 15) * 16;
     for (int k = tid * 8; k < a.s.kblocks * 128; k += THREADS * 8) {
         float x[8];
         half8_t hi, lo;
         q4_load8<TI>(row, k, a.s.inputs, x);
+        if (q4_range<TI>::wide && below) { /* 16 lanes have a block */
+            const unsigned mark = (unsigned)(__ballot(q4_below<TI>(q4_least8(0, x), factor)) >> (tid & 48)) & 0xffffu;
+            if ((tid & 15) == 0)
+                ((unsigned short *)(a.workspace + q4_marks_at(a.s, PIECES, a.batch, XG)))[(size_t)b * a.s.kblocks + (k >> 7)] = (unsigned short)mark;
+            q4_drop_below<TI>(x, factor);
+        }
         q4_split8(x, scale, hi, lo);
         unsigned char *to = out + (size_t)(k >> 7) * block + ((k >> 5) & 3) * 1024 + ((k >> 3) & 3) * 256;
         *(half8_t *)to = hi;
@@ -592,7 +733,27 @@ __global__ __launch_bounds__(THREADS) void q4_prepare_kernel(q4_args a)
     }
 }
 
+/* Whether a row has values that the pieces do not hold, and what they leave of its sum with an output. */
+template <bool XG>
+__device__ __forceinline__ bool q4_is_below(const q4_args &a, float row_factor) { return !XG && a.ranged && row_factor < 0; }
+
+template <int PIECES>
+__device__ __forceinline__ float q4_left_out_of(const q4_args &a, float row_factor, int b, int o)
+{
+    const unsigned short *marks = (const unsigned short *)(a.workspace + q4_marks_at(a.s, PIECES, a.batch, false)) + (size_t)b * a.s.kblocks;
+    return q4_left_out<PIECES == 2 ? DN_F32 : DN_BF16>(a, b, o, [&](int kb) { return (unsigned)marks[kb]; }, [&](int) { return -row_factor; });
+}
+
+/* A sum with its row's factor. */
+template <int PIECES, bool XG>
+__device__ __forceinline__ float q4_scaled(const q4_args &a, float row_factor, int b, int o, float y)
+{
+    if (q4_is_below<XG>(a, row_factor)) return fmaf(y, -row_factor, q4_left_out_of<PIECES>(a, row_factor, b, o));
+    return y * row_factor;
+}
+
 /* A lane's results of one tile of outputs and 16 rows, with the rows' own factors. */
+template <int PIECES, bool XG>
 __device__ __forceinline__ void q4_store_tile(const q4_args &a, const float *row_factors, int tile, int b0, float4_t v)
 {
     const int lane = threadIdx.x & 63, o = tile * 16 + (lane & 15);
@@ -602,14 +763,14 @@ __device__ __forceinline__ void q4_store_tile(const q4_args &a, const float *row
     for (int i = 0; i < 4; ++i) {
         const int b = b0 + (lane >> 4) * 4 + i;
         const float y = i == 0 ? v[0] : i == 1 ? v[1] : i == 2 ? v[2] : v[3];
-        if (b < a.batch) q4_store(a, b, o, y * row_factors[b], bias);
+        if (b < a.batch) q4_store(a, b, o, q4_scaled<PIECES, XG>(a, row_factors[b], b, o, y), bias);
     }
 }
 
 /* The same as one of several parts of the sums, which the next pass joins. */
 __host__ __device__ static inline size_t q4_parts_at(const q4_shape &s, int pieces, int batch, bool groups)
 {
-    return (q4_rows_at(s, pieces, batch, groups) + (size_t)batch * 4 + 15) / 16 * 16;
+    return (q4_marks_at(s, pieces, batch, groups) + (size_t)batch * s.kblocks * 2 + 15) / 16 * 16;
 }
 
 __device__ __forceinline__ void q4_store_part(const q4_args &a, size_t parts_at, int tile, int b0, float4_t v)
@@ -625,6 +786,7 @@ __device__ __forceinline__ void q4_store_part(const q4_args &a, size_t parts_at,
 }
 
 /* Third pass, where the inputs were cut: the parts' sums of an output, in their order. */
+template <int PIECES, bool XG>
 __global__ __launch_bounds__(256) void q4_join_kernel(q4_args a, size_t rows_at, size_t parts_at, int parts)
 {
     const int o = blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
@@ -634,7 +796,7 @@ __global__ __launch_bounds__(256) void q4_join_kernel(q4_args a, size_t rows_at,
     float y = 0;
 #pragma unroll 4
     for (int p = 0; p < parts; ++p) y += part[(size_t)p * a.batch * a.s.outputs];
-    q4_store(a, b, o, y * factor, bias);
+    q4_store(a, b, o, q4_scaled<PIECES, XG>(a, factor, b, o, y), bias);
 }
 
 /* ---- second pass, few outputs: a workgroup takes R row tiles and a tile of input rows, its eight waves an eighth of
@@ -695,7 +857,7 @@ __global__ __launch_bounds__(Q4_THREADS) void q4_stream_kernel(q4_args a)
 #pragma unroll
             for (int q = 1; q < Q4_WAVES; ++q) v += s_red[q][lane];
             if (gridDim.z > 1) q4_store_part(a, q4_parts_at(a.s, PIECES, a.batch, XG), tile0 + k, x_tile * 16, v);
-            else q4_store_tile(a, row_factors, tile0 + k, x_tile * 16, v);
+            else q4_store_tile<PIECES, XG>(a, row_factors, tile0 + k, x_tile * 16, v);
         }
     }
 }
@@ -837,8 +999,18 @@ __global__ __launch_bounds__(Q4_STAGED_WAVES * 64, 2) void q4_staged_kernel(q4_a
         for (int row = tid / (WIDTH / 4); row < 16; row += THREADS / (WIDTH / 4)) {
             const int b = (x0 + x) * 16 + row;
             const float f = s_factors[x * 16 + row];
-            const float4_t factor = {f, f, f, f};
-            if (b < a.batch && o < a.s.outputs) q4_store4(a, b, o, __builtin_elementwise_fma(*(const float4_t *)(s_sum + row * PITCH + column), factor, bias));
+            if (b >= a.batch || o >= a.s.outputs) continue;
+            float4_t y = *(const float4_t *)(s_sum + row * PITCH + column);
+            if (q4_is_below<XG>(a, f))
+#pragma unroll 1
+                for (int i = 0; i < 4; ++i) {
+                    const float s = i == 0 ? y[0] : i == 1 ? y[1] : i == 2 ? y[2] : y[3];
+                    const float x = o + i < a.s.outputs ? q4_scaled<PIECES, XG>(a, f, b, o + i, s) + q4_bias(a, o + i) : 0.f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = i == e ? x : y[e];
+                }
+            else y = __builtin_elementwise_fma(y, (float4_t){f, f, f, f}, bias);
+            q4_store4(a, b, o, y);
         }
         __syncthreads();
     }
@@ -913,8 +1085,7 @@ extern "C" size_t connected_q4_workspace_bytes(int input_type, int batch, int in
     const q4_plan p = q4_plan_of(s, input_type, batch);
     if (p.form == q4_plan::DIRECT) return 0;
     const int pieces = input_type == DN_F32 ? 2 : 1;
-    if (p.gz > 1) return q4_parts_at(s, pieces, batch, input_type == DN_I8) + (size_t)p.gz * batch * outputs * 4;
-    return q4_rows_at(s, pieces, batch, input_type == DN_I8) + (size_t)batch * 4;
+    return q4_parts_at(s, pieces, batch, input_type == DN_I8) + (p.gz > 1 ? (size_t)p.gz * batch * outputs * 4 : 0);
 }
 
 template <int T, int R, int PIECES, int PER, bool XG>
@@ -926,7 +1097,7 @@ static void q4_launch_second(const q4_args &a, const q4_plan &p)
     else if constexpr (T == 1) {
         hipLaunchKernelGGL((q4_stream_kernel<R, PIECES, PER, XG>), grid, dim3(Q4_THREADS), 0, dn_stream(), a);
         if (p.gz > 1)
-            hipLaunchKernelGGL(q4_join_kernel, dim3((unsigned)((a.s.outputs + 255) / 256), (unsigned)a.batch), dim3(256), 0, dn_stream(), a,
+            hipLaunchKernelGGL((q4_join_kernel<PIECES, XG>), dim3((unsigned)((a.s.outputs + 255) / 256), (unsigned)a.batch), dim3(256), 0, dn_stream(), a,
                                q4_rows_at(a.s, PIECES, a.batch, XG), q4_parts_at(a.s, PIECES, a.batch, XG), (int)p.gz);
     }
 }
@@ -990,7 +1161,7 @@ extern "C" int forward_connected_q4_gpu(const void *input, int input_type, const
     if (p.gx > 0x7fffffu || p.gy > 65535u) return dn_refuse(me, "too many outputs or rows for one call");
     hip_require_device(me);
     const q4_args a = {input, input_scales, (const unsigned char *)packed, biases, output, (unsigned char *)workspace,
-                       output_type, batch, xg ? input_group : 0, activation, p.ksplit, p.run, s};
+                       output_type, input_type == DN_F32 || input_type == DN_BF16, batch, xg ? input_group : 0, activation, p.ksplit, p.run, s};
     if (input_type == DN_F32) q4_launch_group<DN_F32, false>(a, p);
     else if (input_type == DN_F16) q4_launch_group<DN_F16, false>(a, p);
     else if (input_type == DN_BF16) q4_launch_group<DN_BF16, false>(a, p);

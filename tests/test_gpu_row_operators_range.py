@@ -1,0 +1,96 @@
+"""Row operators on the device where values of very different sizes meet: products of rows with a few large inputs."""
+import numpy as np
+import pytest
+
+import row_reference as R
+from row_reference import BF16, F16, F32, Buffer
+
+pytestmark = pytest.mark.gpu
+
+
+class Weights:
+    """A layer whose codes, scales and zeros are given."""
+
+    def __init__(self, dn, codes, scales, zeros, group):
+        (self.n, self.k), self.group = codes.shape, group
+        self.w = R.q4_weights(codes, scales, zeros, group)
+        self.packed = Buffer(shape=(dn.q4_packed_bytes(self.k, self.n, group),), dtype=np.uint8, shift=16)
+        src = [Buffer(R.q4_bytes(codes)), Buffer(scales), Buffer(zeros)]
+        assert dn.q4_pack_codes_gpu(src[0].ptr, src[1].ptr, src[2].ptr, self.packed.ptr, self.k, self.n, group) == 0
+        dn.hip_synchronize()
+
+    def product(self, dn, bits, tx, scales=None, x_group=0, t_out=F32, bias=None, act=3):
+        """What the library gives for the rows `bits` of type tx."""
+        batch = len(bits)
+        size = dn.connected_q4_workspace_bytes(tx, batch, self.k, self.n, self.group)
+        ws = Buffer(shape=(size,), dtype=np.uint8, shift=16) if size else None
+        bx, bs, bb = Buffer(bits), Buffer(scales) if scales is not None else None, Buffer(bias) if bias is not None else None
+        out = Buffer(shape=(batch, self.n), dtype=R.STORE[t_out])
+        assert dn.forward_connected_q4_gpu(bx.ptr, tx, bs.ptr if bs else None, x_group, self.packed.ptr, bb.ptr if bb else None, out.ptr, t_out,
+                                           batch, self.k, self.n, self.group, act, ws.ptr if ws else None) == 0
+        dn.hip_synchronize()
+        if ws:
+            ws.get()
+        return R.from_type(out.get(), t_out).astype(np.float64)
+
+
+def single_weights(seed, n, k, group, scale=0.02):
+    """(codes, scales, zeros, column of each output): each output has one weight that is not 0."""
+    r = np.random.default_rng(seed)
+    groups = -(-k // group)
+    zeros = r.integers(0, 16, (n, groups), dtype=np.uint8)
+    scales = ((0.5 + r.random((n, groups))) * scale).astype(np.float32)
+    codes = zeros[:, np.arange(k) // group].copy()
+    column = r.integers(0, k, n)
+    codes[np.arange(n), column] = (codes[np.arange(n), column] + r.integers(1, 16, n)) % 16
+    return codes, scales, zeros, column
+
+
+# rows, inputs, outputs: few rows; 16 rows a workgroup; the inputs cut over workgroups; many outputs, one to four tiles of rows
+FORMS = [(1, 700, 90), (4, 700, 90), (3, 5003, 3000), (5, 700, 90), (20, 700, 90), (5, 8200, 60), (5, 300, 40000), (20, 300, 20000), (40, 200, 14000), (64, 200, 11300)]
+
+
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("batch,k,n", FORMS)
+def test_q4_every_value_keeps_its_bits(dn, batch, k, n, t, group):
+    """Values of all sizes in a row, each alone in the outputs that have its weight: fp32 is held to 2^-23 of a value, the
+    other types exactly; the sum of one product with the group's scale and the scaling takes at most four roundings more."""
+    r = np.random.default_rng(batch + k + n)
+    codes, scales, zeros, column = single_weights(k, n, k, group)
+    low, high = (-24, 15.99) if t == F16 else (-110, 120)
+    x = (np.sign(r.standard_normal((batch, k))) * 2.0 ** r.uniform(low, high, (batch, k))).astype(np.float32)
+    x[:, r.random(k) < 0.02] = 0
+    x[batch // 2] = r.standard_normal(k)                       # one row as usual
+    bits = R.to_type(x, t)
+    x = R.from_type(bits, t).astype(np.float64)
+    m = Weights(dn, codes, scales, zeros, group)
+    got = m.product(dn, bits, t)
+    want = x[:, column] * m.w[np.arange(n), column]
+    tol = np.abs(want) * ((2.0 ** -23 if t == F32 else 0) + 5 * 2.0 ** -24)
+    bad = np.abs(got - want) > tol
+    assert not bad.any(), (int(bad.sum()), float((np.abs(got - want) / np.maximum(np.abs(want), 1e-300)).max()))
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("batch", [1, 4, 5, 64])
+@pytest.mark.parametrize("outlier", [1e6, 1e9, 2.0 ** 60, 3e38])
+def test_q4_an_outlier_whose_weight_is_zero(dn, batch, outlier, t):
+    """Ordinary rows and weights but for one large input that no output has.  Each value is held to 2^-23 (fp32), a group's
+    sum takes a rounding for each of its eight matrix instructions and eight within one, and each group is added once."""
+    k, n, group = 4096, 600, 128
+    r = np.random.default_rng(batch)
+    codes, scales, zeros = R.q4_codes(batch, n, k, group)
+    x = r.standard_normal((batch, k)).astype(np.float32)
+    for b in range(batch):
+        at = 37 + 61 * b
+        x[b, at] = outlier
+        codes[:, at] = zeros[:, at // group]
+    bits = R.to_type(x, t)
+    x = R.from_type(bits, t).astype(np.float64)
+    m = Weights(dn, codes, scales, zeros, group)
+    got = m.product(dn, bits, t)
+    want = x @ m.w.T
+    size = np.abs(x) @ np.abs(m.w).T
+    tol = size * ((2.0 ** -23 if t == F32 else 0) + (64 + k // group + 8) * 2.0 ** -24)
+    assert (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / size).max() * 2 ** 24)
