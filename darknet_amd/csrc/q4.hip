@@ -186,8 +186,9 @@ extern "C" int q4_unpack_weights_gpu(const void *packed, float *weights, int inp
  * that the second meets are 2^-12 times the others).  Values further below are left out there; each eight inputs that
  * have some are marked, and their products are added to the output at the end, one by one: an ordinary row has hardly any,
  * but an output whose weights avoid the large inputs would miss them.  Products are exact in the fp32 accumulators, which
- * a group starts from zero; its sum is then multiplied with the scale and added to the output's.  Where a value is not
- * finite the factor that undoes the scaling is NaN.
+ * a group starts from zero; its sum is then multiplied with the scale and added to the output's, the factors of the input
+ * last: a factor times a scale may be below the normal range where the output is not.  Where a value is not finite the
+ * factor that undoes the scaling is NaN.
  *
  * The input is the instruction's first operand and the weights the second, so that a lane's results are those
  * of one output, whose scale and zero it has read beside the codes.
@@ -461,7 +462,7 @@ __device__ __forceinline__ void q4_multiply(const q4_masks &masks, const q4_tile
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 const float4_t scale = {w[r].scale[g], w[r].scale[g], w[r].scale[g], w[r].scale[g]};
-                sum[r][t] = __builtin_elementwise_fma(acc[r][t], XS ? f * scale : scale, sum[r][t]);
+                sum[r][t] = XS ? __builtin_elementwise_fma(acc[r][t] * scale, f, sum[r][t]) : __builtin_elementwise_fma(acc[r][t], scale, sum[r][t]);
             }
         }
     }
@@ -614,7 +615,7 @@ __global__ __launch_bounds__(Q4_THREADS, 4) void q4_direct_kernel(q4_args a)
                         auto own = [&](float4_t v) { return own_block == 0 ? v[0] : own_block == 1 ? v[1] : own_block == 2 ? v[2] : v[3]; };
                         const float v = SUMS == 2 ? fmaf(own(acc[SUMS - 1]), Q4_LO, own(acc[0])) : own(acc[0]);
                         const float f = TI != DN_I8 || XG ? own_factors[(XG ? kb * PER + g : kb) * 4] : 1.f;
-                        sum = fmaf(v, (q4_range<TI>::wide ? fabsf(f) : f) * w[u].scale[g], sum);
+                        sum = fmaf(v * w[u].scale[g], q4_range<TI>::wide ? fabsf(f) : f, sum);
                     }
                 }
                 if (last ? u < mine && unit0 + stride < units : n + AHEAD + u < mine)

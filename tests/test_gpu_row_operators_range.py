@@ -1,9 +1,11 @@
-"""Row operators on the device where values of very different sizes meet: products of rows with a few large inputs."""
+"""Row operators on the device where values of very different sizes meet, or lie on a border: products of rows with a few
+large inputs, of small inputs and scales, 8-bit codes between two steps, one token far above many."""
 import numpy as np
 import pytest
 
 import row_reference as R
 from row_reference import BF16, F16, F32, Buffer
+from test_gpu_row_operators import check_draw, draw
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +96,28 @@ def test_q4_an_outlier_whose_weight_is_zero(dn, batch, outlier, t):
     size = np.abs(x) @ np.abs(m.w).T
     tol = size * ((2.0 ** -23 if t == F32 else 0) + (64 + k // group + 8) * 2.0 ** -24)
     assert (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / size).max() * 2 ** 24)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("batch", [1, 2, 4, 6, 30])
+def test_q4_small_inputs_with_small_scales(dn, batch, group):
+    """Rows near the least fp32 values, weights whose scales are small too: outputs are within the range of fp32 although
+    the product of a row's factor and a scale is not.  Bounds as above; what is below the normal range has its own step."""
+    k, n = 700, 45
+    r = np.random.default_rng(batch + group)
+    codes, scales, zeros = R.q4_codes(batch, n, k, group)
+    for size, small in ((1e-33, 1e-3), (1e-36, 1.0), (1e-28, 1e-8), (1e-14, 1e-20), (1e-30, 1e20), (1e10, 1e-25)):
+        sc = (scales * np.float32(small)).astype(np.float32)
+        m = Weights(dn, codes, sc, zeros, group)
+        x = (r.standard_normal((batch, k)) * size).astype(np.float32)
+        got, want = m.product(dn, x, F32), x.astype(np.float64) @ m.w.T
+        tol = np.abs(x.astype(np.float64)) @ np.abs(m.w).T * (2.0 ** -23 + (64 + -(-k // group) + 8) * 2.0 ** -24) + (k // group + 8) * 2.0 ** -149
+        assert (np.abs(got - want) <= tol).all(), (size, small)
+        # 8 bits: whole numbers, so that only scales and sums round
+        bits = r.integers(-127, 128, (batch, k), dtype=np.int8)
+        for xg in (0, group):
+            xs = ((0.5 + r.random((batch, -(-k // xg) if xg else 1))) * size).astype(np.float32)
+            v = bits * xs.astype(np.float64)[:, np.arange(k) // xg if xg else np.zeros(k, int)]
+            got, want = m.product(dn, bits, R.I8, xs, xg), v @ m.w.T
+            tol = np.abs(v) @ np.abs(m.w).T * (-(-k // group) + 16) * 2.0 ** -24 + (k // group + 8) * 2.0 ** -149
+            assert (np.abs(got - want) <= tol).all(), (size, small, xg)
