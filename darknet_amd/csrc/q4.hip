@@ -243,6 +243,12 @@ __device__ __forceinline__ float q4_scaling(unsigned largest, float &factor)
     return ldexpf(1.f, shift);
 }
 
+/* A scale of 8-bit input: NaN if it is not finite, as an infinite one times a code may be either. */
+__device__ __forceinline__ float q4_input_scale(const float *p)
+{
+    return fabsf(*p) <= 3.402823466e38f ? *p : __uint_as_float(0x7fc00000u);
+}
+
 /* Eight inputs from k on, zeros behind the row's end, in one access (two of fp32) whatever their alignment: the run that
  * the end cuts is read from eight before the end, and moved. */
 template <int TI>
@@ -574,7 +580,7 @@ __global__ __launch_bounds__(Q4_THREADS, 4) void q4_direct_kernel(q4_args a)
         const int x_groups = (a.s.inputs + a.x_group - 1) / a.x_group, groups = kpad / 128 * PER;
         for (int i = tid; i < a.batch * groups; i += THREADS) {
             const int b = i / groups, g = i - b * groups;
-            factors[g * 4 + b] = g < x_groups ? a.input_scales[(long)b * x_groups + g] : 0.f;
+            factors[g * 4 + b] = g < x_groups ? q4_input_scale(a.input_scales + (long)b * x_groups + g) : 0.f;
         }
     }
     __syncthreads();
@@ -636,7 +642,7 @@ __global__ __launch_bounds__(Q4_THREADS, 4) void q4_direct_kernel(q4_args a)
 #pragma unroll
             for (int q = 0; q < WAVES; ++q)
                 if (q < a.ksplit) y += s_red[r * a.ksplit + q][b][i % WIDTH];
-            if (TI == DN_I8 && !XG) y *= a.input_scales[b];
+            if (TI == DN_I8 && !XG) y *= q4_input_scale(a.input_scales + b);
             if constexpr (q4_range<TI>::wide) {
                 unsigned any = 0;
 #pragma unroll
@@ -709,7 +715,7 @@ __global__ __launch_bounds__(THREADS) void q4_prepare_kernel(q4_args a)
         below = q4_below<TI>(least, factor);
     }
     if (tid == 0)
-        ((float *)(a.workspace + q4_rows_at(a.s, PIECES, a.batch, XG)))[b] = TI == DN_I8 ? (XG ? 1.f : a.input_scales[b]) : below ? -factor : factor;
+        ((float *)(a.workspace + q4_rows_at(a.s, PIECES, a.batch, XG)))[b] = TI == DN_I8 ? (XG ? 1.f : q4_input_scale(a.input_scales + b)) : below ? -factor : factor;
     unsigned char *out = a.workspace + (size_t)(b >> 4) * a.s.kblocks * block + (b & 15) * 16;
     for (int k = tid * 8; k < a.s.kblocks * 128; k += THREADS * 8) {
         float x[8];
@@ -730,7 +736,7 @@ __global__ __launch_bounds__(THREADS) void q4_prepare_kernel(q4_args a)
         const int x_groups = (a.s.inputs + a.x_group - 1) / a.x_group, per = 128 / a.s.group;
         unsigned char *to = a.workspace + (size_t)(b >> 4) * a.s.kblocks * block + PIECES * 4096 + (b & 15) * 4;
         for (int g = tid; g < a.s.groups; g += THREADS)
-            *(float *)(to + (size_t)(g / per) * block + g % per * 64) = g < x_groups ? a.input_scales[(long)b * x_groups + g] : 0.f;
+            *(float *)(to + (size_t)(g / per) * block + g % per * 64) = g < x_groups ? q4_input_scale(a.input_scales + (long)b * x_groups + g) : 0.f;
     }
 }
 

@@ -484,8 +484,8 @@ int forward_rmsnorm_gpu(const void *input, const void *add, const float *scales,
  * is 0).  Every output is the same in every run.  fp32 input is held to 2^-23 of each value, whatever else the row
  * holds, the other types exactly; sums are fp32, for scales of weights that are 0 or between 2^-100 and 2^100 in
  * absolute value.  (A row whose values lie very far apart, more than 2^28 in fp32 and 2^31 in
- * bf16, takes longer.)  For a row of the input that holds a value that is not finite all the sums are NaN; the
- * activation is applied to that. */
+ * bf16, takes longer.)  For a row of the input that holds a value, or a scale, that is not finite all
+ * the sums are NaN; the activation is applied to that. */
 size_t q4_packed_bytes(int inputs, int outputs, int group);
 int q4_pack_codes_gpu(const unsigned char *codes, const float *scales, const unsigned char *zeros, void *packed,
                       int inputs, int outputs, int group);

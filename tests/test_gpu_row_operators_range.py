@@ -121,3 +121,23 @@ def test_q4_small_inputs_with_small_scales(dn, batch, group):
             got, want = m.product(dn, bits, R.I8, xs, xg), v @ m.w.T
             tol = np.abs(v) @ np.abs(m.w).T * (-(-k // group) + 16) * 2.0 ** -24 + (k // group + 8) * 2.0 ** -149
             assert (np.abs(got - want) <= tol).all(), (size, small, xg)
+
+
+@pytest.mark.parametrize("batch", [1, 3, 5, 20])
+@pytest.mark.parametrize("n", [40, 12000])
+def test_q4_scales_of_8_bit_rows_that_are_not_finite(dn, batch, n):
+    """A row with an infinite or NaN scale: all its sums are NaN, whatever its codes; the other rows are as without it."""
+    k, group = 300, 32
+    codes, scales, zeros = R.q4_codes(batch, n, k, group)
+    m = Weights(dn, codes, scales, zeros, group)
+    r = np.random.default_rng(n)
+    bits = r.integers(-127, 128, (batch, k), dtype=np.int8)
+    for value in (np.inf, -np.inf, np.nan):
+        for xg in (0, group):
+            xs = (0.5 + r.random((batch, -(-k // xg) if xg else 1))).astype(np.float32)
+            fine = m.product(dn, bits, R.I8, xs, xg)
+            xs[batch // 2, -1] = value
+            got = m.product(dn, bits, R.I8, xs, xg)
+            assert np.isnan(got[batch // 2]).all()
+            rest = np.arange(batch) != batch // 2
+            assert np.array_equal(got[rest], fine[rest])
