@@ -21,7 +21,6 @@ struct norm_args {
     float *q8_scales;
     int rows, n, group; /* group: values that share a scale, 0 = the row */
     float eps;
-    double inv_n;
 };
 
 /* Sum (or maximum) over the workgroup, the same bits on every lane and in every run. */
@@ -39,10 +38,15 @@ __device__ __forceinline__ double block_all(double v, double *lds)
     return t;
 }
 
-/* The scale of a group whose largest |y| is given; NaN where that is not finite. */
-__device__ __forceinline__ float q8_step(double largest)
+/* A value y can lie half-way between two steps only if the row's root mean square has few bits: y = p / rms, where p = s *
+ * scales has 48 at most, is then a product of the step, a float, and a number of 8 bits.  In such rows (all values alike, say,
+ * without eps) what reciprocals give is looked at once more. */
+__device__ __forceinline__ bool q8_may_tie(double rms) { return ((unsigned long long)__double_as_longlong(rms) & 0xffffff) == 0; }
+
+/* The scale of a group whose largest |p| is given; NaN where that is not finite. */
+__device__ __forceinline__ float q8_step(double largest, double rms, double r, bool ties)
 {
-    const float c = (float)(largest * (1. / 127));
+    const float c = ties ? (float)(largest / rms / 127) : (float)(largest * r * (1. / 127));
     return c <= 3.402823466e38f ? c : __int_as_float(0x7fc00000);
 }
 
@@ -72,6 +76,15 @@ __device__ __forceinline__ double group_largest(double v, int lanes)
 __device__ __forceinline__ int q8_code(double p, double factor)
 {
     const int q = (int)__double_as_longlong(fma(p, factor, 0x1.8p52));
+    return max(-127, min(127, q));
+}
+
+/* rint(p / step) next to q, ties to even: the sign of a remainder that is rounded once is exact. */
+__device__ __forceinline__ int q8_nearest(int q, double p, double step)
+{
+    const double above = fma(-(q + .5), step, p), below = fma(-(q - .5), step, p);
+    if (above > 0 || (above == 0 && q & 1)) ++q;
+    else if (below < 0 || (below == 0 && q & 1)) --q;
     return max(-127, min(127, q));
 }
 
@@ -172,7 +185,7 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_kernel(norm_args a)
             }
         }
         acc = block_all<THREADS, false>(acc, lds);
-        const double r = 1. / sqrt(fma(acc, a.inv_n, (double)a.eps));
+        const double rms = sqrt(acc / n + (double)a.eps), r = 1. / rms;
         auto values = [&](int j, float v[V]) {
             if (RUNS) {
 #pragma unroll
@@ -200,6 +213,7 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_kernel(norm_args a)
                 for (int e = 0; e < V; ++e) asm volatile("" : "+v"(s[j][e]));
             const int lanes = a.group / V, groups = a.group ? (n + a.group - 1) / a.group : 1;
             const bool finite = acc <= 1.7976931348623157e308; /* and so every s */
+            const bool ties = __builtin_amdgcn_readfirstlane(q8_may_tie(rms));
             const double inf = __longlong_as_double(0x7ff0000000000000LL);
             /* p of a run, and max|p|: infinity where a factor is not finite (x * 0 is NaN then) */
             auto products = [&](int j, double p[V]) {
@@ -233,12 +247,18 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_kernel(norm_args a)
                 double p[V];
                 const double largest = a.group ? group_largest(products(j, p), lanes) : (products(j, p), row_largest);
                 /* an infinite maximum stays one: r may be 0 then */
-                const float c = largest < inf ? q8_step(largest * r) : __int_as_float(0x7fc00000);
+                const float c = largest < inf ? q8_step(largest, rms, r, ties) : __int_as_float(0x7fc00000);
                 const double factor = c > 0 ? q8_factor(r, c) : 0; /* codes are 0 where c is 0 or NaN */
                 if (a.group ? i < n && (tid & (lanes - 1)) == 0 : i == 0) a.q8_scales[row * groups + (a.group ? i / a.group : 0)] = c;
                 unsigned q[V];
+                if (ties) {
+                    const double step = rms * (double)c; /* 29 and 24 bits: exact */
 #pragma unroll
-                for (int e = 0; e < V; ++e) q[e] = (unsigned)(c > 0 ? q8_code(p[e], factor) : 0);
+                    for (int e = 0; e < V; ++e) q[e] = (unsigned)(c > 0 ? q8_nearest(q8_code(p[e], factor), p[e], step) : 0);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) q[e] = (unsigned)(c > 0 ? q8_code(p[e], factor) : 0);
+                }
                 signed char *to = a.q8 + row * n;
                 if (i + V <= n) {
                     typedef unsigned __attribute__((ext_vector_type(V / 4))) words;
@@ -319,7 +339,7 @@ extern "C" int forward_rmsnorm_gpu(const void *input, const void *add, const flo
         !dn_aligned(scales, 4) || !dn_aligned(q8_scales, 4))
         return dn_refuse(me, "a buffer is not aligned to its element type");
     hip_require_device(me);
-    const norm_args a = {input, add, scales, sum_output, output, q8_output, q8_scales, rows, n, q8_group, eps, 1. / n};
+    const norm_args a = {input, add, scales, sum_output, output, q8_output, q8_scales, rows, n, q8_group, eps};
     if (type == DN_F32) q8_output ? norm_launch<DN_F32, true>(a) : norm_launch<DN_F32, false>(a);
     else if (type == DN_F16) q8_output ? norm_launch<DN_F16, true>(a) : norm_launch<DN_F16, false>(a);
     else q8_output ? norm_launch<DN_BF16, true>(a) : norm_launch<DN_BF16, false>(a);

@@ -141,3 +141,28 @@ def test_q4_scales_of_8_bit_rows_that_are_not_finite(dn, batch, n):
             assert np.isnan(got[batch // 2]).all()
             rest = np.arange(batch) != batch // 2
             assert np.array_equal(got[rest], fine[rest])
+
+
+# ---- norm ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("n", [64, 300, 1000, 4096, 20000])
+def test_norm_codes_between_two_steps(dn, n, t):
+    """Rows whose root mean square is a whole number, scales that put values half-way between two steps: ties go to even."""
+    r = np.random.default_rng(n)
+    for rms in (1, 2, 3, 5, 7, 0.75):
+        x = (rms * r.choice([-1, 1], (2, n))).astype(np.float32)
+        for group in (0, 32, 128):
+            g = np.empty(n, np.float32)
+            for lo in range(0, n, group or n):
+                part = g[lo:lo + (group or n)]
+                step = np.float32(r.integers(1, 1 << 12) * 2.0 ** r.integers(-8, 3))
+                part[:] = step * (r.integers(-127, 127, len(part)) + np.float32(0.5))
+                part[r.integers(len(part))] = step * 127
+            bx, bg = Buffer(R.to_type(x, t)), Buffer(g)
+            q, c = Buffer(shape=(2, n), dtype=np.int8), Buffer(shape=(2, -(-n // (group or n))), dtype=np.float32)
+            assert dn.forward_rmsnorm_gpu(bx.ptr, None, bg.ptr, None, None, q.ptr, c.ptr, t, 2, n, group, 0.0) == 0
+            dn.hip_synchronize()
+            _, y = R.rmsnorm(R.to_type(x, t), None, g, 0.0, t)
+            assert np.array_equal(np.abs(y), np.abs(np.broadcast_to(g, y.shape)).astype(np.float64))    # exact
+            codes, want = R.q8(y, group)
+            assert np.array_equal(c.get(), want) and np.array_equal(q.get(), codes), (rms, group, int((q.get() != codes).sum()))
