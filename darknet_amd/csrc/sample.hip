@@ -7,11 +7,14 @@
  *   min-p   of these the tokens with w >= min_p (the largest has w = 1)
  * The answer is the first token in index order at which the running mass reaches u times the mass kept.
  *
- * Masses are whole numbers, rint(w * 2^38) with w in 64 bits: their sums do not depend on the order in which
- * lanes and atomics add them, so the same row gives the same token in every run, and a border between two
- * tokens lies where the formula puts it to within 2^-38 of the largest mass.
+ * Masses are whole numbers, rint(w * 2^b) with w in 64 bits: their sums do not depend on the order in which
+ * lanes and atomics add them, so the same row gives the same token in every run.  b is as large as the sum of a row
+ * whose tokens are all alike allows, 63 less the bits of an index: 46 for 131072 tokens, 39 for 2^24; and 48 at most, as
+ * the last bin has to weigh nothing.  Each mass is off by 2^-(b + 1) of the largest token's at most, in the same direction
+ * where logits are the same: a border between two tokens lies where the formula puts it to within n * 2^-(b + 1) of the
+ * largest mass, 2^-30 for 131072 tokens, and 2^-16 for 2^24.
  *
- * No row is sorted.  The logits are counted and weighed in 512 bins below the largest, a sixteenth of T wide (what is
+ * No row is sorted.  The logits are counted and weighed in 512 bins below the largest, a fifteenth of T wide (what is
  * further below weighs nothing) or, where the row's logits lie closer together, as much narrower.  The bin in which the
  * order's prefix ends is known from the running sums, everything in the bins before it is kept, and only that
  * bin's tokens (the candidates) are looked at more closely: digit by digit of their places.
@@ -25,8 +28,8 @@ typedef unsigned long long u64;
 typedef float float2_t __attribute__((ext_vector_type(2)));
 
 #define SM_BINS 512
-#define SM_PER_T 16
-#define SM_SHIFT 38
+#define SM_PER_T 15
+#define SM_SHIFT 48 /* of a mass, at most: what lies 511 / SM_PER_T times T below the largest has a weight below 2^-49 */
 #define SM_CANDIDATES 2048 /* that are kept in LDS */
 #define SM_LISTED 8192     /* of a long row that are kept in memory */
 #define SM_FOUND 512       /* of a segment that are handed on */
@@ -42,6 +45,7 @@ struct sample_args {
     long stride;
     int rows, n;
     int index_bits; /* that hold n - 1 */
+    double unit;    /* the mass of the largest token */
     int segments, length, block; /* length: tokens of a segment, block: of what its mass is summed over */
 };
 
@@ -50,6 +54,7 @@ struct sample_row {
     double log2_per_logit; /* log2(e) / T */
     double floor;          /* min-p */
     double uniform;        /* in 0 .. 1 */
+    double unit;           /* the mass of the largest token */
     float bins_per_logit;
     float p;               /* 2: off */
     int k;                 /* 0: off */
@@ -74,6 +79,7 @@ __device__ __forceinline__ sample_row settings_of(const sample_args &a, long row
     s.floor = a.min_p && m_of > 0 ? (double)fminf(m_of, 1.f) : 0.;
     s.uniform = u > 0 ? (double)fminf(u, 1.f) : 0.;
     s.log2_per_logit = 1.4426950408889634 / (double)t;
+    s.unit = a.unit;
     s.bins_per_logit = fminf(SM_PER_T / t, 3.402823466e38f);
     return s;
 }
@@ -100,30 +106,32 @@ struct sample_places {
     __device__ int index(u64 place) const { return (int)((1u << bits) - 1 - ((unsigned)place & ((1u << bits) - 1))); }
 };
 
-/* 2^x for x <= 0 as the first ten terms of its series around the nearest whole exponent: to 7e-12. */
+/* 2^x for x <= 0 around the nearest whole exponent: 1 + f * q(f), q the polynomial that meets (2^f - 1) / f in the ten
+ * Chebyshev points of -1/2 .. 1/2; to 2^-50. */
 __device__ __forceinline__ double weight_of(float l, float largest, const sample_row &s)
 {
     if (l == largest) return 1; /* also where both are infinite */
     const double x = ((double)l - (double)largest) * s.log2_per_logit;
     if (!(x > -64)) return 0;
     const double whole = rint(x), f = x - whole;
-    double p = 1.0178086009239696e-07;
-    p = fma(p, f, 1.3215486790144305e-06);
-    p = fma(p, f, 1.5252733804059838e-05);
-    p = fma(p, f, 0.00015403530393381606);
-    p = fma(p, f, 0.0013333558146428441);
-    p = fma(p, f, 0.009618129107628477);
-    p = fma(p, f, 0.055504108664821576);
-    p = fma(p, f, 0.2402265069591007);
-    p = fma(p, f, 0.6931471805599453);
+    double p = 7.070977866508138e-09;
+    p = fma(p, f, 1.0205905413765595e-07);
+    p = fma(p, f, 1.3215451633221434e-06);
+    p = fma(p, f, 1.5252672924850737e-05);
+    p = fma(p, f, 0.00015403530424776529);
+    p = fma(p, f, 0.0013333558200794592);
+    p = fma(p, f, 0.009618129107618665);
+    p = fma(p, f, 0.05550410866465167);
+    p = fma(p, f, 0.24022650695910075);
+    p = fma(p, f, 0.6931471805599462);
     p = fma(p, f, 1.);
     return ldexp(p, (int)whole);
 }
 
-/* rint(w * 2^38): added to 2^52 the number stands in the low bits of the sum. */
-__device__ __forceinline__ u64 mass_of(double w)
+/* rint(w * 2^b): added to 2^52 the number stands in the low bits of the sum. */
+__device__ __forceinline__ u64 mass_of(double w, const sample_row &s)
 {
-    return (u64)__double_as_longlong(w * 0x1p38 + 0x1p52) & 0xfffffffffffffull;
+    return (u64)__double_as_longlong(fma(w, s.unit, 0x1p52)) & 0xfffffffffffffull;
 }
 
 __device__ __forceinline__ int bin_of(float l, float largest, const sample_row &s)
@@ -243,7 +251,7 @@ __device__ __forceinline__ void find_border(sample_lds &s, const sample_row &r)
             u64 before;
             bin = counts.find(0, (u64)r.k, before);
             need = r.k - (int)before;
-            /* all that weighs anything is among the first k: what is in the last bin lies 31 T or more below the largest
+            /* all that weighs anything is among the first k: what is in the last bin lies 34 T or more below the largest
              * (but for a T next to which the difference of two logits is infinite) */
             if (bin == SM_BINS || (bin == SM_BINS - 1 && r.bins_per_logit > 1e-30f)) bin = -1;
         }
@@ -331,7 +339,7 @@ __device__ __forceinline__ void narrow_bins(sample_row &r, float2_t ends)
 __device__ __forceinline__ u64 weigh(float l, float largest, const sample_row &r)
 {
     const double w = weight_of(l, largest, r);
-    return mass_of(w) | (w >= r.floor ? SM_KEPT : 0);
+    return mass_of(w, r) | (w >= r.floor ? SM_KEPT : 0);
 }
 
 /* The candidates of a row: places and what weigh() says of them in LDS; where they are too many, a list of places
@@ -540,7 +548,7 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
                 if (!(l > -INFINITY)) continue;
                 const int b = bin_slot(bin_of(l, largest, r));
                 if (r.k) atomicAdd(&s.count[b], 1u);
-                if (r.p < 1) atomicAdd(&s.mass[b], mass_of(weight_of(l, largest, r)));
+                if (r.p < 1) atomicAdd(&s.mass[b], mass_of(weight_of(l, largest, r), r));
             }
             find_border(s, r);
             const sample_border b = s.border;
@@ -694,7 +702,7 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_bins_kernel(sample_ar
                 if (!(l[e] > -INFINITY)) continue;
                 const int b = bin_of(l[e], largest, r);
                 if (r.k) atomicAdd(&count[b], 1u);
-                if (r.p < 1) atomicAdd(&mass[b], mass_of(weight_of(l[e], largest, r)));
+                if (r.p < 1) atomicAdd(&mass[b], mass_of(weight_of(l[e], largest, r), r));
             }
         }
         __syncthreads();
@@ -742,7 +750,7 @@ __global__ __launch_bounds__(SM_SPLIT_THREADS) void sample_kept_kernel(sample_ar
                     const int bin = bin_of(l[e], largest, r);
                     if (bin < b.first) {
                         const double w = weight_of(l[e], largest, r);
-                        if (w >= r.floor) own += mass_of(w);
+                        if (w >= r.floor) own += mass_of(w, r);
                     } else if (is_candidate(b, bin)) {
                         const unsigned at = atomicAdd(&s_count, 1u);
                         if (at < SM_FOUND) s_list[at] = places.of(l[e], i + e);
@@ -929,8 +937,9 @@ extern "C" int sample_rows_gpu(const void *logits, int type, int rows, int n, lo
     if (!workspace && !sample_in_one(n)) return dn_refuse(me, "the workspace is missing");
     hip_require_device(me);
     sample_args a = {logits, temperature, top_p, min_p, uniform, top_k, tokens, probs, (unsigned char *)workspace,
-                     stride, rows, n, 1, 1, n, n};
+                     stride, rows, n, 1, 0, 1, n, n};
     while (1 << a.index_bits < n) ++a.index_bits;
+    a.unit = ldexp(1., 63 - a.index_bits < SM_SHIFT ? 63 - a.index_bits : SM_SHIFT);
     if (!sample_in_one(n)) sample_cut(a);
     if (type == DN_F32) sample_launch<DN_F32>(a);
     else if (type == DN_F16) sample_launch<DN_F16>(a);

@@ -509,8 +509,10 @@ int forward_connected_q4_gpu(const void *input, int input_type, const float *inp
  *   probs         NULL, or the token's share of the mass kept
  * Each array holds one value for each row, on the device.  NaN and -inf logits are never drawn; a row of
  * nothing else gives token -1 and probability 0.  If the largest logit is +inf the tokens that have it are
- * equally likely.  Masses are held as whole numbers of at least 38 bits below the largest token's, so sums do not
- * depend on their order: the same row gives the same token in every run and at every place in a batch.
+ * equally likely.  Masses are held as whole multiples of 2^-b of the largest token's, b = 48 for up to 32768 tokens
+ * and one less for each doubling beyond (46 for 131072, 39 for 2^24), so sums do not depend on their order: the same row
+ * gives the same token in every run and at every place in a batch.  A token of less than half such a multiple is not drawn,
+ * and many tokens that are alike, far below the largest, may together be off by n halves of it.
  * workspace: sample_workspace_bytes() bytes (NULL if that is 0). */
 size_t sample_workspace_bytes(int rows, int n);
 int sample_rows_gpu(const void *logits, int type, int rows, int n, long stride, const float *temperature,

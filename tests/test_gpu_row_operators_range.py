@@ -166,3 +166,72 @@ def test_norm_codes_between_two_steps(dn, n, t):
             assert np.array_equal(np.abs(y), np.abs(np.broadcast_to(g, y.shape)).astype(np.float64))    # exact
             codes, want = R.q8(y, group)
             assert np.array_equal(c.get(), want) and np.array_equal(q.get(), codes), (rms, group, int((q.get() != codes).sum()))
+
+
+# ---- sampling --------------------------------------------------------------------------------
+def mass_bits(n):
+    """The largest token's weight is 2^this in a row of n tokens."""
+    return min(48, 63 - max(1, (n - 1).bit_length()))
+
+
+@pytest.mark.parametrize("n,below", [(5000, 20.0), (8192, 27.0), (30000, 24.0), (131072, 25.0), (262144, 27.05), (1 << 20, 26.0), (1500001, 24.0), (1 << 24, 22.0)])
+@pytest.mark.parametrize("settings", ["none", "p", "min"])
+def test_sample_one_token_above_a_flat_vocabulary(dn, n, below, settings):
+    """One token, and all the others alike far below it, whose masses add up: each is a whole multiple of 2^-bits of the
+    largest, so the share of the others is known to n * 2^-(bits + 1), and the place of a draw among them accordingly."""
+    x = np.full((1, n), -below, np.float32)
+    top = n // 3
+    x[0, top] = 0
+    w = np.exp(-np.float64(np.float32(below)))
+    off = n * 2.0 ** -(mass_bits(n) + 1)
+    total = 1 + (n - 1) * w
+    u = np.float32([0.5, 1 - total ** -1 * (n - 1) * w * 0.5, 1 - 2.0 ** -24, total ** -1 * (top * w) * 0.5, 1.0])
+    rows = np.repeat(x, len(u), 0) if n < 1 << 20 else x
+    kw = dict(p=dict(top_p=[1 - 2.0 ** -24] * len(u)), min=dict(min_p=[w * 0.99] * len(u)), none={})[settings]
+    kept = n - 1                                             # of the others
+    if settings == "p":                                      # of the others the first by index
+        kept = max(0, min(n - 1, int(np.ceil((float(np.float32(1 - 2.0 ** -24)) * total - 1) / w))))
+    slack = off / w + 2
+    place = lambda rank: rank if rank < top else rank + 1    # noqa: E731  (of the others, by index)
+    for i in range(len(u)):
+        one = {a: v[:1] for a, v in kw.items()}
+        tok, prob = (draw(dn, rows[i:i + 1], F32, u[i:i + 1], **one) if len(rows) > 1 else draw(dn, x, F32, u[i:i + 1], **one))
+        if u[i] == 0.5 or kept == 0:
+            assert tok[0] == top
+            share = 1 / (1 + kept * w)
+            room = off + (slack * w if settings == "p" else 0)
+            assert abs(prob[0] - share) <= 2.0 ** -24 + room
+            continue
+        mass = float(u[i]) * (1 + kept * w)
+        rank = mass / w if mass < top * w else None if mass <= top * w + 1 else (mass - 1) / w
+        if rank is None or (settings == "p" and abs(mass - top * w - 1) < 2 * off):
+            continue
+        room = slack * (2 if settings == "p" else 1) + float(u[i]) * 2.0 ** -52 * n
+        assert abs(int(tok[0]) - place(min(kept - 1, max(0, int(rank))))) <= room + 1, (u[i], tok[0], rank)
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("n", [(1 << 20) + 1, (1 << 21) + 5000, 1 << 24])
+def test_sample_rows_beyond_a_million(dn, n, t):
+    """Blocks of several strips of 2048 tokens: draws into the first, the second and the last strips of a block."""
+    r = np.random.default_rng(n)
+    x = (r.standard_normal((1, n)) * 2).astype(np.float32)
+    x[0, r.integers(0, n, 40)] += 6
+    held = R.from_type(R.to_type(x, t), t)[0].astype(np.float64)
+    w = np.exp(held - held.max())
+    running = np.cumsum(w)
+    block = -(-n // (2048 * 512)) * 2048
+    places = [0, 2047, 2048, block - 1, block, 3 * block + 2048 + 77, n - 1, (n // block) * block, n - n // 7]
+    u = np.float32([(running[p] - 0.5 * w[p]) / running[-1] for p in places if p < n])
+    off = n * 2.0 ** -(mass_bits(n) + 1) + 2.0 ** -24 * running[-1]     # of masses; u in 32 bits
+    for one in u:
+        tok, prob = draw(dn, x, t, [one])
+        lo, hi = np.searchsorted(running, float(one) * running[-1] - off), np.searchsorted(running, float(one) * running[-1] + off)
+        assert lo <= tok[0] <= hi
+        assert abs(prob[0] - w[tok[0]] / running[-1]) <= 2.0 ** -24 + off
+    # borders among a few, among many and among equal tokens
+    for kw in (dict(top_k=[50]), dict(top_p=[0.4]), dict(top_k=[n // 2], top_p=[0.9], min_p=[1e-3])):
+        check_draw(dn, x, t, np.float32([0.61]), None, **kw)
+    flat = np.round(x * 0.5)
+    check_draw(dn, flat, t, np.float32([0.37]), None, top_k=[n // 3])
+    check_draw(dn, flat, t, np.float32([0.73]), None, top_p=[0.55])
