@@ -183,9 +183,10 @@ extern "C" int q4_unpack_weights_gpu(const void *packed, float *weights, int inp
  * exact there.  fp32 and bf16 input is scaled by a power of two that brings the largest value (of the row, or of 128
  * inputs) to 2^14 .. 2^15, and held as one fp16 value (bf16: exact from 2^-31 of the largest up) or as two, of which the
  * second is the 2^12-fold of what the first leaves (fp32: to 2^-23 of each value from 2^-28 of the largest up; the weights
- * that the second meets are 2^-12 times the others).  Values further below are left out there; each eight inputs that
- * have some are marked, and their products are added to the output at the end, one by one: an ordinary row has hardly any,
- * but an output whose weights avoid the large inputs would miss them.  Products are exact in the fp32 accumulators, which
+ * that the second meets are 2^-12 times the others).  Where values lie further apart some are left out there (the scale of a
+ * row is then the one under which most are held); each eight inputs that have such values are marked, and their products
+ * are added to the output at the end, one by one: an ordinary row has hardly any, but an output whose weights avoid the
+ * large inputs would miss the small ones.  Products are exact in the fp32 accumulators, which
  * a group starts from zero; its sum is then multiplied with the scale and added to the output's, the factors of the input
  * last: a factor times a scale may be below the normal range where the output is not.  Where a value is not finite the
  * factor that undoes the scaling is NaN.
@@ -220,15 +221,21 @@ struct q4_args {
     q4_shape s;
 };
 
-/* Input types whose values may be too far apart for the pieces, and the least that these take: what is below would be
- * subnormal in the first piece (fp32; the matrix instruction aligns its addends by their exponents, and takes that of a
- * subnormal factor as 2^-14), or lose bits (bf16). */
-template <int TI> struct q4_range { static constexpr bool wide = TI == DN_F32 || TI == DN_BF16; };
+/* Input types whose values may be too far apart for the pieces, and what these take: absolute values (as bits) from `least`
+ * on and below `most`.  What is below would be subnormal in the first piece (fp32; the matrix instruction aligns its
+ * addends by their exponents, and takes that of a subnormal factor as 2^-14), or lose bits (bf16). */
 template <int TI>
-__device__ __forceinline__ unsigned q4_least_held(float factor) /* as bits of the value itself */
-{
-    return __float_as_uint((TI == DN_F32 ? 0x1p-14f : 0x1p-17f) * factor);
-}
+struct q4_range {
+    static constexpr bool wide = TI == DN_F32 || TI == DN_BF16;
+    static constexpr int exponents = TI == DN_F32 ? 29 : 32;
+    unsigned least, most;
+    __device__ q4_range(float factor) : least(__float_as_uint((TI == DN_F32 ? 0x1p-14f : 0x1p-17f) * factor)), most(__float_as_uint(0x1p15f * factor)) {}
+    __device__ bool holds(float x) const /* 0 is not said to be held: it makes no difference */
+    {
+        const unsigned v = __float_as_uint(x) & 0x7fffffffu;
+        return v >= least && v < most;
+    }
+};
 
 /* The power of two that values are scaled by, from the largest of their absolute values' bits, and the factor that undoes
  * it: a power of two, NaN if a value is not finite.  fp16 input is not scaled down: it fits, and would lose its last bit. */
@@ -297,7 +304,7 @@ __device__ __forceinline__ unsigned q4_least8(unsigned m, const float x[8])
 template <int TI>
 __device__ __forceinline__ bool q4_below(unsigned least, float factor)
 {
-    return q4_range<TI>::wide && factor > 0 && least > 0u - q4_least_held<TI>(factor);
+    return q4_range<TI>::wide && factor > 0 && least > 0u - q4_range<TI>(factor).least;
 }
 
 /* The operand form of eight inputs, scaled by a power of two: hi, and 2^12 times what it leaves of the value in lo.
@@ -326,43 +333,57 @@ __device__ __forceinline__ float q4_split8(const float x[8], float scale, half8_
     return least;
 }
 
-/* Of eight inputs those that the pieces take. */
+/* Of eight inputs those that the pieces take.  Returns whether there are others. */
 template <int TI>
-__device__ __forceinline__ void q4_drop_below(float x[8], float factor)
+__device__ __forceinline__ bool q4_keep_held(float x[8], float factor)
 {
-    const unsigned least = q4_least_held<TI>(factor);
+    const q4_range<TI> range(factor);
+    bool others = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (__float_as_uint(x[i]) & 0x7fffffffu) < least ? 0.f : x[i];
+    for (int i = 0; i < 8; ++i) {
+        const bool holds = range.holds(x[i]);
+        others = others || (!holds && x[i] != 0);
+        x[i] = holds ? x[i] : 0.f;
+    }
+    return others;
 }
 
-/* What the pieces leave of row b's sum with output o: the small values of the eights that are marked, 16 bits for each
- * 128 inputs (eights without such values may be marked too).  mask(kb), factor(kb): of a block.  One thread's work, for the
- * few rows that need it. */
-template <int TI, class Mask, class Factor>
-__device__ __forceinline__ float q4_left_out(const q4_args &a, int b, int o, Mask mask, Factor factor)
+/* What the pieces leave of row b's sums with N outputs from o on: the values of marked eights that they do not hold.  Of
+ * blocks of 128 inputs: some(kb), whether one of eight from kb on has marks; marks(kb), 16 bits (eights that hold all may be
+ * marked too); factor(kb).  One thread's work, for the few rows that need it. */
+template <int TI, int N, class Some, class Marks, class Factor>
+__device__ __forceinline__ void q4_left_out(const q4_args &a, int b, int o, float (&sum)[N], Some some, Marks marks, Factor factor)
 {
     typedef typename dn_elt<TI>::store E;
     const E *row = (const E *)a.input + (long)b * a.s.inputs;
-    float sum = 0;
-#pragma unroll 1
-    for (int kb = 0; kb < a.s.kblocks; ++kb) {
-#pragma unroll 1
-        for (unsigned m = mask(kb); m; m &= m - 1) {
-            const int k = kb * 128 + (__ffs((int)m) - 1) * 8;
-            const unsigned least = q4_least_held<TI>(factor(kb));
-            float x[8];
-            q4_load8<TI>(row, k, a.s.inputs, x);
-            const unsigned codes = ((const unsigned *)a.packed)[q4_dword_at(a.s, o, k)];
-            const long g = q4_group_at(a.s, o, k / a.s.group);
-            const int zero = a.packed[a.s.zeros_at + g];
-            const float scale = ((const float *)(a.packed + a.s.scales_at))[g];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if ((__float_as_uint(x[i]) & 0x7fffffffu) < least)
-                    sum = fmaf(x[i], (float)((int)(codes >> q4_bit_of(i) & 15) - zero) * scale, sum);
+    for (int n = 0; n < N; ++n) sum[n] = 0;
+#pragma unroll 1
+    for (int kb0 = 0; kb0 < a.s.kblocks; kb0 += 8) {
+        if (!some(kb0)) continue;
+#pragma unroll 1
+        for (int kb = kb0; kb < min(kb0 + 8, a.s.kblocks); ++kb) {
+#pragma unroll 1
+            for (unsigned m = marks(kb); m; m &= m - 1) {
+                const int k = kb * 128 + (__ffs((int)m) - 1) * 8;
+                const q4_range<TI> range(factor(kb));
+                float x[8];
+                q4_load8<TI>(row, k, a.s.inputs, x);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = range.holds(x[i]) ? 0.f : x[i];
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    const int on = min(o + n, a.s.outputs - 1);
+                    const unsigned codes = ((const unsigned *)a.packed)[q4_dword_at(a.s, on, k)];
+                    const long g = q4_group_at(a.s, on, k / a.s.group);
+                    const int zero = a.packed[a.s.zeros_at + g];
+                    const float scale = ((const float *)(a.packed + a.s.scales_at))[g];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sum[n] = fmaf(x[i], (float)((int)(codes >> q4_bit_of(i) & 15) - zero) * scale, sum[n]);
+                }
+            }
         }
     }
-    return sum;
 }
 
 /* One tile of 16 outputs x 128 inputs as a lane holds it; PER groups in 128 inputs. */
@@ -437,7 +458,10 @@ __device__ __forceinline__ void q4_multiply(const q4_masks &masks, const q4_tile
 {
 #pragma unroll
     for (int g = 0; g < PER; ++g) {
-        float4_t acc[R][T];
+        /* the second piece has sums of its own (4 instructions for a group and tile of 16 rows, not 4 for each 8 weights of a
+         * lane: 64 x 4096 -> 32768 fp32 53.1 us, 55.4 with the weights multiplied; in groups of 32 60.7 and 58.0) */
+        constexpr int SUMS = PIECES == 2 && PER < 4 && R * T <= 4 ? 2 : 1;
+        float4_t part[SUMS][R][T], acc[R][T];
         half2_t z1024[R], z64[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) q4_zeros(w[r], g, z1024[r], z64[r]);
@@ -448,7 +472,7 @@ __device__ __forceinline__ void q4_multiply(const q4_masks &masks, const q4_tile
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 wv[r] = q4_unpack8(w[r].code[step], z1024[r], z64[r], masks);
-                if (PIECES == 2) wl[r] = wv[r] * (_Float16)Q4_LO; /* exact: 15 * 2^-12 at most, 2^-12 at least */
+                if (PIECES == 2 && SUMS == 1) wl[r] = wv[r] * (_Float16)Q4_LO; /* exact: 15 * 2^-12 at most, 2^-12 at least */
             }
 #pragma unroll
             for (int t = 0; t < T; ++t)
@@ -457,10 +481,15 @@ __device__ __forceinline__ void q4_multiply(const q4_masks &masks, const q4_tile
                     const half8_t x = operand(t, p, step);
 #pragma unroll
                     for (int r = 0; r < R; ++r)
-                        acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            x, p ? wl[r] : wv[r], i || p ? acc[r][t] : (float4_t){0, 0, 0, 0}, 0, 0, 0);
+                        part[p % SUMS][r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            x, p && SUMS == 1 ? wl[r] : wv[r], i || p >= SUMS ? part[p % SUMS][r][t] : (float4_t){0, 0, 0, 0}, 0, 0, 0);
                 }
         }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+                acc[r][t] = SUMS == 2 ? __builtin_elementwise_fma(part[SUMS - 1][r][t], (float4_t){Q4_LO, Q4_LO, Q4_LO, Q4_LO}, part[0][r][t]) : part[0][r][t];
 #pragma unroll
         for (int t = 0; t < T; ++t) {
             float4_t f = {1, 1, 1, 1};
@@ -565,7 +594,7 @@ __global__ __launch_bounds__(Q4_THREADS, 4) void q4_direct_kernel(q4_args a)
             }
             const float least = q4_split8(x[m], scale, hi, lo);
             if (q4_range<TI>::wide && least < 0x1p-14f && q4_below<TI>(q4_least8(0, x[m]), factor)) {
-                q4_drop_below<TI>(x[m], factor);
+                (void)q4_keep_held<TI>(x[m], factor);
                 (void)q4_split8(x[m], scale, hi, lo);
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); /* behind the write above, which is the same wave's */
                 factors[(at[m] >> 4) * 4 + of[m]] = -factor;
@@ -649,7 +678,9 @@ __global__ __launch_bounds__(Q4_THREADS, 4) void q4_direct_kernel(q4_args a)
                 for (int q = 0; q < WAVES; ++q) any |= s_below[q];
                 if (__builtin_expect(any != 0, 0)) {
                     auto factor = [&](int kb) { return -factors[kb * 4 + b]; };
-                    y += q4_left_out<TI>(a, b, o, [&](int kb) { return factor(kb) > 0 ? 0xffffu : 0u; }, factor);
+                    float left[1];
+                    q4_left_out<TI>(a, b, o, left, [](int) { return true; }, [&](int kb) { return factor(kb) > 0 ? 0xffffu : 0u; }, factor);
+                    y += left[0];
                 }
             }
             q4_store(a, b, o, y, bias);
@@ -660,7 +691,7 @@ __global__ __launch_bounds__(Q4_THREADS, 4) void q4_direct_kernel(q4_args a)
 /* ---- larger input, first pass: one workgroup for each row scales it and writes it in the order in which the second
  * pass feeds it to the matrix instruction: [row / 16][inputs / 128] blocks of [piece][step][lane][8 halves] and, for
  * 8-bit input with groups, [group in 128][16] factors.  Behind the blocks a factor for each row, negative (fp32 and bf16
- * input) where values lie below what the pieces hold; then [row][inputs / 128] the 16 bits of the eights that have
+ * input) where the pieces do not hold all values; then [row][inputs / 128, in eights] the 16 bits of the eights that have
  * such values, written for these rows only.  A pass over a few kilobytes, 3 to 5 us with its launch; it saves every
  * workgroup of the second pass a scaling of its own (16 rows of 8192 values read as they are by that pass, without this
  * one: the same time in groups of 128, 27 us against 20 in groups of 32).  1024 threads for long rows: 8 rows of 20787
@@ -677,7 +708,43 @@ __host__ __device__ static inline size_t q4_rows_at(const q4_shape &s, int piece
 
 __host__ __device__ static inline size_t q4_marks_at(const q4_shape &s, int pieces, int batch, bool groups)
 {
-    return q4_rows_at(s, pieces, batch, groups) + (size_t)batch * 4;
+    return (q4_rows_at(s, pieces, batch, groups) + (size_t)batch * 4 + 15) / 16 * 16;
+}
+__host__ __device__ static inline size_t q4_marks_pitch(const q4_shape &s) { return ((size_t)s.kblocks + 7) / 8 * 8; }
+
+/* The factor under which the pieces hold most of a row's values: of the runs of as many exponents as they hold the one
+ * with most values.  The whole workgroup. */
+template <int TI, int THREADS>
+__device__ __forceinline__ float q4_factor_for_most(const char *row, int inputs, float &scale)
+{
+    typedef unsigned long long u64;
+    __shared__ unsigned s_exponents[256];
+    __shared__ u64 s_best[THREADS / 64];
+    const int tid = threadIdx.x;
+    static_assert(THREADS >= 256, "a thread for each exponent");
+    if (tid < 256) s_exponents[tid] = 0;
+    __syncthreads();
+    for (int k = tid * 8; k < inputs; k += THREADS * 8) {
+        float x[8];
+        q4_load8<TI>(row, k, inputs, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (x[i] != 0) atomicAdd(&s_exponents[(__float_as_uint(x[i]) & 0x7fffffffu) >> 23], 1u);
+    }
+    __syncthreads();
+    u64 best = 0; /* the number of values, and the last exponent of the run */
+    if (tid < 255) {
+        for (int e = max(tid - q4_range<TI>::exponents + 1, 0); e <= tid; ++e) best += s_exponents[e];
+        best = best << 8 | (unsigned)tid;
+    }
+    best = dn_wave_max(best);
+    if ((tid & 63) == 0) s_best[tid >> 6] = best;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) best = best > s_best[w] ? best : s_best[w];
+    const int shift = min(141 - (int)(best & 255), 126); /* the values are below 2^(exponent - 126) */
+    scale = ldexpf(1.f, shift);
+    return ldexpf(1.f, -shift);
 }
 
 template <int TI, bool XG, int THREADS>
@@ -713,19 +780,21 @@ __global__ __launch_bounds__(THREADS) void q4_prepare_kernel(q4_args a)
         }
         scale = q4_scaling<TI>(m, factor);
         below = q4_below<TI>(least, factor);
+        if constexpr (q4_range<TI>::wide)
+            if (below) factor = q4_factor_for_most<TI, THREADS>(row, a.s.inputs, scale);
     }
     if (tid == 0)
         ((float *)(a.workspace + q4_rows_at(a.s, PIECES, a.batch, XG)))[b] = TI == DN_I8 ? (XG ? 1.f : q4_input_scale(a.input_scales + b)) : below ? -factor : factor;
     unsigned char *out = a.workspace + (size_t)(b >> 4) * a.s.kblocks * block + (b & 15) * 16;
+    unsigned short *marks = (unsigned short *)(a.workspace + q4_marks_at(a.s, PIECES, a.batch, XG)) + b * q4_marks_pitch(a.s);
+    if (q4_range<TI>::wide && below && tid < 8 && a.s.kblocks + tid < q4_marks_pitch(a.s)) marks[a.s.kblocks + tid] = 0;
     for (int k = tid * 8; k < a.s.kblocks * 128; k += THREADS * 8) {
         float x[8];
         half8_t hi, lo;
         q4_load8<TI>(row, k, a.s.inputs, x);
         if (q4_range<TI>::wide && below) { /* 16 lanes have a block */
-            const unsigned mark = (unsigned)(__ballot(q4_below<TI>(q4_least8(0, x), factor)) >> (tid & 48)) & 0xffffu;
-            if ((tid & 15) == 0)
-                ((unsigned short *)(a.workspace + q4_marks_at(a.s, PIECES, a.batch, XG)))[(size_t)b * a.s.kblocks + (k >> 7)] = (unsigned short)mark;
-            q4_drop_below<TI>(x, factor);
+            const unsigned mark = (unsigned)(__ballot(q4_keep_held<TI>(x, factor)) >> (tid & 48)) & 0xffffu;
+            if ((tid & 15) == 0) marks[k >> 7] = (unsigned short)mark;
         }
         q4_split8(x, scale, hi, lo);
         unsigned char *to = out + (size_t)(k >> 7) * block + ((k >> 5) & 3) * 1024 + ((k >> 3) & 3) * 256;
@@ -740,23 +809,31 @@ __global__ __launch_bounds__(THREADS) void q4_prepare_kernel(q4_args a)
     }
 }
 
-/* Whether a row has values that the pieces do not hold, and what they leave of its sum with an output. */
+/* Whether a row has values that the pieces do not hold, and what they leave of its sums with N outputs. */
 template <bool XG>
 __device__ __forceinline__ bool q4_is_below(const q4_args &a, float row_factor) { return !XG && a.ranged && row_factor < 0; }
 
-template <int PIECES>
-__device__ __forceinline__ float q4_left_out_of(const q4_args &a, float row_factor, int b, int o)
+template <int PIECES, int N>
+__device__ __forceinline__ void q4_left_out_of(const q4_args &a, float row_factor, int b, int o, float (&left)[N])
 {
-    const unsigned short *marks = (const unsigned short *)(a.workspace + q4_marks_at(a.s, PIECES, a.batch, false)) + (size_t)b * a.s.kblocks;
-    return q4_left_out<PIECES == 2 ? DN_F32 : DN_BF16>(a, b, o, [&](int kb) { return (unsigned)marks[kb]; }, [&](int) { return -row_factor; });
+    const unsigned short *marks = (const unsigned short *)(a.workspace + q4_marks_at(a.s, PIECES, a.batch, false)) + b * q4_marks_pitch(a.s);
+    q4_left_out<PIECES == 2 ? DN_F32 : DN_BF16>(
+        a, b, o, left,
+        [&](int kb) {
+            const uint4_t m = *(const uint4_t *)(marks + kb);
+            return (m[0] | m[1] | m[2] | m[3]) != 0;
+        },
+        [&](int kb) { return (unsigned)marks[kb]; }, [&](int) { return -row_factor; });
 }
 
 /* A sum with its row's factor. */
 template <int PIECES, bool XG>
 __device__ __forceinline__ float q4_scaled(const q4_args &a, float row_factor, int b, int o, float y)
 {
-    if (q4_is_below<XG>(a, row_factor)) return fmaf(y, -row_factor, q4_left_out_of<PIECES>(a, row_factor, b, o));
-    return y * row_factor;
+    if (!q4_is_below<XG>(a, row_factor)) return y * row_factor;
+    float left[1];
+    q4_left_out_of<PIECES>(a, row_factor, b, o, left);
+    return fmaf(y, -row_factor, left[0]);
 }
 
 /* A lane's results of one tile of outputs and 16 rows, with the rows' own factors. */
@@ -777,7 +854,7 @@ __device__ __forceinline__ void q4_store_tile(const q4_args &a, const float *row
 /* The same as one of several parts of the sums, which the next pass joins. */
 __host__ __device__ static inline size_t q4_parts_at(const q4_shape &s, int pieces, int batch, bool groups)
 {
-    return (q4_marks_at(s, pieces, batch, groups) + (size_t)batch * s.kblocks * 2 + 15) / 16 * 16;
+    return q4_marks_at(s, pieces, batch, groups) + batch * q4_marks_pitch(s) * 2;
 }
 
 __device__ __forceinline__ void q4_store_part(const q4_args &a, size_t parts_at, int tile, int b0, float4_t v)
@@ -1008,15 +1085,13 @@ __global__ __launch_bounds__(Q4_STAGED_WAVES * 64, 2) void q4_staged_kernel(q4_a
             const float f = s_factors[x * 16 + row];
             if (b >= a.batch || o >= a.s.outputs) continue;
             float4_t y = *(const float4_t *)(s_sum + row * PITCH + column);
-            if (q4_is_below<XG>(a, f))
-#pragma unroll 1
-                for (int i = 0; i < 4; ++i) {
-                    const float s = i == 0 ? y[0] : i == 1 ? y[1] : i == 2 ? y[2] : y[3];
-                    const float x = o + i < a.s.outputs ? q4_scaled<PIECES, XG>(a, f, b, o + i, s) + q4_bias(a, o + i) : 0.f;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) y[e] = i == e ? x : y[e];
-                }
-            else y = __builtin_elementwise_fma(y, (float4_t){f, f, f, f}, bias);
+            if (q4_is_below<XG>(a, f)) {
+                float left[4];
+                q4_left_out_of<PIECES>(a, f, b, o, left);
+                y = __builtin_elementwise_fma(y, (float4_t){-f, -f, -f, -f}, (float4_t){left[0], left[1], left[2], left[3]}) + bias;
+            } else {
+                y = __builtin_elementwise_fma(y, (float4_t){f, f, f, f}, bias);
+            }
             q4_store4(a, b, o, y);
         }
         __syncthreads();
