@@ -130,9 +130,9 @@ __device__ __forceinline__ void store_run(E *p, int i, int n, const float *v)
  *
  * The 8-bit form works on p = s * scales, exact in 64 bits: max|y| = max|p| * r, and code = rint(p * (r / c)).
  *
- * Bound by memory: 16384 x 4096 fp32 with residual, sum and output (1.07 GB) 187 us, 5.7 TB/s, where a copy reaches
- * 5.1; 4096 x 8192 bf16 likewise 60 us, 4.5 TB/s.  With 8-bit output in groups of 128 (236 MB) 54 us, 4.3 TB/s,
- * beside 600 vector instructions for 16 values a lane.  One row of 4096: 3 us, a launch. */
+ * Bound by memory: 16384 x 4096 fp32 with residual, sum and output (1.07 GB) 187 us, 5.7 TB/s, where a large copy reaches
+ * 5.1 and an addition 6.0; 4096 x 8192 bf16 likewise 60 us, 4.5 TB/s.  With 8-bit output in groups of 128 (236 MB) 54 us, 4.3 TB/s,
+ * beside 540 vector instructions for 16 values a lane.  One row of 4096: 3 us, a launch. */
 template <int T, int THREADS, int RUNS, int V, bool Q8>
 __global__ __launch_bounds__(THREADS) void rmsnorm_kernel(norm_args a)
 {

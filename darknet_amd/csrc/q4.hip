@@ -524,9 +524,11 @@ __device__ __forceinline__ float q4_bias(const q4_args &a, int o) { return a.bia
  * result with its own block is what counts.  So a workgroup has fewer outputs, and each operand that is read from LDS
  * serves H blocks; but a wave then reads pieces of 256 / H bytes, which costs more than it gives with many tiles.
  *
- * Measured, fp32 input: 4096 -> 4096 in groups of 128 5.2 us (1.7 TB/s; a launch that does nothing 3), 12544 -> 1715 in
- * groups of 32 8.4 us (1.7 TB/s), 25088 -> 4096 17.5 us (3.2 TB/s).  Of the second 4 us are the launch, the first loads
- * and the join, 1.5 the scaling of the input, the rest the weights: few CUs, each at what it can have in flight. */
+ * Measured, fp32 input: 4096 -> 4096 in groups of 128 5.4 us (1.7 TB/s; a launch that does nothing 3; 6.7 with weights
+ * that come from memory), 12544 -> 1715 in groups of 32 8.9 us (1.6 TB/s), 25088 -> 4096 17.8 us (3.1 TB/s); bf16, weights
+ * from memory: 8192 -> 28672 28 us, 4096 -> 131072 60 us (4.8 TB/s).  Of the second 4 us are the launch, the first loads
+ * and the join, 2 the scaling of the input, the rest the weights: few CUs, each at what it can have in flight.  A block
+ * of 128 values far below an outlier costs some 10 us more. */
 template <int TI, int PER, bool XG, int H>
 __global__ __launch_bounds__(Q4_THREADS, 4) void q4_direct_kernel(q4_args a)
 {
@@ -982,9 +984,9 @@ __device__ __forceinline__ void q4_store4(const q4_args &a, int b, int o, float4
  * needs them.
  *
  * Measured: 64 x 4096 -> 131072 bf16, groups of 128, fp32 output: 100 us, 3.2 TB/s and 690 TFLOP/s; its bytes alone
- * would take 64 us and its products 66.  A SIMD has two waves, and an instruction count of 40 us of vector and 27 us
- * of matrix instructions, which overlap in part.  Four row tiles a wave or three workgroups a CU gave nothing
- * (registers), one chunk on its way instead of two 117 us. */
+ * take 54 us at the rate of a large addition and its products 52 at that of a large product.  A SIMD has two waves, and an
+ * instruction count of 40 us of vector and 27 us of matrix instructions, which overlap in part.  One chunk on its way
+ * instead of two 117 us; four row tiles a wave or three workgroups a CU gave nothing. */
 #define Q4_STAGED_WAVES 4
 template <int T, int R, int PIECES, int PER, bool XG>
 __global__ __launch_bounds__(Q4_STAGED_WAVES * 64, 2) void q4_staged_kernel(q4_args a)
@@ -1100,14 +1102,15 @@ __global__ __launch_bounds__(Q4_STAGED_WAVES * 64, 2) void q4_staged_kernel(q4_a
 
 /* Which form a product takes (times of both sides, groups of 128):
  *   direct  at most 4 rows (the matrix instruction's rows and columns are laid out for that) which fit into LDS: one row
- *           25088 -> 4096 fp32 17.5 us, by the second pass below 31; four rows 4096 -> 4096 bf16 6.4 us against 8.7.
- *           The border is near: four rows of 18000 20.5 against 19.7.
+ *           25088 -> 4096 fp32 18.3 us, by the second pass below 29.4; four rows 4096 -> 4096 bf16 6.4 us against 8.8.
+ *           The border is rough: four rows of 18000 bf16 21.3 against 16.9.
  *   staged  so many tiles that workgroups of 4 or 8 of them fill the chip: its time hardly depends on their number
- *           up to there, while stream's grows with it.  64 x 4096 -> 11200 bf16 24.2 against 28.6 us, 8192 outputs
- *           (2048 tiles) 20.4 by stream; 32 x 4096 -> 22400 21.8 against 28.3; fp32 input 36.6 against 41.5
+ *           up to there, while stream's grows with it.  64 x 4096 -> 11200 (2800 tiles) bf16 25.2 against 31.3 us, fp32
+ *           36.1 and 46.9; 9216 (2304) 24.9 and 26.2, 36.0 and 40.1; 8192 (2048) 24.8 and 22.4, 35.9 and 34.4.  (Fewer
+ *           rows would have it lower: 32 x 4096 -> 16384, 2048 tiles, bf16 18.7 and 22.5.)
  *   stream  the others
- * Blocks (H): 12544 -> 1715 (108 tiles) 7.9 us by two, 9.7 by one; 160 tiles 11.0 by two, 10.0 by one; 63 tiles of
- * 8192 5.4 by four, 5.5 by two, 7.0 by one.
+ * Blocks (H): 12544 -> 1715 (108 tiles) 7.3 us by two, 9.5 by one; 160 tiles 10.1 by two, 9.6 by one; 63 tiles of
+ * 8192 5.3 by four, 5.7 by two, 7.2 by one.
  * Row tiles (R): staged 64 x 4096 -> 131072 100 us by two, 113 by one, no difference at 49152; stream 16 x 8192 -> 8192
  * 15.0 and 15.4. */
 struct q4_plan {

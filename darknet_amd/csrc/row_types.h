@@ -32,8 +32,7 @@ static inline bool dn_is_float_type(int type) { return type == DN_F32 || type ==
 static inline bool dn_aligned(const void *p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
 /* Reductions and running sums over the 64 lanes by data-parallel-primitive moves between registers (rows of 16
- * lanes, then row 0 to 1 and 2 to 3, then the lower half to the upper): a quarter of the time of the shuffles, which
- * go through the LDS crossbar.  All 64 lanes must be active.  Lanes without a source take `none`. */
+ * lanes, then row 0 to 1 and 2 to 3, then the lower half to the upper), which wait for no LDS as shuffles do.  All 64 lanes must be active.  Lanes without a source take `none`. */
 template <int CTRL, int ROWS>
 __device__ __forceinline__ unsigned dn_move(unsigned none, unsigned v)
 {

@@ -600,9 +600,9 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(sample_args a)
  * 3 borders from the bins; the kept mass of each block of tokens and each segment's candidates
  * 4 one workgroup a row: the prefix' end among the candidates, the block that the draw falls into, the token
  *
- * Measured: one row of 32768 fp32, top-k and top-p, 22 us (2, 4, 5 and 7 in the four); 64 rows of 131072 with settings of
- * all kinds 51 us (6, 15, 17, 10), with top-k alone 36.  A pass over the logits is 6 us at the memory's
- * rate; the second and third are bound by their instructions: a weight is 22 of 64 bits, the additions to 64-bit bins
+ * Measured: one row of 32768 fp32, top-k and top-p, 22 us (2, 4, 6 and 8 in the four); 64 rows of 131072 with settings of
+ * all kinds 51 us (7, 15, 17, 10).  A pass over the logits is 6 us at the memory's
+ * rate; the second and third are bound by their instructions: a weight is 23 of 64 bits, the additions to 64-bit bins
  * wait for each other, and a token of a bin that is kept is weighed twice rather than 8 bytes stored for each.  The
  * fourth is a chain of latencies. */
 #define SM_SPLIT_THREADS 256
