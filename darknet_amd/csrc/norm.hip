@@ -21,6 +21,7 @@ struct norm_args {
     float *q8_scales;
     int rows, n, group; /* group: values that share a scale, 0 = the row */
     float eps;
+    double inv_n;
 };
 
 /* Sum (or maximum) over the workgroup, the same bits on every lane and in every run. */
@@ -131,8 +132,8 @@ __device__ __forceinline__ void store_run(E *p, int i, int n, const float *v)
  * The 8-bit form works on p = s * scales, exact in 64 bits: max|y| = max|p| * r, and code = rint(p * (r / c)).
  *
  * Bound by memory: 16384 x 4096 fp32 with residual, sum and output (1.07 GB) 187 us, 5.7 TB/s, where a large copy reaches
- * 5.1 and an addition 6.0; 4096 x 8192 bf16 likewise 60 us, 4.5 TB/s.  With 8-bit output in groups of 128 (236 MB) 54 us, 4.3 TB/s,
- * beside 540 vector instructions for 16 values a lane.  One row of 4096: 3 us, a launch. */
+ * 5.1 and an addition 6.0; 4096 x 8192 bf16 likewise 50 us, 5.3 TB/s.  With 8-bit output in groups of 128 (236 MB) 50
+ * us, 4.7 TB/s, beside 540 vector instructions for 16 values a lane.  One row of 4096: 3 us, a launch. */
 template <int T, int THREADS, int RUNS, int V, bool Q8>
 __global__ __launch_bounds__(THREADS) void rmsnorm_kernel(norm_args a)
 {
@@ -185,7 +186,9 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_kernel(norm_args a)
             }
         }
         acc = block_all<THREADS, false>(acc, lds);
-        const double rms = sqrt(acc / n + (double)a.eps), r = 1. / rms;
+        double mean = acc * a.inv_n;
+        if (Q8 && acc <= 1.7976931348623157e308) mean = fma(fma(-mean, (double)n, acc), a.inv_n, mean); /* acc / n as it rounds */
+        const double rms = sqrt(mean + (double)a.eps), r = 1. / rms;
         auto values = [&](int j, float v[V]) {
             if (RUNS) {
 #pragma unroll
@@ -277,15 +280,14 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_kernel(norm_args a)
             }
         }
         if (a.output) {
-            const float rf = (float)r;
-            const bool ordinary = r >= 0x1p-100 && r <= 0x1p100; /* else r itself may leave the range of 32 bits */
+            /* in 64 bits: either product of two factors may leave the range of 32 where the result does not */
 #pragma unroll
             for (int j = 0; j < runs; ++j) {
                 float v[V], g[V];
                 values(j, v);
                 scales(j, g);
 #pragma unroll
-                for (int e = 0; e < V; ++e) v[e] = ordinary ? v[e] * rf * g[e] : (float)((double)v[e] * r * (double)g[e]);
+                for (int e = 0; e < V; ++e) v[e] = (float)((double)v[e] * r * (double)g[e]);
                 store_run<E, V>((E *)a.output + row * n, at(j), n, v);
             }
         }
@@ -293,10 +295,11 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_kernel(norm_args a)
 }
 
 /* Which form a row takes: one run a lane up to 256 lanes, then two, so that several rows share a CU and their loads
- * and stores overlap (2048 fp32 to 8 bits: 47 us by 256 lanes, 55 by 512; 8192 bf16: 60 by 512, 62 by 1024, 80 by 256 with
- * four), but for 16-bit rows of 257 to 512 runs of eight, whose two runs take the registers of a row more (4096 bf16: 27.7
- * by 512, 29.7 by 256).  768 lanes for what leaves a third of 1024 idle (3795 x 6000 fp32 71 us, 79 by 1024; 384 below 512
- * gave nothing).  A row of more than 16384 values is read again for each step. */
+ * and stores overlap (8192 bf16, 4096 rows: 50 us by 512 lanes with two, 58 by 1024 with one, 56 by 256 with four), but
+ * for 16-bit rows of 257 to 512 runs of eight, whose two runs take the registers of a row more (4096 bf16, 16384 rows with
+ * residual: 92 us by 512, 94 by 256; without one 55 and 51, and to 8 bits 123 and 103: there 256 would be ahead).  768
+ * lanes for what leaves a third of 1024 idle (3795 x 6000 fp32 69 us, 77 by 1024; bf16 43 and 54; 384 below 512 gave
+ * nothing).  A row of more than 16384 values is read again for each step. */
 template <int T, bool Q8>
 static void norm_launch(const norm_args &a)
 {
@@ -339,7 +342,7 @@ extern "C" int forward_rmsnorm_gpu(const void *input, const void *add, const flo
         !dn_aligned(scales, 4) || !dn_aligned(q8_scales, 4))
         return dn_refuse(me, "a buffer is not aligned to its element type");
     hip_require_device(me);
-    const norm_args a = {input, add, scales, sum_output, output, q8_output, q8_scales, rows, n, q8_group, eps};
+    const norm_args a = {input, add, scales, sum_output, output, q8_output, q8_scales, rows, n, q8_group, eps, 1. / n};
     if (type == DN_F32) q8_output ? norm_launch<DN_F32, true>(a) : norm_launch<DN_F32, false>(a);
     else if (type == DN_F16) q8_output ? norm_launch<DN_F16, true>(a) : norm_launch<DN_F16, false>(a);
     else q8_output ? norm_launch<DN_BF16, true>(a) : norm_launch<DN_BF16, false>(a);

@@ -168,6 +168,24 @@ def test_norm_codes_between_two_steps(dn, n, t):
             assert np.array_equal(c.get(), want) and np.array_equal(q.get(), codes), (rms, group, int((q.get() != codes).sum()))
 
 
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("n", [40, 1000, 20000])
+def test_norm_values_and_scales_of_all_sizes(dn, n, t):
+    """Elements far below their row with large scales, large rows with small scales: the result is within the range of
+    fp32, and right to two roundings, although a product on the way to it in 32 bits would not be."""
+    r = np.random.default_rng(n)
+    for size, small, scale in ((1.0, 1e-38, 1e6), (1e30, 1e-8, 1e-9), (1e-25, 1e-12, 1e20), (1e35, 1.0, 1e-30), (3e3, 1e-30, 1e12)):
+        x = (r.standard_normal((3, n)) * size).astype(np.float32)
+        x[:, r.random(n) < 0.5] *= np.float32(small)
+        bits, g = R.to_type(x, t), ((0.5 + r.random(n)) * scale).astype(np.float32)
+        bx, bg, out = Buffer(bits), Buffer(g), Buffer(shape=(3, n), dtype=bits.dtype)
+        assert dn.forward_rmsnorm_gpu(bx.ptr, None, bg.ptr, None, out.ptr, None, None, t, 3, n, 0, 0.0) == 0
+        dn.hip_synchronize()
+        _, y = R.rmsnorm(bits, None, g, 0.0, t)
+        tol = np.abs(y) * (R.HALF_STEP[t] + 4 * 2.0 ** -24) + R.HALF_TINY[t]
+        assert (np.abs(R.from_type(out.get(), t) - y) <= tol).all(), (size, small, scale)
+
+
 # ---- sampling --------------------------------------------------------------------------------
 def mass_bits(n):
     """The largest token's weight is 2^this in a row of n tokens."""
