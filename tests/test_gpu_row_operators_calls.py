@@ -1,5 +1,7 @@
 """Calls of the row operators that their documentation allows and other tests leave out: the least and the most rows and
 columns, few rows that are not ordinary, a workspace in use again, some activations, more rows than a grid has."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -147,3 +149,45 @@ def test_sample_more_rows_than_a_grid(dn, n):
     dn.hip_synchronize()
     assert np.array_equal(tok.get(), np.floor(u.astype(np.float64) * n).astype(np.int32))
     assert (np.abs(prob.get() - 1 / n) <= 2.0 ** -24 / n).all()
+
+
+@pytest.mark.parametrize("batch,k,n", [(3, 2000, 300), (6, 700, 90), (5, 8200, 60), (20, 300, 20000)])
+def test_q4_captured_rows_that_change_their_kind(dn, batch, k, n):
+    """A captured product replayed with ordinary rows, rows with outliers and rows of all sizes in turn, eager work between:
+    every replay gives the bits that the eager call gives, and they are right."""
+    group = 128
+    codes, scales, zeros = R.q4_codes(n, n, k, group)
+    m = Weights(dn, codes, scales, zeros, group)
+    r = np.random.default_rng(n)
+    kinds = [r.standard_normal((batch, k)).astype(np.float32) for _ in range(3)]
+    kinds[1][np.arange(batch), r.integers(0, k, batch)] = 1e15
+    kinds[2] *= (2.0 ** r.uniform(-90, 60, (batch, k))).astype(np.float32)
+    size = dn.connected_q4_workspace_bytes(F32, batch, k, n, group)
+    ws = Buffer(shape=(size,), dtype=np.uint8, shift=16) if size else None
+    x, out = Buffer(kinds[0]), Buffer(shape=(batch, n), dtype=np.float32)
+    call = lambda: dn.forward_connected_q4_gpu(x.ptr, F32, None, 0, m.packed.ptr, None, out.ptr, F32, batch, k, n, group, 3,  # noqa: E731
+                                               ws.ptr if ws else None)
+    hip = Hip()
+    st, graph, ex = hip.stream(), C.c_void_p(), C.c_void_p()
+    try:
+        dn.hip_set_stream(st)
+        hip.hipStreamBeginCapture(st, C.c_int(2))   # relaxed
+        assert call() == 0
+        hip.hipStreamEndCapture(st, C.byref(graph))
+        hip.hipGraphInstantiate(C.byref(ex), graph, None, None, C.c_size_t(0))
+        for rows in (kinds[i] for i in (1, 0, 2, 0, 1, 2)):
+            dn.hip_push_array(x.ptr, rows.ctypes.data_as(C.POINTER(C.c_float)), rows.size)
+            hip.hipGraphLaunch(ex, st)
+            hip.hipStreamSynchronize(st)
+            replayed = out.get()
+            v = rows.astype(np.float64)
+            y = v @ m.w.T
+            assert (np.abs(replayed - y) <= close(v, m.w, group, F32, F32, y)).all()
+            assert call() == 0
+            hip.hipStreamSynchronize(st)
+            assert np.array_equal(out.get(), replayed)
+    finally:
+        dn.hip_set_stream(None)
+    hip.hipGraphExecDestroy(ex)
+    hip.hipGraphDestroy(graph)
+    hip.hipStreamDestroy(st)
